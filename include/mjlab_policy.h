@@ -1,0 +1,64 @@
+/* mjlab_policy.h -- C ABI of the policy network's operators (mjlab_amd/csrc/libmjlab_policy.so).
+ *
+ * The environments of mjlab_amd.h return observation rows and take action rows; what lies between is a network of dense layers
+ * (reference src/mjlab/tasks/velocity/config/g1/rl_cfg.py:17-28: 512-256-128, ELU), gated layers and, for a memory over the control
+ * steps, linear attention with a decay per head whose state is cut where an environment was reset.  Forward and backward of each,
+ * hand-written for gfx950.
+ *
+ * Conventions of mjlab_amd.h: plain pointers and sizes, device memory owned by the caller, host structs passed by pointer, every call
+ * only ENQUEUES work on `stream` (a hipStream_t as void*), nothing synchronises, nothing is allocated.  Return value 0, or a hipError_t /
+ * negative library error with mjlab_policy_last_error() as its text (per thread).  Strides count elements.
+ */
+#ifndef MJLAB_POLICY_H_
+#define MJLAB_POLICY_H_
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define MJLAB_POLICY_ABI_VERSION 1
+
+enum { MJLAB_DTYPE_F32 = 0, MJLAB_DTYPE_F16 = 1, MJLAB_DTYPE_BF16 = 2 };
+enum { MJLAB_ACT_NONE = 0, MJLAB_ACT_RELU, MJLAB_ACT_ELU, MJLAB_ACT_TANH, MJLAB_ACT_SIGMOID, MJLAB_ACT_SILU, MJLAB_ACT_GELU, MJLAB_ACT_COUNT };
+
+int mjlab_policy_abi_version(void);
+const char* mjlab_policy_last_error(void);
+
+/* One layer over `rows` rows.
+ *   dense (w_up == NULL):  y = act(x w^T + b) + r
+ *   gated (w_up != NULL):  y = act(x w^T + b) * (x w_up^T + b_up)
+ * x (rows, in), w and w_up (out, in), b and b_up (out) or NULL, r (rows, out) or NULL (dense only), y (rows, out); the innermost stride of
+ * each is 1, ld* is the distance of rows.  All arrays hold `dtype`; sums are held in 32 bits and each output is rounded once.
+ * z / z_up (rows, out), dense, or NULL: the sums before the activation, which the backward pass reads. */
+typedef struct mjlab_layer {
+  int dtype, act;
+  long long rows, in, out;
+  const void *x, *w, *w_up, *b, *b_up, *r;
+  long long ldx, ldw, ldw_up, ldr, ldy;
+  void *y, *z, *z_up;
+} mjlab_layer_t;
+int mjlab_layer_forward(const mjlab_layer_t* f, void* stream);
+int mjlab_sizeof_layer(void);
+
+/* The backward pass of the layer `f` (x, w, w_up, z, z_up and the sizes are read; b, r, y are not) for the upstream gradient dy:
+ *   dense: dz = dy act'(z);                          dx = dz w;            dw = dz^T x;  db = sum over rows of dz
+ *   gated: dg = dy z_up act'(z), du = dy act(z);     dx = dg w + du w_up;  dw = dg^T x, dw_up = du^T x;  db, db_up likewise
+ * (the residual's gradient is dy itself).  A dense layer without activation needs no z.  Each output is dense and may be NULL (not wanted);
+ * dw / dw_up and db / db_up come together.  dz is rounded to `dtype`, since the matrix cores read it.  workspace: device memory of
+ * mjlab_layer_backward_workspace() bytes, free again when the launches have run. */
+typedef struct mjlab_layer_grad {
+  mjlab_layer_t f;
+  const void* dy;
+  long long ld_dy;
+  void *dx, *dw, *dw_up, *db, *db_up;
+  void* workspace;
+  long long workspace_bytes;
+} mjlab_layer_grad_t;
+long long mjlab_layer_backward_workspace(const mjlab_layer_grad_t* g); /* -1: bad arguments */
+int mjlab_layer_backward(const mjlab_layer_grad_t* g, void* stream);
+int mjlab_sizeof_layer_grad(void);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* MJLAB_POLICY_H_ */

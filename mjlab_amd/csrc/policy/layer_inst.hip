@@ -1,0 +1,139 @@
+// layer_inst.hip -- the layers' launches for ONE element type: compiled with -DMJLAB_POLICY_DTYPE=<0 f32 | 1 f16 | 2 bf16> (mjlab_amd/native.py).
+#include "product.h"
+#include "policy_launch.h"
+
+#if MJLAB_POLICY_DTYPE == 0
+using T = float;
+#define POLICY_NAME(x) x##_f32
+#elif MJLAB_POLICY_DTYPE == 1
+using T = _Float16;
+#define POLICY_NAME(x) x##_f16
+#else
+using T = __bf16;
+#define POLICY_NAME(x) x##_bf16
+#endif
+
+namespace {
+
+constexpr int CUS = 256;
+constexpr long long MAX_BLOCKS = (1LL << 24) - 1;  // of 256 threads: a launch counts its threads in 32 bits
+
+template <bool AK, bool BK, int BM, int BN, int EPI> hipError_t launch_tile(const Product& p, int splits, hipStream_t st) {
+  using TA = Tile<T, AK, BM>;
+  using TB = Tile<T, BK, BN>;
+  constexpr int BNO = EPI == EPI_GATED ? BN / 2 : BN;
+  constexpr int EPILOGUE = 4 * 32 * (BN / 2 + 4) * 4, LDS = 2 * (TA::BYTES + TB::BYTES) > EPILOGUE ? 2 * (TA::BYTES + TB::BYTES) : EPILOGUE;
+  const long long tiles = ((p.M + BM - 1) / BM) * ((p.N + BNO - 1) / BNO);
+  if (tiles > MAX_BLOCKS) return hipErrorInvalidValue;
+  auto kern = k_product<T, AK, BK, BM, BN, EPI>;
+  if (LDS > 64 * 1024) {
+    hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(kern, dim3((unsigned)tiles, (unsigned)splits), dim3(256), LDS, st, p);
+  return hipGetLastError();
+}
+
+// 128 x 128 tiles where they fill the device, else 64 x 64.
+template <bool AK, bool BK, int EPI> hipError_t launch_product(const Product& p, int splits, hipStream_t st) {
+  const long long nout = EPI == EPI_GATED ? 2 * p.N : p.N;
+  const long long big = ((p.M + 127) / 128) * ((nout + 127) / 128) * splits;
+  return big >= CUS ? launch_tile<AK, BK, 128, 128, EPI>(p, splits, st) : launch_tile<AK, BK, 64, 64, EPI>(p, splits, st);
+}
+
+// How many ways the sum over the rows is split in dw = dz^T x: few tiles, many rows.
+int weight_splits(long long out, long long in, long long rows) {
+  const long long tiles = ((out + 127) / 128) * ((in + 127) / 128);
+  const long long most = (rows + 255) / 256, want = (2 * CUS + tiles - 1) / tiles;
+  const long long s = want < most ? want : most;
+  return (int)(s < 1 ? 1 : s);
+}
+
+long long up256(long long x) { return (x + 255) & ~255LL; }
+
+struct Plan {
+  bool gated, slope, sums, weights;
+  long long ns, blocks, o_dz, o_sums, o_partial, bytes;
+  int splits;
+};
+
+Plan plan(const mjlab_layer_grad_t* g) {
+  const mjlab_layer_t& f = g->f;
+  Plan q;
+  q.gated = f.w_up != nullptr;
+  q.ns = q.gated ? 2 : 1;
+  q.slope = q.gated || f.act != MJLAB_ACT_NONE;
+  q.sums = g->db != nullptr;
+  q.weights = g->dw != nullptr;
+  q.blocks = (f.rows + SLOPE_ROWS - 1) / SLOPE_ROWS;
+  q.splits = weight_splits(q.ns * f.out, f.in, f.rows);
+  long long at = 0;
+  q.o_dz = at;
+  if (q.slope) at += up256(f.rows * q.ns * f.out * (long long)sizeof(T));
+  q.o_sums = at;
+  if (q.sums) at += up256(q.blocks * q.ns * f.out * 4);
+  q.o_partial = at;
+  if (q.weights && (q.splits > 1 || q.gated)) at += up256((long long)q.splits * q.ns * f.out * f.in * 4);
+  q.bytes = at;
+  return q;
+}
+
+}  // namespace
+
+hipError_t POLICY_NAME(mjlab_launch_layer_forward)(const mjlab_layer_t* f, hipStream_t st) {
+  Product p = {};
+  p.A = f->x; p.lda = f->ldx; p.B = f->w; p.ldb = f->ldw; p.B2 = f->w_up; p.ldb2 = f->ldw_up;
+  p.M = f->rows; p.N = f->out; p.K = p.kb2 = p.ksplit = f->in;
+  p.act = f->act; p.b = f->b; p.b_up = f->b_up; p.r = f->r; p.ldr = f->ldr; p.y = f->y; p.ldy = f->ldy; p.z = f->z; p.z_up = f->z_up;
+  return f->w_up ? launch_product<true, true, EPI_GATED>(p, 1, st) : launch_product<true, true, EPI_LAYER>(p, 1, st);
+}
+
+long long POLICY_NAME(mjlab_layer_backward_bytes)(const mjlab_layer_grad_t* g) { return plan(g).bytes; }
+
+hipError_t POLICY_NAME(mjlab_launch_layer_backward)(const mjlab_layer_grad_t* g, hipStream_t st) {
+  const mjlab_layer_t& f = g->f;
+  const Plan q = plan(g);
+  char* ws = (char*)g->workspace;
+  T* dz = (T*)(ws + q.o_dz);
+  float *sums = q.sums ? (float*)(ws + q.o_sums) : nullptr, *partial = (float*)(ws + q.o_partial);
+  hipError_t e = hipSuccess;
+  if (q.slope || q.sums) {
+    constexpr int V = Elem<T>::VEC;
+    const long long colblocks = (f.out + 32 * V - 1) / (32 * V);
+    if (colblocks * q.blocks > MAX_BLOCKS) return hipErrorInvalidValue;
+    auto kern = q.gated ? k_layer_slope<T, true> : k_layer_slope<T, false>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(colblocks * q.blocks)), dim3(256), 0, st, (const T*)g->dy, g->ld_dy, (const T*)f.z, (const T*)f.z_up, q.slope ? dz : nullptr, sums, f.rows, f.out, (unsigned)colblocks, f.act);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    if (q.sums) {
+      const long long cols = q.ns * f.out;
+      hipLaunchKernelGGL(k_join_sums<T>, dim3((unsigned)((cols + 15) / 16)), dim3(256), 0, st, sums, (T*)g->db, (T*)g->db_up, f.out, cols, q.blocks);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+  }
+  const void* d = q.slope ? (const void*)dz : g->dy;
+  const long long ldd = q.slope ? q.ns * f.out : g->ld_dy;
+  if (g->dx) {
+    Product p = {};
+    p.A = d; p.lda = ldd; p.B = f.w; p.ldb = f.ldw; p.B2 = f.w_up; p.ldb2 = f.ldw_up;
+    p.M = f.rows; p.N = f.in; p.K = p.ksplit = q.ns * f.out; p.kb2 = f.out;
+    p.y = g->dx; p.ldy = f.in;
+    if ((e = launch_product<true, false, EPI_STORE>(p, 1, st)) != hipSuccess) return e;
+  }
+  if (g->dw) {
+    Product p = {};
+    p.A = d; p.lda = ldd; p.B = f.x; p.ldb = f.ldx;
+    p.M = q.ns * f.out; p.N = f.in; p.K = p.kb2 = f.rows;
+    p.ksplit = ((f.rows + q.splits - 1) / q.splits + 63) / 64 * 64;
+    const int splits = (int)((f.rows + p.ksplit - 1) / p.ksplit);
+    p.y = g->dw; p.ldy = f.in; p.partial = partial;
+    if (splits == 1 && !q.gated) return launch_product<false, false, EPI_STORE>(p, 1, st);
+    if ((e = launch_product<false, false, EPI_PARTIAL>(p, splits, st)) != hipSuccess) return e;
+    const long long n = f.out * f.in;
+    for (int u = 0; u < (q.gated ? 2 : 1); ++u) {
+      // (a gated layer's partials hold both matrices: 2 n floats per split)
+      hipLaunchKernelGGL(k_join_splits<T>, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, st, partial + u * n, (T*)(u ? g->dw_up : g->dw), n, q.ns * n, splits);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
+  }
+  return hipSuccess;
+}

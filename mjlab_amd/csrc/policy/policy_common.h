@@ -1,0 +1,84 @@
+// policy_common.h -- element types, matrix instructions and activations of the policy network's kernels (gfx950).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "../../../include/mjlab_policy.h"
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+
+// VEC: elements of a 16-byte chunk.
+template <typename T> struct Elem;
+template <> struct Elem<float> { static constexpr int DTYPE = MJLAB_DTYPE_F32, VEC = 4; };
+template <> struct Elem<_Float16> { static constexpr int DTYPE = MJLAB_DTYPE_F16, VEC = 8; };
+template <> struct Elem<__bf16> { static constexpr int DTYPE = MJLAB_DTYPE_BF16, VEC = 8; };
+
+template <typename T> struct alignas(16) Chunk {
+  T e[Elem<T>::VEC];
+};
+
+// 16 bytes from / to any element address: global memory takes unaligned 16-byte accesses here, so rows of odd length keep the wide path.
+template <typename T> __device__ __forceinline__ Chunk<T> load_chunk(const T* p) {
+  Chunk<T> c;
+  __builtin_memcpy(&c, p, 16);
+  return c;
+}
+template <typename T> __device__ __forceinline__ void store_chunk(T* p, const Chunk<T>& c) { __builtin_memcpy(p, &c, 16); }
+
+// the first `n` elements of a chunk (n <= 0: none), the rest zero
+template <typename T> __device__ __forceinline__ Chunk<T> load_part(const T* p, long long n) {
+  constexpr int V = Elem<T>::VEC;
+  if (n >= V) return load_chunk(p);
+  Chunk<T> c;
+#pragma unroll
+  for (int i = 0; i < V; ++i) c.e[i] = i < n ? p[i] : (T)0.f;
+  return c;
+}
+template <typename T> __device__ __forceinline__ void store_part(T* p, const Chunk<T>& c, long long n) {
+  constexpr int V = Elem<T>::VEC;
+  if (n >= V) { store_chunk(p, c); return; }
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (i < n) p[i] = c.e[i];
+}
+
+// ---- activations, in float.  NaN goes through every one of them.
+__device__ __forceinline__ float sigmoid_f(float z) { return 1.f / (1.f + __expf(-z)); }
+
+__device__ __forceinline__ float act_value(float z, int act) {
+  switch (act) {
+    case MJLAB_ACT_RELU: return z < 0.f ? 0.f : z;
+    case MJLAB_ACT_ELU: return z > 0.f ? z : expm1f(z);
+    case MJLAB_ACT_TANH: return tanhf(z);
+    case MJLAB_ACT_SIGMOID: return sigmoid_f(z);
+    case MJLAB_ACT_SILU: return z * sigmoid_f(z);
+    case MJLAB_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678f));
+    default: return z;
+  }
+}
+
+// Derivative at z.  Beyond |z| = 100 the derivative of each is its limit to all 24 bits: z is cut there, so that a z that 16 bits hold
+// as infinite gives the limit and not infinity times zero.
+__device__ __forceinline__ float act_slope(float z, int act) {
+  z = z > 100.f ? 100.f : (z < -100.f ? -100.f : z);
+  switch (act) {
+    case MJLAB_ACT_RELU: return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
+    case MJLAB_ACT_ELU: return z > 0.f ? 1.f : __expf(z);
+    case MJLAB_ACT_TANH: { const float t = tanhf(z); return 1.f - t * t; }
+    case MJLAB_ACT_SIGMOID: { const float s = sigmoid_f(z); return s * (1.f - s); }
+    case MJLAB_ACT_SILU: { const float s = sigmoid_f(z); return s * (1.f + z * (1.f - s)); }
+    case MJLAB_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+    default: return 1.f;
+  }
+}
+
+// Workgroup b of n: consecutive workgroups go to the eight XCDs in turn, each with an L2 of its own, so the index is dealt out such that
+// one XCD works on neighbouring tiles (which share operand rows).
+__device__ __forceinline__ long long xcd_tile(long long b, long long n) {
+  const long long per = n / 8, rest = n % 8, x = b % 8, i = b / 8;
+  return x * per + (x < rest ? x : rest) + i;
+}

@@ -112,8 +112,104 @@ json.dumps(dict(sorted(cone_choice.items())), indent=1) + "\n")
   return out
 
 
+# The policy network's operators (include/mjlab_policy.h): a library of its own, so that the physics library's code stays what it is.
+POLICY_LIB_PATH = Path(os.environ.get("MJLAB_POLICY_LIB", CSRC / "libmjlab_policy.so"))
+POLICY_CSRC = CSRC / "policy"
+POLICY_HEADER = Path(__file__).parents[1] / "include" / "mjlab_policy.h"
+POLICY_UNITS = ("layer_inst.hip",)  # compiled once per element type
+POLICY_ABI_VERSION = 1  # include/mjlab_policy.h MJLAB_POLICY_ABI_VERSION
+# packed fp32 instructions off: these kernels are written for plain ones
+POLICY_HIPCC_FLAGS = [*HIPCC_FLAGS, "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
+def _policy_sources() -> list[Path]:
+  return [POLICY_HEADER, *sorted(POLICY_CSRC.glob("*.h")), *sorted(POLICY_CSRC.glob("*.hip"))]
+
+
+def build_policy(force: bool = False, verbose: bool = False, jobs: int | None = None) -> Path:
+  """Compile libmjlab_policy.so for gfx950: policy.hip (C ABI) and each unit of POLICY_UNITS once per element type, in parallel, then one link."""
+  import fcntl
+  from concurrent.futures import ThreadPoolExecutor
+
+  out = POLICY_LIB_PATH
+  newest_src = max(p.stat().st_mtime for p in _policy_sources())
+  if out.exists() and not force and out.stat().st_mtime >= newest_src:
+    return out
+  hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+  objdir = CSRC / "build" / out.stem
+  objdir.mkdir(parents=True, exist_ok=True)
+  units = [(POLICY_CSRC / "policy.hip", objdir / "policy.o", [])]
+  units += [(POLICY_CSRC / u, objdir / f"{Path(u).stem}_{d}.o", [f"-DMJLAB_POLICY_DTYPE={d}"]) for u in POLICY_UNITS for d in (0, 1, 2)]
+
+  def run(cmd: list) -> None:
+    if verbose:
+      print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, stderr=subprocess.PIPE, text=True)
+    err = "\n".join(x for x in r.stderr.splitlines() if "packed-fp32-ops" not in x)  # the host pass does not know the feature: harmless
+    if err.strip():
+      print(err, flush=True)
+    r.check_returncode()
+
+  with open(objdir / ".build.lock", "w") as lock:
+    fcntl.flock(lock, fcntl.LOCK_EX)  # one builder at a time, like build()
+    if out.exists() and not force and out.stat().st_mtime >= newest_src:
+      return out
+    with ThreadPoolExecutor(max_workers=jobs or min(len(units), os.cpu_count() or 4)) as pool:
+      list(pool.map(lambda u: run([hipcc, *POLICY_HIPCC_FLAGS, *u[2], "-c", str(u[0]), "-o", str(u[1])]), units))
+    tmp = out.with_name(out.name + f".tmp{os.getpid()}")
+    run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", str(tmp), *[str(u[1]) for u in units]])
+    os.replace(tmp, out)
+  return out
+
+
 class NativeLibraryError(RuntimeError):
   pass
+
+
+_POLICY_LIB: ctypes.CDLL | None = None
+
+POLICY_SYMBOLS = ("mjlab_policy_abi_version", "mjlab_policy_last_error", "mjlab_layer_forward", "mjlab_sizeof_layer", "mjlab_layer_backward_workspace",
+                  "mjlab_layer_backward", "mjlab_sizeof_layer_grad")  # fmt: skip
+
+
+def policy_lib() -> ctypes.CDLL:
+  """The policy operators' library; raises NativeLibraryError (never falls back) when unavailable."""
+  global _POLICY_LIB
+  if _POLICY_LIB is not None:
+    return _POLICY_LIB
+  path = POLICY_LIB_PATH
+  stale = not path.exists() or ("MJLAB_POLICY_LIB" not in os.environ and shutil.which("hipcc") is not None
+                                and path.stat().st_mtime < max(p.stat().st_mtime for p in _policy_sources()))
+  if stale and not os.environ.get("MJLAB_AMD_NO_AUTOBUILD"):
+    try:
+      build_policy()
+    except Exception as e:  # noqa: BLE001
+      raise NativeLibraryError(f"could not build {path}: {e}") from e
+  if not path.exists():
+    raise NativeLibraryError(f"{path} is missing; run `python -c 'import __graft_entry__ as g; g.build()'`")
+  try:
+    L = ctypes.CDLL(str(path))
+  except OSError as e:
+    raise NativeLibraryError(f"could not load {path}: {e}") from e
+  vp = ctypes.c_void_p
+  L.mjlab_policy_last_error.restype = ctypes.c_char_p
+  L.mjlab_layer_forward.argtypes = [vp, vp]
+  L.mjlab_layer_backward_workspace.argtypes, L.mjlab_layer_backward_workspace.restype = [vp], ctypes.c_longlong
+  L.mjlab_layer_backward.argtypes = [vp, vp]
+  if L.mjlab_policy_abi_version() != POLICY_ABI_VERSION:
+    raise NativeLibraryError(f"{path}: ABI version {L.mjlab_policy_abi_version()}, this package speaks {POLICY_ABI_VERSION}; rebuild it")
+  from .policy_ops import Layer, LayerGrad  # (imported here: policy_ops imports this module)
+
+  for what, mine, theirs in (("mjlab_layer_t", ctypes.sizeof(Layer), L.mjlab_sizeof_layer()), ("mjlab_layer_grad_t", ctypes.sizeof(LayerGrad), L.mjlab_sizeof_layer_grad())):
+    if mine != theirs:
+      raise NativeLibraryError(f"{path}: sizeof({what}) is {theirs} in the library, {mine} in the Python mirror; rebuild the library")
+  _POLICY_LIB = L
+  return L
+
+
+def policy_check(rc: int, what: str) -> None:
+  if rc != 0:
+    raise RuntimeError(f"{what} failed: {policy_lib().mjlab_policy_last_error().decode()}")
 
 
 _LIB: ctypes.CDLL | None = None

@@ -1,0 +1,91 @@
+"""The policy operators' library without a GPU: symbols, struct mirrors, and every refusal of the C ABI (nothing is launched)."""
+
+import ctypes
+import re
+from pathlib import Path
+
+import pytest
+import torch
+
+from mjlab_amd import native, policy_ops
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+def test_exports_every_declared_symbol():
+  lib = native.policy_lib()
+  declared = set(re.findall(r"\b(mjlab_[a-z_]+)\s*\(", (ROOT / "include" / "mjlab_policy.h").read_text()))
+  assert declared == set(native.POLICY_SYMBOLS)
+  for sym in declared:
+    assert hasattr(lib, sym), sym
+  assert lib.mjlab_policy_abi_version() == native.POLICY_ABI_VERSION
+
+
+def test_no_cpu_fallback():
+  with pytest.raises(TypeError, match="no CPU fallback"):
+    policy_ops.dense(torch.zeros((2, 3)), torch.zeros((4, 3)))
+  with pytest.raises(TypeError, match="no CPU fallback"):
+    policy_ops.gated(torch.zeros((2, 3)), torch.zeros((4, 3)), torch.zeros((4, 3)))
+
+
+def _layer(**kw):
+  f = policy_ops.Layer()
+  vals = dict(dtype=0, act=1, rows=4, inp=8, out=3, x=64, w=64, ldx=8, ldw=8, y=64, ldy=3)  # (addresses that no refused call reads)
+  vals.update(kw)
+  for k, v in vals.items():
+    setattr(f, k, v)
+  return f
+
+
+@pytest.mark.parametrize("kw,text", [
+  (dict(dtype=3), "dtype"), (dict(act=7), "activation"), (dict(act=-1), "activation"), (dict(rows=0), "sizes"), (dict(inp=0), "sizes"), (dict(out=-1), "sizes"),
+  (dict(inp=1 << 30), "sizes"), (dict(x=None), "null x or w"), (dict(w=None), "null x or w"), (dict(y=None), "null y"), (dict(ldx=-8), "negative"),
+  (dict(ldy=2), "overlap"), (dict(w_up=64, ldw_up=8, r=64), "residual"), (dict(b_up=64), "b_up"), (dict(z_up=64), "z_up"),
+])  # fmt: skip
+def test_layer_forward_refuses(kw, text):
+  lib = native.policy_lib()
+  assert lib.mjlab_layer_forward(ctypes.byref(_layer(**kw)), None) < 0
+  assert text in lib.mjlab_policy_last_error().decode()
+  assert lib.mjlab_layer_forward(None, None) < 0
+
+
+@pytest.mark.parametrize("kw,text", [
+  (dict(dy=None), "null dy"), (dict(f=dict(z=None)), "(z)"), (dict(f=dict(w_up=64, ldw_up=8)), "z_up"),
+  (dict(f=dict(w_up=64, ldw_up=8, z_up=64), dw=64), "together"), (dict(workspace_bytes=16), "workspace"), (dict(workspace=None), "workspace"),
+  (dict(f=dict(rows=-1)), "sizes"),
+])  # fmt: skip
+def test_layer_backward_refuses(kw, text):
+  lib = native.policy_lib()
+  g = policy_ops.LayerGrad()
+  kw = dict(kw)
+  g.f = _layer(**{"z": 64, **kw.pop("f", {})})
+  vals = dict(dy=64, ld_dy=3, dx=64, workspace=64, workspace_bytes=1 << 30)
+  vals.update(kw)
+  for k, v in vals.items():
+    setattr(g, k, v)
+  assert lib.mjlab_layer_backward(ctypes.byref(g), None) < 0
+  assert text in lib.mjlab_policy_last_error().decode()
+
+
+def test_workspace_covers_what_the_backward_pass_stores():
+  lib = native.policy_lib()
+  for dtype, size in ((0, 4), (1, 2), (2, 2)):
+    for gated in (False, True):
+      g = policy_ops.LayerGrad()
+      g.f = _layer(dtype=dtype, rows=5000, inp=70, out=33, **(dict(w_up=64, ldw_up=70) if gated else {}))
+      g.dw, g.db = 64, 64
+      pairs = 2 if gated else 1
+      need = lib.mjlab_layer_backward_workspace(ctypes.byref(g))
+      assert need >= 5000 * 33 * pairs * size + pairs * 33 * 4 * 40 + pairs * 33 * 70 * 4
+  g.f.rows = 0
+  assert lib.mjlab_layer_backward_workspace(ctypes.byref(g)) == -1
+
+
+def test_no_kernel_spills_ahead_of_its_exec_restore():
+  """As for the physics library: no spill store of the policy kernels may sit in front of an EXEC restore -- and no product kernel spills at all."""
+  from mjlab_amd import code_check
+
+  if not (code_check.LLVM / "llvm-objdump").exists():
+    pytest.skip("ROCm LLVM tools not installed")
+  native.policy_lib()
+  assert not code_check.fatal_hits(native.POLICY_LIB_PATH)
