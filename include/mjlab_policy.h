@@ -58,6 +58,52 @@ long long mjlab_layer_backward_workspace(const mjlab_layer_grad_t* g); /* -1: ba
 int mjlab_layer_backward(const mjlab_layer_grad_t* g, void* stream);
 int mjlab_sizeof_layer_grad(void);
 
+/* Linear attention with a decay per head.  Per sequence and head, with decay = exp(log_decay[head]) and keep_t = 0 where reset[t], else 1:
+ *   S_t = decay keep_t S_{t-1} + k_t v_t^T      (dk x dv, 32 bits)          o_t = scale * q_t S_t
+ * reset[t] means that token t is the first of an episode.  q, k (batch, length, heads, dk), v, o (batch, length, heads, dv) of `dtype`, any strides
+ * but 1 for the innermost; dk, dv <= MJLAB_DECAY_MAX_DIM.  state (the S before token 0; NULL = 0) and state_out (S after the last token; NULL =
+ * not wanted) are dense (batch, heads, dk, dv) floats and may be the same memory.  reset (batch, length) of reset_bytes 1 or 4 per element, non-zero =
+ * reset, or NULL.  lengths (batch) ints or NULL: sequence b ends before token lengths[b] (clamped to [0, length]); the rows of o behind it are
+ * written as zeros.  A NaN or infinity reaches only the tokens that the recurrence takes it to: not earlier ones, not other episodes.
+ * workspace: mjlab_decay_workspace() bytes of device memory. */
+#define MJLAB_DECAY_MAX_DIM 128
+typedef struct mjlab_decay_rows { const void* p; long long batch, time, head; } mjlab_decay_rows_t; /* strides in elements */
+typedef struct mjlab_decay {
+  int dtype, reset_bytes;
+  long long batch, length;
+  int heads, dk, dv;
+  float scale;
+  mjlab_decay_rows_t q, k, v, o; /* o.p is written */
+  const float* log_decay;        /* (heads) */
+  const float* state;
+  float* state_out;
+  const void* reset;
+  long long reset_batch, reset_time; /* strides of reset in elements */
+  const int* lengths;
+  void* workspace;
+  long long workspace_bytes;
+} mjlab_decay_t;
+long long mjlab_decay_workspace(const mjlab_decay_t* d); /* -1: bad arguments; the forward and the backward pass need the same */
+int mjlab_decay_forward(const mjlab_decay_t* d, void* stream);
+int mjlab_sizeof_decay(void);
+
+/* The backward pass for the upstream gradients `d_out` of o and `d_state_out` of state_out (NULL = 0):
+ *   dq_t = scale S_t do_t;   G_t = scale q_t do_t^T + decay keep_{t+1} G_{t+1} (after the last token: d_state_out);
+ *   dk_t = G_t v_t;  dv_t = G_t^T k_t;  d_state = decay keep_0 G_0
+ * dq, dk, dv: written (zeros behind a sequence's end), p NULL = not wanted; d_state dense, NULL = not
+ * wanted, else together with dv.  log_decay and scale are constants. */
+typedef struct mjlab_decay_grad {
+  mjlab_decay_t f; /* o, state_out are not used */
+  mjlab_decay_rows_t d_out, dq, dk, dv;
+  const float* d_state_out;
+  float* d_state;
+} mjlab_decay_grad_t;
+int mjlab_decay_backward(const mjlab_decay_grad_t* g, void* stream);
+int mjlab_sizeof_decay_grad(void);
+
+/* The recurrence for ONE token: length is 1 (the time strides are not read), state must be given, state_out may be `state` itself. */
+int mjlab_decay_step(const mjlab_decay_t* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

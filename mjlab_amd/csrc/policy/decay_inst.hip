@@ -1,0 +1,94 @@
+// decay_inst.hip -- the launches of linear attention with a decay for ONE element type (policy_type.h).
+#include "policy_type.h"
+#include "decay.h"
+
+namespace {
+
+struct Split {
+  int segments, seg_chunks;
+};
+
+// Segments per sequence: one where the sequences fill the device (a workgroup each), else as many as give it two workgroups per CU, of four chunks
+// at least: the first pass reads two of the operands again and moves R through memory once per segment.
+Split split(long long batch, int heads, long long length) {
+  constexpr int C = DecayCfg<T>::C;
+  const long long chunks = (length + C - 1) / C, rows = batch * heads;
+  if (rows >= CUS || chunks < 8) return {1, (int)chunks};
+  const long long want = (2 * CUS + rows - 1) / rows, most = chunks / 4, s = want < most ? want : most;
+  const long long per = (chunks + s - 1) / s;
+  return {(int)((chunks + per - 1) / per), (int)per};
+}
+
+long long up256(long long x) { return (x + 255) & ~255LL; }
+long long state_bytes(const mjlab_decay_t* d, const Split& s) { return up256(d->batch * d->heads * (s.segments - 1) * (long long)d->dk * d->dv * 4); }
+
+template <int DA, int DC> hipError_t launch_pass(const DecayPass& p, long long rows, hipStream_t st) {
+  constexpr int LDS = (int)sizeof(DecayLds<T, DA, DC>);
+  hipError_t e;
+  if (rows * p.segments > MAX_BLOCKS) return hipErrorInvalidValue;
+  if (p.segments > 1) {
+    auto first = k_decay_chunks<T, DA, DC, true>;
+    if ((e = allow_lds(first, LDS)) != hipSuccess) return e;
+    hipLaunchKernelGGL(first, dim3((unsigned)(rows * (p.segments - 1))), dim3(256), LDS, st, p);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    hipLaunchKernelGGL(k_decay_scan<T>, dim3((unsigned)(rows * ((p.da * p.dc + 255) / 256))), dim3(256), 0, st, p);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
+  auto kern = k_decay_chunks<T, DA, DC, false>;
+  if ((e = allow_lds(kern, LDS)) != hipSuccess) return e;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(rows * p.segments)), dim3(256), LDS, st, p);
+  return hipGetLastError();
+}
+
+template <int DA> hipError_t launch_dc(const DecayPass& p, long long rows, hipStream_t st) {
+  return p.dc <= 32 ? launch_pass<DA, 32>(p, rows, st) : p.dc <= 64 ? launch_pass<DA, 64>(p, rows, st) : launch_pass<DA, 128>(p, rows, st);
+}
+
+// out = the pass over a, b (heads of da) and c (of dc); see decay.h
+hipError_t launch(const mjlab_decay_t* d, const mjlab_decay_rows_t& a, const mjlab_decay_rows_t& b, const mjlab_decay_rows_t& c, const mjlab_decay_rows_t& out, int da,
+                  int dc, bool reverse, const float* state_in, bool turned, float* state_out, hipStream_t st) {
+  const Split s = split(d->batch, d->heads, d->length);
+  DecayPass p = {};
+  p.a = a.p; p.a_b = a.batch; p.a_t = a.time; p.a_h = a.head;
+  p.b = b.p; p.b_b = b.batch; p.b_t = b.time; p.b_h = b.head;
+  p.c = c.p; p.c_b = c.batch; p.c_t = c.time; p.c_h = c.head;
+  p.out = (void*)out.p; p.o_b = out.batch; p.o_t = out.time; p.o_h = out.head;
+  p.log_decay = d->log_decay;
+  p.state_in = state_in; p.in_r = turned ? 1 : dc; p.in_c = turned ? da : 1; p.state_out = state_out;
+  p.reset = d->reset; p.reset_bytes = d->reset_bytes; p.reset_b = d->reset_batch; p.reset_t = d->reset_time;
+  p.heads = d->heads; p.da = da; p.dc = dc; p.e0 = reverse ? 0 : 1; p.reverse = reverse; p.segments = s.segments; p.seg_chunks = s.seg_chunks;
+  p.length = d->length; p.lengths = d->lengths;
+  p.ps = d->scale; p.is = reverse ? 1.f : d->scale; p.us = reverse ? d->scale : 1.f;
+  p.seg_state = (float*)d->workspace; p.seg_factor = (float*)((char*)d->workspace + state_bytes(d, s));
+  const long long rows = d->batch * d->heads;
+  return da <= 32 ? launch_dc<32>(p, rows, st) : da <= 64 ? launch_dc<64>(p, rows, st) : launch_dc<128>(p, rows, st);
+}
+
+template <int LPR> hipError_t launch_step(const mjlab_decay_t* d, hipStream_t st) {
+  hipLaunchKernelGGL((k_decay_step<T, LPR>), dim3((unsigned)(d->batch * d->heads)), dim3(256), 0, st, *d);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+long long POLICY_NAME(mjlab_decay_bytes)(const mjlab_decay_t* d) {
+  const Split s = split(d->batch, d->heads, d->length);
+  return s.segments > 1 ? state_bytes(d, s) + up256(d->batch * d->heads * (s.segments - 1) * 4) : 0;
+}
+
+hipError_t POLICY_NAME(mjlab_launch_decay_forward)(const mjlab_decay_t* d, hipStream_t st) {
+  return launch(d, d->q, d->k, d->v, d->o, d->dk, d->dv, false, d->state, false, d->state_out, st);
+}
+
+hipError_t POLICY_NAME(mjlab_launch_decay_backward)(const mjlab_decay_grad_t* g, hipStream_t st) {
+  const mjlab_decay_t* d = &g->f;
+  hipError_t e;
+  if (g->dq.p && (e = launch(d, g->d_out, d->v, d->k, g->dq, d->dv, d->dk, false, d->state, true, nullptr, st)) != hipSuccess) return e;
+  if (g->dk.p && (e = launch(d, d->v, g->d_out, d->q, g->dk, d->dv, d->dk, true, g->d_state_out, true, nullptr, st)) != hipSuccess) return e;
+  if (g->dv.p && (e = launch(d, d->k, d->q, g->d_out, g->dv, d->dk, d->dv, true, g->d_state_out, false, g->d_state, st)) != hipSuccess) return e;
+  return hipSuccess;
+}
+
+hipError_t POLICY_NAME(mjlab_launch_decay_step)(const mjlab_decay_t* d, hipStream_t st) {
+  return d->dv <= 32 ? launch_step<8>(d, st) : d->dv <= 64 ? launch_step<16>(d, st) : launch_step<32>(d, st);
+}

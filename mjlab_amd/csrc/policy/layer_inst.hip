@@ -1,22 +1,8 @@
 // layer_inst.hip -- the layers' launches for ONE element type: compiled with -DMJLAB_POLICY_DTYPE=<0 f32 | 1 f16 | 2 bf16> (mjlab_amd/native.py).
+#include "policy_type.h"
 #include "product.h"
-#include "policy_launch.h"
-
-#if MJLAB_POLICY_DTYPE == 0
-using T = float;
-#define POLICY_NAME(x) x##_f32
-#elif MJLAB_POLICY_DTYPE == 1
-using T = _Float16;
-#define POLICY_NAME(x) x##_f16
-#else
-using T = __bf16;
-#define POLICY_NAME(x) x##_bf16
-#endif
 
 namespace {
-
-constexpr int CUS = 256;
-constexpr long long MAX_BLOCKS = (1LL << 24) - 1;  // of 256 threads: a launch counts its threads in 32 bits
 
 template <bool AK, bool BK, int BM, int BN, int EPI> hipError_t launch_tile(const Product& p, int splits, hipStream_t st) {
   using TA = Tile<T, AK, BM>;
@@ -26,10 +12,7 @@ template <bool AK, bool BK, int BM, int BN, int EPI> hipError_t launch_tile(cons
   const long long tiles = ((p.M + BM - 1) / BM) * ((p.N + BNO - 1) / BNO);
   if (tiles > MAX_BLOCKS) return hipErrorInvalidValue;
   auto kern = k_product<T, AK, BK, BM, BN, EPI>;
-  if (LDS > 64 * 1024) {
-    hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
-    if (e != hipSuccess) return e;
-  }
+  if (hipError_t e = allow_lds(kern, LDS); e != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3((unsigned)tiles, (unsigned)splits), dim3(256), LDS, st, p);
   return hipGetLastError();
 }

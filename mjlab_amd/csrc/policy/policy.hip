@@ -65,4 +65,57 @@ int mjlab_layer_backward(const mjlab_layer_grad_t* g, void* stream) {
   return done(BY_TYPE(g->f.dtype, mjlab_launch_layer_backward, g, (hipStream_t)stream), "layer_backward launch failed");
 }
 
+static int check_decay(const mjlab_decay_t& d) {
+  if (bad_type(d.dtype)) return fail(-2, "decay: unknown dtype");
+  if (d.batch < 1 || d.heads < 1 || d.length < 1 || d.batch >= (1LL << 31) || d.length >= (1LL << 31) || d.batch * d.heads >= (1LL << 24)) return fail(-2, "decay: batch, length and heads must be positive (batch x heads below 2^24)");
+  if (d.dk < 1 || d.dv < 1 || d.dk > MJLAB_DECAY_MAX_DIM || d.dv > MJLAB_DECAY_MAX_DIM) return fail(-2, "decay: dk and dv must be in [1, MJLAB_DECAY_MAX_DIM]");
+  if (!d.q.p || !d.k.p || !d.v.p || !d.log_decay) return fail(-2, "decay: null q, k, v or log_decay");
+  if (d.reset && d.reset_bytes != 1 && d.reset_bytes != 4) return fail(-2, "decay: reset_bytes must be 1 or 4");
+  return 0;
+}
+
+int mjlab_sizeof_decay(void) { return (int)sizeof(mjlab_decay_t); }
+int mjlab_sizeof_decay_grad(void) { return (int)sizeof(mjlab_decay_grad_t); }
+
+long long mjlab_decay_workspace(const mjlab_decay_t* d) {
+  if (!d) return fail(-1, "decay_workspace: null argument");
+  if (check_decay(*d)) return -1;
+  return BY_TYPE(d->dtype, mjlab_decay_bytes, d);
+}
+
+static int check_decay_workspace(const mjlab_decay_t& d) {
+  const long long need = BY_TYPE(d.dtype, mjlab_decay_bytes, &d);
+  return need > 0 && (!d.workspace || d.workspace_bytes < need) ? fail(-3, "decay: workspace too small") : 0;
+}
+
+int mjlab_decay_forward(const mjlab_decay_t* d, void* stream) {
+  if (!d) return fail(-1, "decay_forward: null argument");
+  int rc = check_decay(*d);
+  if (rc) return rc;
+  if (!d->o.p) return fail(-2, "decay_forward: null o");
+  if (d->state && d->state == d->state_out) return fail(-2, "decay_forward: state_out must not be state");
+  if ((rc = check_decay_workspace(*d))) return rc;
+  return done(BY_TYPE(d->dtype, mjlab_launch_decay_forward, d, (hipStream_t)stream), "decay_forward launch failed");
+}
+
+int mjlab_decay_backward(const mjlab_decay_grad_t* g, void* stream) {
+  if (!g) return fail(-1, "decay_backward: null argument");
+  int rc = check_decay(g->f);
+  if (rc) return rc;
+  if (!g->d_out.p) return fail(-2, "decay_backward: null d_out");
+  if (g->d_state && (!g->dv.p || g->d_state == g->d_state_out)) return fail(-2, "decay_backward: d_state comes with dv and must not be d_state_out");
+  if ((rc = check_decay_workspace(g->f))) return rc;
+  return done(BY_TYPE(g->f.dtype, mjlab_launch_decay_backward, g, (hipStream_t)stream), "decay_backward launch failed");
+}
+
+int mjlab_decay_step(const mjlab_decay_t* d, void* stream) {
+  if (!d) return fail(-1, "decay_step: null argument");
+  int rc = check_decay(*d);
+  if (rc) return rc;
+  if (d->length != 1) return fail(-2, "decay_step: length must be 1");
+  if (!d->o.p || !d->state || !d->state_out) return fail(-2, "decay_step: null o, state or state_out");
+  if (d->lengths) return fail(-2, "decay_step: lengths do not apply to one token");
+  return done(BY_TYPE(d->dtype, mjlab_launch_decay_step, d, (hipStream_t)stream), "decay_step launch failed");
+}
+
 }  // extern "C"

@@ -116,7 +116,7 @@ json.dumps(dict(sorted(cone_choice.items())), indent=1) + "\n")
 POLICY_LIB_PATH = Path(os.environ.get("MJLAB_POLICY_LIB", CSRC / "libmjlab_policy.so"))
 POLICY_CSRC = CSRC / "policy"
 POLICY_HEADER = Path(__file__).parents[1] / "include" / "mjlab_policy.h"
-POLICY_UNITS = ("layer_inst.hip",)  # compiled once per element type
+POLICY_UNITS = ("layer_inst.hip", "decay_inst.hip")  # compiled once per element type
 POLICY_ABI_VERSION = 1  # include/mjlab_policy.h MJLAB_POLICY_ABI_VERSION
 # packed fp32 instructions off: these kernels are written for plain ones
 POLICY_HIPCC_FLAGS = [*HIPCC_FLAGS, "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
@@ -169,7 +169,8 @@ class NativeLibraryError(RuntimeError):
 _POLICY_LIB: ctypes.CDLL | None = None
 
 POLICY_SYMBOLS = ("mjlab_policy_abi_version", "mjlab_policy_last_error", "mjlab_layer_forward", "mjlab_sizeof_layer", "mjlab_layer_backward_workspace",
-                  "mjlab_layer_backward", "mjlab_sizeof_layer_grad")  # fmt: skip
+                  "mjlab_layer_backward", "mjlab_sizeof_layer_grad", "mjlab_decay_workspace", "mjlab_decay_forward", "mjlab_decay_backward", "mjlab_decay_step",
+                  "mjlab_sizeof_decay", "mjlab_sizeof_decay_grad")  # fmt: skip
 
 
 def policy_lib() -> ctypes.CDLL:
@@ -195,12 +196,15 @@ def policy_lib() -> ctypes.CDLL:
   L.mjlab_policy_last_error.restype = ctypes.c_char_p
   L.mjlab_layer_forward.argtypes = [vp, vp]
   L.mjlab_layer_backward_workspace.argtypes, L.mjlab_layer_backward_workspace.restype = [vp], ctypes.c_longlong
-  L.mjlab_layer_backward.argtypes = [vp, vp]
+  for name in ("mjlab_layer_backward", "mjlab_decay_forward", "mjlab_decay_backward", "mjlab_decay_step"):
+    getattr(L, name).argtypes = [vp, vp]
+  L.mjlab_decay_workspace.argtypes, L.mjlab_decay_workspace.restype = [vp], ctypes.c_longlong
   if L.mjlab_policy_abi_version() != POLICY_ABI_VERSION:
     raise NativeLibraryError(f"{path}: ABI version {L.mjlab_policy_abi_version()}, this package speaks {POLICY_ABI_VERSION}; rebuild it")
-  from .policy_ops import Layer, LayerGrad  # (imported here: policy_ops imports this module)
+  from .policy_ops import Decay, DecayGrad, Layer, LayerGrad  # (imported here: policy_ops imports this module)
 
-  for what, mine, theirs in (("mjlab_layer_t", ctypes.sizeof(Layer), L.mjlab_sizeof_layer()), ("mjlab_layer_grad_t", ctypes.sizeof(LayerGrad), L.mjlab_sizeof_layer_grad())):
+  for what, mine, theirs in (("mjlab_layer_t", ctypes.sizeof(Layer), L.mjlab_sizeof_layer()), ("mjlab_layer_grad_t", ctypes.sizeof(LayerGrad), L.mjlab_sizeof_layer_grad()),
+                             ("mjlab_decay_t", ctypes.sizeof(Decay), L.mjlab_sizeof_decay()), ("mjlab_decay_grad_t", ctypes.sizeof(DecayGrad), L.mjlab_sizeof_decay_grad())):
     if mine != theirs:
       raise NativeLibraryError(f"{path}: sizeof({what}) is {theirs} in the library, {mine} in the Python mirror; rebuild the library")
   _POLICY_LIB = L

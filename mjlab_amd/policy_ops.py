@@ -2,9 +2,11 @@
 
   dense(x, weight, bias, activation, residual)   y = act(x W^T + b) + r
   gated(x, weight, weight_up, ...)               y = act(x W^T + b) * (x W_up^T + b_up)
+  decay_attention(q, k, v, log_decay, ...)       S_t = decay S_{t-1} + k_t v_t^T, o_t = scale q_t S_t over stored steps, S cut at resets
+  decay_attention_step(q, k, v, log_decay, state, ...)  the same for one control step
 
-``x`` has any leading dimensions and its last one is the layer's input; float32, float16 or bfloat16, the same type everywhere, sums in 32
-bits, each output rounded once.  Both are differentiable in every tensor argument (once).  Every call enqueues on torch's current stream of
+float32, float16 or bfloat16, the same type everywhere, sums and states in 32 bits, each output rounded once.  The first three are
+differentiable (once) in every tensor argument but log_decay.  Every call enqueues on torch's current stream of
 the tensors' device and may be captured into a hipGraph; nothing synchronises.  The last dimension of an argument must be contiguous, rows may
 be any distance apart.  No fallback: without the HIP library, or for a tensor that is not on the GPU, these raise.
 
@@ -34,6 +36,21 @@ class Layer(ctypes.Structure):  # mjlab_layer_t
 class LayerGrad(ctypes.Structure):  # mjlab_layer_grad_t
   _fields_ = [("f", Layer), ("dy", _vp), ("ld_dy", _ll), ("dx", _vp), ("dw", _vp), ("dw_up", _vp), ("db", _vp), ("db_up", _vp),
               ("workspace", _vp), ("workspace_bytes", _ll)]  # fmt: skip
+
+
+class Rows(ctypes.Structure):  # mjlab_decay_rows_t
+  _fields_ = [("p", _vp), ("batch", _ll), ("time", _ll), ("head", _ll)]
+
+
+class Decay(ctypes.Structure):  # mjlab_decay_t
+  _fields_ = [("dtype", ctypes.c_int), ("reset_bytes", ctypes.c_int), ("batch", _ll), ("length", _ll), ("heads", ctypes.c_int), ("dk", ctypes.c_int),
+              ("dv", ctypes.c_int), ("scale", ctypes.c_float), ("q", Rows), ("k", Rows), ("v", Rows), ("o", Rows), ("log_decay", _vp), ("state", _vp),
+              ("state_out", _vp), ("reset", _vp), ("reset_batch", _ll), ("reset_time", _ll), ("lengths", _vp), ("workspace", _vp),
+              ("workspace_bytes", _ll)]  # fmt: skip
+
+
+class DecayGrad(ctypes.Structure):  # mjlab_decay_grad_t
+  _fields_ = [("f", Decay), ("d_out", Rows), ("dq", Rows), ("dk", Rows), ("dv", Rows), ("d_state_out", _vp), ("d_state", _vp)]
 
 
 def _stream(dev: torch.device) -> int:
@@ -214,3 +231,179 @@ def _check_out(what: str, out: torch.Tensor, like: torch.Tensor, shape: tuple, o
     others = (*others, same_as)
   if any(t is not None and _overlap(out, t) for t in (like, *others)):
     raise ValueError(f"{what}: out overlaps an input")
+
+
+MAX_HEAD_DIM = 128  # MJLAB_DECAY_MAX_DIM
+
+
+def _decay_arguments(what: str, q, k, v, log_decay, state, reset, lead: tuple) -> None:
+  """Checks shared by the chunked form (lead = batch, length) and the step (lead = batch)."""
+  if q.dtype not in DTYPES or not q.is_cuda:
+    raise TypeError(f"{what}: q must be a float32, float16 or bfloat16 device tensor, got {q.dtype} on {q.device} (there is no CPU fallback)")
+  h, dk = q.shape[-2:]
+  _check(k, f"{what}: k", q, (*lead, h, dk))
+  if v.dim() != q.dim():
+    raise ValueError(f"{what}: v must have the dimensions of q, got {tuple(v.shape)}")
+  dv = v.shape[-1]
+  _check(q, f"{what}: q", q, (*lead, h, dk))
+  _check(v, f"{what}: v", q, (*lead, h, dv))
+  if h < 1 or not 1 <= dk <= MAX_HEAD_DIM or not 1 <= dv <= MAX_HEAD_DIM:
+    raise ValueError(f"{what}: at least one head, and head sizes in [1, {MAX_HEAD_DIM}], got {h} heads of {dk} and {dv}")
+  if log_decay.dtype != torch.float32 or log_decay.device != q.device or tuple(log_decay.shape) != (h,) or not log_decay.is_contiguous():
+    raise ValueError(f"{what}: log_decay must be a contiguous float32 tensor ({h},) on {q.device}, got {log_decay.dtype} {tuple(log_decay.shape)} on {log_decay.device}")
+  if log_decay.requires_grad:
+    raise ValueError(f"{what}: the decays are constants; log_decay must not require gradients")
+  if state is not None and (state.dtype != torch.float32 or state.device != q.device or tuple(state.shape) != (lead[0], h, dk, dv) or not state.is_contiguous()):
+    raise ValueError(f"{what}: state must be a contiguous float32 tensor {(lead[0], h, dk, dv)} on {q.device}, got {state.dtype} {tuple(state.shape)} on {state.device}")
+  if reset is not None and (reset.dtype not in (torch.bool, torch.uint8, torch.int32) or reset.device != q.device or tuple(reset.shape) != lead):
+    raise ValueError(f"{what}: reset must be a bool, uint8 or int32 tensor {lead} on {q.device}, got {reset.dtype} {tuple(reset.shape)} on {reset.device}")
+
+
+def _decay_struct(q, k, v, log_decay, scale: float, state, reset, lengths) -> Decay:
+  """q, k, v: (batch, length, heads, d)."""
+  d = Decay()
+  d.dtype, d.scale = DTYPES[q.dtype], scale
+  d.batch, d.length, d.heads, d.dk = q.shape
+  d.dv = v.shape[3]
+  d.q, d.k, d.v = _strided(q), _strided(k), _strided(v)
+  d.log_decay = log_decay.data_ptr()
+  d.state = None if state is None else state.data_ptr()
+  if reset is not None:
+    d.reset, d.reset_bytes, d.reset_batch, d.reset_time = reset.data_ptr(), reset.element_size(), reset.stride(0), reset.stride(1)
+  d.lengths = None if lengths is None else lengths.data_ptr()
+  return d
+
+
+def _strided(t: torch.Tensor) -> Rows:
+  return Rows(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+
+def _rows_like(t: torch.Tensor, d: int) -> torch.Tensor:
+  """A new (batch, length, heads, d) tensor with the batch and time axes in memory in the order they have in `t`."""
+  b, n, h, _ = t.shape
+  return t.new_empty((n, b, h, d)).transpose(0, 1) if b > 1 and n > 1 and t.stride(1) > t.stride(0) else t.new_empty((b, n, h, d))
+
+
+def _decay_launch(fn: str, struct: ctypes.Structure, d: Decay, dev: torch.device) -> None:
+  lib = native.policy_lib()
+  need = lib.mjlab_decay_workspace(ctypes.byref(d))
+  native.policy_check(min(0, need), "mjlab_decay_workspace")
+  ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+  if need:
+    d.workspace, d.workspace_bytes = ws.data_ptr(), need
+  if struct is not d:
+    struct.f = d
+  with torch.cuda.device(dev):
+    native.policy_check(getattr(lib, fn)(ctypes.byref(struct), _stream(dev)), fn)
+
+
+def _decay_forward(q, k, v, state, log_decay, scale, reset, lengths):
+  b, n, h, dk = q.shape
+  o = _rows_like(q, v.shape[3])
+  if b == 0 or n == 0:
+    final = q.new_zeros((b, h, dk, v.shape[3]), dtype=torch.float32) if state is None else state.clone()
+    return o, final
+  final = torch.empty((b, h, dk, v.shape[3]), dtype=torch.float32, device=q.device)
+  d = _decay_struct(q, k, v, log_decay, scale, state, reset, lengths)
+  d.o, d.state_out = _strided(o), final.data_ptr()
+  _decay_launch("mjlab_decay_forward", d, d, q.device)
+  return o, final
+
+
+class _DecayAttention(torch.autograd.Function):
+  @staticmethod
+  def forward(ctx, q, k, v, state, log_decay, scale, reset, lengths):
+    ctx.save_for_backward(q, k, v, state, log_decay, reset, lengths)
+    ctx.scale = scale
+    ctx.set_materialize_grads(False)
+    return _decay_forward(q, k, v, state, log_decay, scale, reset, lengths)
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, do, dfinal):
+    q, k, v, state, log_decay, reset, lengths = ctx.saved_tensors
+    need_q, need_k, need_v, need_s = ctx.needs_input_grad[:4]
+    if do is None and dfinal is None:
+      return (None,) * 8
+    b, n, h, dk = q.shape
+    if b == 0 or n == 0:
+      ds = None
+      if need_s:
+        ds = torch.zeros_like(state) if dfinal is None else dfinal
+      return tuple(torch.zeros_like(t) if need else None for t, need in ((q, need_q), (k, need_k), (v, need_v))) + (ds, None, None, None, None)
+    if do is None:
+      do = torch.zeros((1, 1, 1, v.shape[3]), dtype=q.dtype, device=q.device).expand(b, n, h, v.shape[3])
+    elif v.shape[3] > 1 and do.stride(3) != 1:
+      do = do.contiguous()
+    dfinal = None if dfinal is None else dfinal.contiguous()
+    g = DecayGrad()
+    dq = _rows_like(q, dk) if need_q else None
+    dk_ = _rows_like(k, dk) if need_k else None
+    dv = _rows_like(v, v.shape[3]) if need_v or need_s else None
+    ds = torch.empty_like(state) if need_s else None
+    for name, t in (("d_out", do), ("dq", dq), ("dk", dk_), ("dv", dv)):
+      if t is not None:
+        setattr(g, name, _strided(t))
+    g.d_state_out = None if dfinal is None else dfinal.data_ptr()
+    g.d_state = None if ds is None else ds.data_ptr()
+    _decay_launch("mjlab_decay_backward", g, _decay_struct(q, k, v, log_decay, ctx.scale, state, reset, lengths), q.device)
+    return dq, dk_, dv if need_v else None, ds, None, None, None, None
+
+
+def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, scale: float | None = None, state: torch.Tensor | None = None,
+                    reset: torch.Tensor | None = None, lengths: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+  """Linear attention with a decay per head over stored steps -> (o (batch, length, heads, dv), final state (batch, heads, dk, dv) float32).
+
+  q, k (batch, length, heads, dk), v (batch, length, heads, dv): any strides with a contiguous last dimension, so a time-major rollout buffer goes in
+  as ``buffer.transpose(0, 1)``.  ``log_decay`` (heads,) float32, constants (<= 0; a positive one grows).  ``scale`` defaults to dk ** -0.5.  ``state``: what
+  was carried into the first step (zeros if None).  ``reset`` (batch, length), non-zero where a step is the first of an episode: nothing is carried into
+  it.  ``lengths`` (batch,) int32: sequence b ends before step lengths[b]; o is zero behind it and the final state is the one at its end.  A NaN or
+  infinity of one step does not reach earlier steps or other episodes."""
+  if q.dim() != 4:
+    raise ValueError(f"decay_attention: q must be (batch, length, heads, dk), got {tuple(q.shape)}")
+  lead = tuple(q.shape[:2])
+  _decay_arguments("decay_attention", q, k, v, log_decay, state, reset, lead)
+  if lengths is not None and (lengths.dtype != torch.int32 or lengths.device != q.device or tuple(lengths.shape) != lead[:1] or not lengths.is_contiguous()):
+    raise ValueError(f"decay_attention: lengths must be a contiguous int32 tensor {lead[:1]} on {q.device}, got {lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
+  scale = q.shape[3] ** -0.5 if scale is None else float(scale)
+  if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
+    return _DecayAttention.apply(q, k, v, state, log_decay, scale, reset, lengths)
+  return _decay_forward(q, k, v, state, log_decay, scale, reset, lengths)
+
+
+def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor, scale: float | None = None,
+                         reset: torch.Tensor | None = None, out: torch.Tensor | None = None, out_state: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+  """One control step of the same recurrence -> (o (batch, heads, dv), state).  q, k (batch, heads, dk), v (batch, heads, dv); ``state`` (batch, heads, dk, dv) float32 is
+  updated in place, or left alone and written to ``out_state``.  ``reset`` (batch,): non-zero where the environment was reset before this step (what
+  PhysicsRollout.step() returned).  No gradients: an update replays stored steps through decay_attention()."""
+  if q.dim() != 3:
+    raise ValueError(f"decay_attention_step: q must be (batch, heads, dk), got {tuple(q.shape)}")
+  b, h, dk = q.shape
+  _decay_arguments("decay_attention_step", q, k, v, log_decay, state, reset, (b,))
+  dv = v.shape[2]
+  if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+    raise ValueError("decay_attention_step takes no part in a graph of gradients: call it under torch.no_grad()")
+  if out_state is None:
+    out_state = state
+  elif out_state is not state:
+    if out_state.dtype != torch.float32 or out_state.device != q.device or out_state.shape != state.shape or not out_state.is_contiguous():
+      raise ValueError("decay_attention_step: out_state must be like state")
+    if out_state.data_ptr() != state.data_ptr() and _overlap(out_state, state):
+      raise ValueError("decay_attention_step: out_state overlaps state")
+  if any(_overlap(out_state, t) for t in (q, k, v)):
+    raise ValueError("decay_attention_step: the state overlaps an input")
+  if out is None:
+    out = q.new_empty((b, h, dv))
+  else:
+    _check_out("decay_attention_step", out, q, (b, h, dv), (k, v, state, out_state))
+  if b:
+    d = Decay()
+    d.dtype, d.scale = DTYPES[q.dtype], dk**-0.5 if scale is None else float(scale)
+    d.batch, d.length, d.heads, d.dk, d.dv = b, 1, h, dk, dv
+    d.q, d.k, d.v, d.o = (Rows(t.data_ptr(), t.stride(0), 0, t.stride(1)) for t in (q, k, v, out))
+    d.log_decay, d.state, d.state_out = log_decay.data_ptr(), state.data_ptr(), out_state.data_ptr()
+    if reset is not None:
+      d.reset, d.reset_bytes, d.reset_batch = reset.data_ptr(), reset.element_size(), reset.stride(0)
+    with torch.cuda.device(q.device):
+      native.policy_check(native.policy_lib().mjlab_decay_step(ctypes.byref(d), _stream(q.device)), "mjlab_decay_step")
+  return out, out_state

@@ -81,6 +81,58 @@ def test_workspace_covers_what_the_backward_pass_stores():
   assert lib.mjlab_layer_backward_workspace(ctypes.byref(g)) == -1
 
 
+def _decay(**kw):
+  d = policy_ops.Decay()
+  vals = dict(dtype=0, batch=2, length=5, heads=2, dk=8, dv=8, scale=1.0, log_decay=64, state=64, state_out=128)
+  rows = {n: policy_ops.Rows(64, 80, 16, 8) for n in ("q", "k", "v", "o")}
+  for n, p in kw.items():
+    if n in rows:
+      rows[n].p = p
+    else:
+      vals[n] = p
+  for n, val in {**vals, **rows}.items():
+    setattr(d, n, val)
+  return d
+
+
+@pytest.mark.parametrize("kw,text", [
+  (dict(dtype=5), "dtype"), (dict(batch=0), "positive"), (dict(length=0), "positive"), (dict(heads=0), "positive"), (dict(batch=1 << 23, heads=2), "positive"),
+  (dict(dk=129), "dk and dv"), (dict(dv=0), "dk and dv"), (dict(q=None), "null q"), (dict(v=None), "null q"), (dict(log_decay=None), "log_decay"),
+  (dict(reset=64, reset_bytes=2), "reset_bytes"), (dict(o=None), "null o"), (dict(state=128), "state_out"), (dict(length=5000), "workspace"),
+])  # fmt: skip
+def test_decay_forward_refuses(kw, text):
+  lib = native.policy_lib()
+  assert lib.mjlab_decay_forward(ctypes.byref(_decay(**kw)), None) < 0
+  assert text in lib.mjlab_policy_last_error().decode()
+  assert lib.mjlab_decay_forward(None, None) < 0
+
+
+@pytest.mark.parametrize("kw,text", [(dict(), "length"), (dict(length=1, state=None), "null o"), (dict(length=1, state_out=None), "null o"), (dict(length=1, lengths=64), "lengths")])
+def test_decay_step_refuses(kw, text):
+  lib = native.policy_lib()
+  assert lib.mjlab_decay_step(ctypes.byref(_decay(**kw)), None) < 0
+  assert text in lib.mjlab_policy_last_error().decode()
+
+
+def test_decay_backward_refuses():
+  lib = native.policy_lib()
+  g = policy_ops.DecayGrad()
+  g.f = _decay()
+  assert lib.mjlab_decay_backward(ctypes.byref(g), None) < 0 and "d_out" in lib.mjlab_policy_last_error().decode()
+  g.d_out, g.d_state = policy_ops.Rows(64, 80, 16, 8), 64
+  assert lib.mjlab_decay_backward(ctypes.byref(g), None) < 0 and "d_state" in lib.mjlab_policy_last_error().decode()
+  g.f.length = 100000
+  g.d_state = None
+  assert lib.mjlab_decay_backward(ctypes.byref(g), None) < 0 and "workspace" in lib.mjlab_policy_last_error().decode()
+
+
+def test_decay_workspace_grows_only_where_sequences_are_split():
+  lib = native.policy_lib()
+  assert lib.mjlab_decay_workspace(ctypes.byref(_decay(length=24, batch=4096))) == 0
+  assert lib.mjlab_decay_workspace(ctypes.byref(_decay(length=8192, batch=4096))) == 0
+  assert lib.mjlab_decay_workspace(ctypes.byref(_decay(length=8192))) >= 4 * 8 * 8 * 4
+
+
 def test_no_kernel_spills_ahead_of_its_exec_restore():
   """As for the physics library: no spill store of the policy kernels may sit in front of an EXEC restore -- and no product kernel spills at all."""
   from mjlab_amd import code_check
