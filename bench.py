@@ -189,6 +189,9 @@ def main() -> None:
                   "interleaved (mjlab_amd.dist.pingpong_steps; key `pipelined`).  `value` is always the plain synchronous exchange")
   ap.add_argument("--cone", choices=["pyramidal", "elliptic"], default="pyramidal",
                   help="friction cone of the compiled model (the tasks configure pyramidal: the headline workload; elliptic = the cone variants of the kernels, an experiment line)")
+  ap.add_argument("--policy", choices=["mlp", "memory"], default=None,
+                  help="actions from a policy network (randomly initialised, 512-256-128) inside the captured control step instead of random ones: "
+                  "an experiment line, not the headline workload (N = 1; memory: two blocks of linear attention with a decay)")
   ap.add_argument("--no-cpu-baseline", action="store_true")
   ap.add_argument("--no-latency-bound", action="store_true", help="skip the one-wave-per-SIMD launch that measures roofline.latency")
   ap.add_argument("--no-big-batch", action="store_true", help="skip the 16 384-world leg (value_at_16384)")
@@ -234,8 +237,16 @@ def main() -> None:
 
     roll.readback = EntityReadback(sim)
   step_graph = not args.no_graph and not args.no_step_graph
+  policy = None
+  if args.policy:
+    if info.world_size != 1 or not step_graph:
+      raise SystemExit("--policy: one GPU, with the control step captured")
+    from mjlab_amd.policy import Policy, PolicyCfg
+
+    torch.manual_seed(args.seed)
+    policy = Policy(PolicyCfg(roll.observation_rows().shape[1], model.nu, memory_blocks=2 if args.policy == "memory" else 0), dev)
   if step_graph:
-    roll.capture_graph()
+    roll.capture_graph(policy)
   exchange = (info.world_size > 1 or bool(os.environ.get("MJLAB_DIST_FORCE"))) and not args.no_gather
   nu = model.nu
   learner_gen = torch.Generator(device=dev)
@@ -251,7 +262,7 @@ def main() -> None:
       a_all = torch.rand((info.global_envs, nu), device=dev, generator=learner_gen) * 2 - 1 if info.rank == 0 else None
       action = mdist.scatter_actions(info, a_all, nu, dev)
     else:
-      action = roll.random_action(out=roll.action_buffer)
+      action = roll.random_action(out=roll.action_buffer) if policy is None else None
     if args.balance_every and roll.control_kernel:
       if step_no[0] % args.balance_every == 0:
         roll.balance_worlds()
@@ -667,7 +678,7 @@ def main() -> None:
       "scaling": "weak",
       "vs_baseline": None,
       "dtype": "f32",
-      "data": "synthetic (random actions, " + ("resets to random phases of a synthetic 10 s motion (SURVEY 8d(4)) with the task's pose / velocity / joint noise" if "motion" in events else "keyframe resets")
+      "data": ("synthetic (random actions, " if policy is None else f"synthetic (actions of a randomly initialised policy, {args.policy}, ") + ("resets to random phases of a synthetic 10 s motion (SURVEY 8d(4)) with the task's pose / velocity / joint noise" if "motion" in events else "keyframe resets")
       + ("" if args.no_task_events else ", per-env foot friction U(0.3,1.2), velocity pushes every U(1,3) s") + "; compiled model from the reference MJCF)",
       "config": {
         "workload": f"{args.scene}: {args.envs_per_gpu} envs/GPU, timestep 0.005, decimation 4, Newton 10 it / 20 ls "

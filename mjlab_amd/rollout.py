@@ -338,6 +338,8 @@ class PhysicsRollout:
       time_left = lo_t + (hi_t - lo_t) * torch.rand((n,), device=dev, generator=self.gen)
       self.push = (float(lo_t), float(hi_t), rng6, time_left)
     self._graph: torch.cuda.CUDAGraph | None = None
+    self._policy = None  # the policy whose control step capture_graph() recorded
+    self._memory: dict = {}  # a policy's memory of these environments (Policy.initial_state), by policy
     self._action_buf: torch.Tensor | None = None
     self._obs_buf: torch.Tensor | None = None
     # load balance of the control kernel (mjlab_control_t.world_order): see balance_worlds()
@@ -375,6 +377,8 @@ class PhysicsRollout:
   def reset_all(self) -> None:
     d = self.sim.data
     n = self.sim.num_envs
+    for _, memory in self._memory.values():
+      memory.zero_()
     if self.motion is not None:
       torch.rand(self.motion["rnd"].shape, device=self.key_qpos.device, generator=self.gen, out=self.motion["rnd"])
       t_new = self._motion_rows()
@@ -391,27 +395,34 @@ class PhysicsRollout:
     d.qacc_warmstart[:] = 0.0
     self.sim.forward()
 
-  def step(self, action: torch.Tensor) -> torch.Tensor:
-    """One control step; returns the reset mask of shape ``(num_envs,)``: int32 (non-zero = reset) with the fused
+  def step(self, action: torch.Tensor | None = None) -> torch.Tensor:
+    """One control step (``action`` None: the policy's that capture_graph(policy) recorded); returns the
+    reset mask of shape ``(num_envs,)``: int32 (non-zero = reset) with the fused
     reset -- the array the library wrote, no conversion launch -- and bool with ``fused_reset=False``.
 
     With ``capture_graph()`` done, the whole control step -- action processing, the
     ``decimation`` physics steps, termination test, masked reset and the forward pass -- is
     ONE hipGraph replay (resets are mask based, so there is no
     ``nonzero()`` host sync and nothing data dependent on the host side)."""
+    if (action is None) != (self._graph is not None and self._policy is not None):
+      raise ValueError("step(): an action is needed, unless the captured control step has a policy, which then decides it")
     self._nstep = getattr(self, "_nstep", 0) + 1
     if self._nstep % 16 == 0:  # wave-priority classes follow the batch (a few small device ops, outside the graph)
       self.sim.update_priority_thresholds()
     if self._graph is not None:
-      if action is not self._action_buf:  # random_action(out=...) / a policy may write the static buffer directly
+      if action is not None and action is not self._action_buf:  # random_action(out=...) / a policy may write the static buffer directly
         self._action_buf.copy_(action)
       self._graph.replay()
       return self._reset_buf
     return self._step_eager(action)
 
-  def capture_graph(self) -> None:
+  def capture_graph(self, policy=None) -> None:
     """Capture one control step into a hipGraph (the physics kernels are launched directly
-    inside the capture, not through the Simulation's own step/forward graphs)."""
+    inside the capture, not through the Simulation's own step/forward graphs).  With a ``policy``
+    (mjlab_amd.policy.Policy) the graph begins with its action: observation rows -> network -> physics, then
+    ``step()`` takes no action.  Its parameters are read at every replay, so an update in place takes effect."""
+    self._graph = None
+    self._policy = policy
     n = self.sim.num_envs
     dev = self.key_qpos.device
     self._action_buf = torch.zeros((n, self.m.nu), device=dev)
@@ -435,6 +446,8 @@ class PhysicsRollout:
       self.sim.use_graph = sim_graph
 
   def _capture_body(self) -> None:
+    if self._policy is not None:
+      self.policy_action(self._policy, out=self._action_buf)
     r = self._step_eager(self._action_buf)
     if r is not self._reset_buf:
       self._reset_buf.copy_(r)
@@ -515,6 +528,8 @@ class PhysicsRollout:
         self.motion["time_steps"].copy_(torch.where(reset, t_new, self.motion["time_steps"].long() + 1).to(torch.int32))
       d.qacc_warmstart[:] = torch.where(rm, torch.zeros_like(d.qacc_warmstart), torch.nan_to_num(d.qacc_warmstart))
       self.episode_length.copy_(torch.where(reset, torch.zeros_like(self.episode_length), self.episode_length))
+      if self._memory:  # a policy's memory is cut by the mask at its next step
+        self._reset_mask.copy_(reset)
     self.sim.forward(reset if self.masked_forward else None)
     if self.push is not None:  # interval events come after the reset's forward() (manager_based_rl_env.py:134-137)
       lo_t, hi_t, rng6, time_left = self.push
@@ -558,6 +573,16 @@ class PhysicsRollout:
     if out is None:
       out = torch.empty((self.sim.num_envs, self.m.nu), device=self.key_qpos.device)
     return out.uniform_(-1.0, 1.0, generator=self.gen)
+
+  def policy_action(self, policy, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The action of a ``policy`` (mjlab_amd.policy.Policy) at the present observation rows; ``out=self.action_buffer`` writes the captured graph's input in
+    place.  A policy with memory carries one state per environment here, cut where the last control step reset it, emptied by reset_all()."""
+    memory = None
+    if policy.cfg.memory_blocks:
+      if id(policy) not in self._memory:
+        self._memory[id(policy)] = (policy, policy.initial_state(self.sim.num_envs))
+      memory = self._memory[id(policy)][1]
+    return policy.act(self.observation_rows(), state=memory, reset=self._reset_mask, out=out)
 
   @property
   def action_buffer(self) -> torch.Tensor | None:
