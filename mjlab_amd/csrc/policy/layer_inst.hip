@@ -5,10 +5,7 @@
 namespace {
 
 template <bool AK, bool BK, int BM, int BN, int EPI> hipError_t launch_tile(const Product& p, int splits, hipStream_t st) {
-  using TA = Tile<T, AK, BM>;
-  using TB = Tile<T, BK, BN>;
-  constexpr int BNO = EPI == EPI_GATED ? BN / 2 : BN;
-  constexpr int EPILOGUE = 4 * 32 * (BN / 2 + 4) * 4, LDS = 2 * (TA::BYTES + TB::BYTES) > EPILOGUE ? 2 * (TA::BYTES + TB::BYTES) : EPILOGUE;
+  constexpr int BNO = EPI == EPI_GATED ? BN / 2 : BN, LDS = ProductLds<T, AK, BK, BM, BN, EPI>::BYTES;
   const long long tiles = ((p.M + BM - 1) / BM) * ((p.N + BNO - 1) / BNO);
   if (tiles > MAX_BLOCKS) return hipErrorInvalidValue;
   auto kern = k_product<T, AK, BK, BM, BN, EPI>;
@@ -17,11 +14,13 @@ template <bool AK, bool BK, int BM, int BN, int EPI> hipError_t launch_tile(cons
   return hipGetLastError();
 }
 
-// 128 x 128 tiles where they fill the device, else 64 x 64.
+// The largest tile of which there is one per CU.
 template <bool AK, bool BK, int EPI> hipError_t launch_product(const Product& p, int splits, hipStream_t st) {
-  const long long nout = EPI == EPI_GATED ? 2 * p.N : p.N;
-  const long long big = ((p.M + 127) / 128) * ((nout + 127) / 128) * splits;
-  return big >= CUS ? launch_tile<AK, BK, 128, 128, EPI>(p, splits, st) : launch_tile<AK, BK, 64, 64, EPI>(p, splits, st);
+  const long long nout = EPI == EPI_GATED ? 2 * p.N : p.N, tn = (nout + 127) / 128;
+  if constexpr (sizeof(T) == 2)
+    if ((p.M + 255) / 256 * tn * splits >= CUS) return launch_tile<AK, BK, 256, 128, EPI>(p, splits, st);
+  if ((p.M + 127) / 128 * tn * splits >= CUS) return launch_tile<AK, BK, 128, 128, EPI>(p, splits, st);
+  return launch_tile<AK, BK, 64, 64, EPI>(p, splits, st);
 }
 
 // How many ways the sum over the rows is split in dw = dz^T x: few tiles, many rows.

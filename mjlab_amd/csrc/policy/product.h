@@ -4,10 +4,16 @@
 //   y  = x w^T     A = x  (k contiguous)    B = w  (k contiguous)
 //   dx = dz w      A = dz (k contiguous)    B = w  (n contiguous)
 //   dw = dz^T x    A = dz (m contiguous)    B = x  (n contiguous)
-// A k-contiguous tile lies in LDS as rows of 128 bytes whose eight 16-byte chunks are exchanged by the row's low bits, so that the 32 rows
-// one fragment reads meet all banks evenly; the other kind lies as it is in memory, k rows of m elements, and 16-bit fragments are turned by
-// the transposing LDS read (ds_read_b64_tr_b16: four k of one m per lane).  Global loads go through registers one k-tile ahead of the
-// matrix instructions, two LDS buffers, one barrier per k-tile.
+// A k-contiguous tile lies in LDS as rows of 64 or 128 bytes whose 16-byte chunks are exchanged by the row's low bits, so that the 32 rows one
+// fragment reads meet all banks evenly; the other kind lies as it is in memory, k rows of m elements, and 16-bit fragments are turned by the
+// transposing LDS read (ds_read_b64_tr_b16: four k of one m per lane).  Global loads go through registers one k-tile ahead of the matrix
+// instructions; rows behind the last are read from the last (their results are not stored), so only a tile that k or a row's end cuts pays
+// for bounds.
+//
+// float: the bf16 matrix cores are sixteen times as fast as those for float.  A float is the sum of three bf16 h + m + l (each the nearest to what is
+// left: 3 x 8 bits and their signs hold all 24), so a b = hh + hm + mh + mm + hl + lh and terms below 2^-23 |a b|, which are left out: six products
+// of 16 bits, summed in 32, for one of float -- the error of a float product's own rounding, at up to twice the float instruction's rate.  A number that has no
+// such sum (infinite, NaN, or so large that h overflows) sets a flag, and its workgroup's product is formed again with the float instruction.
 #pragma once
 #include "policy_common.h"
 
@@ -25,9 +31,6 @@ struct Product {
   float* partial;              // EPI_PARTIAL: (splits, M, N)
 };
 
-template <typename T> struct Frag { using type = s16x8; };
-template <> struct Frag<float> { using type = f32x4; };
-
 __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c, _Float16) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
 }
@@ -40,24 +43,82 @@ __device__ __forceinline__ f32x16 mma(f32x4 a, f32x4 b, f32x16 c, float) {
   return c;
 }
 
-// LDS layout of one operand tile of R rows (m or n) and 128 bytes of k per row
-template <typename T, bool KC, int R> struct Tile {
-  static constexpr int V = Elem<T>::VEC, KT = 8 * V, NCH = R * 8 / 256;  // k per tile, 16-byte chunks per thread
-  static constexpr int STRIDE = KC ? 128 : R * (int)sizeof(T) + 32;      // bytes; + 32: the four k rows a transposing read takes lie in other banks
-  static constexpr int BYTES = KC ? R * 128 : KT * STRIDE;
+template <typename E> struct Frag { using type = s16x8; };
+template <> struct Frag<float> { using type = f32x4; };
 
-  static __device__ __forceinline__ int address(int idx) {
-    if constexpr (KC) { const int row = idx >> 3, c = idx & 7; return row * 128 + ((c ^ (row & 7)) << 4); }
-    else { const int row = idx / (R / V), c = idx % (R / V); return row * STRIDE + c * 16; }
+// A unit: what one thread loads, keeps and stages at a time, UE neighbouring elements of memory.
+template <typename T, int UE> struct alignas(16) Unit {
+  T e[UE];
+};
+template <typename T, int UE> __device__ __forceinline__ void load_unit(Unit<T, UE>& u, const T* p) { __builtin_memcpy(&u, p, sizeof(u)); }
+template <typename T, int UE> __device__ __forceinline__ void load_unit_part(Unit<T, UE>& u, const T* p, long long n) {
+  if (n >= UE) { load_unit(u, p); return; }
+#pragma unroll
+  for (int i = 0; i < UE; ++i) u.e[i] = i < n ? p[i] : (T)0.f;
+}
+
+// How T is multiplied: as it is (E = T; 16 bits, or the float instruction) or as the sum of three bf16 (SPLIT).
+// KB: bytes of k per row and plane of a tile; a k-step of the inner loop is two 16-byte chunks.
+template <typename T, bool SPLIT, int KB> struct How {
+  using E = __bf16;
+  static constexpr int PLANES = 3, UE = 8, KT = KB / 2, STEPS = KB / 32;
+};
+template <typename T, int KB> struct How<T, false, KB> {
+  using E = T;
+  static constexpr int PLANES = 1, UE = 16 / sizeof(T), KT = KB / sizeof(T), STEPS = KB / 32;
+};
+
+// h, m, l of eight floats; true if one of them has none
+__device__ __forceinline__ bool split3(const float* x, b16x8& h, b16x8& m, b16x8& l) {
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    h[i] = (__bf16)x[i];
+    const float hf = (float)h[i], r = x[i] - hf;
+    m[i] = (__bf16)r;
+    l[i] = (__bf16)(r - (float)m[i]);
+    odd |= (__float_as_uint(hf) & 0x7f800000u) == 0x7f800000u;
+  }
+  return odd;
+}
+
+// LDS layout of one operand tile of R rows (m or n)
+template <typename T, bool SPLIT, int KB, bool KC, int R> struct Tile {
+  using H = How<T, SPLIT, KB>;
+  using E = typename H::E;
+  static constexpr int UE = H::UE, KT = H::KT, NU = R * KT / UE / 256;  // units per thread
+  static constexpr int STRIDE = KC ? KB : R * (int)sizeof(E) + 32;      // bytes; + 32: the four k rows a transposing read takes lie in other banks
+  static constexpr int PLANE = KC ? R * KB : KT * STRIDE, BYTES = H::PLANES * PLANE;
+  static constexpr int UPR = KC ? KT / UE : R / UE;                     // units per row of the tile (KC: m rows; else k rows)
+
+  static __device__ __forceinline__ int swizzle(int row, int c) { return KB == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3); }
+  static __device__ __forceinline__ int row_of(int u) { return u / UPR; }
+  static __device__ __forceinline__ int col_of(int u) { return u % UPR * UE; }
+
+  static __device__ __forceinline__ bool put(char* s, int u, const Unit<T, UE>& x) {
+    const int row = u / UPR, c = u % UPR;
+    char* at = s + (KC ? row * KB + (swizzle(row, c) << 4) : row * STRIDE + c * 16);
+    if constexpr (SPLIT) {
+      b16x8 h, m, l;
+      const bool odd = split3(x.e, h, m, l);
+      *(b16x8*)at = h;
+      *(b16x8*)(at + PLANE) = m;
+      *(b16x8*)(at + 2 * PLANE) = l;
+      return odd;
+    } else {
+      *(Unit<T, UE>*)at = x;
+      return false;
+    }
   }
 
-  // the fragment of rows row0 .. row0 + 31 for the kk-th eighth-pair of the tile: lanes 0-31 hold chunk 2 kk, lanes 32-63 chunk 2 kk + 1 of k
-  static __device__ __forceinline__ typename Frag<T>::type frag(const char* s, int row0, int kk, int lane) {
+  // the fragment of rows row0 .. row0 + 31 at k-step kk: lanes 0-31 hold chunk 2 kk, lanes 32-63 chunk 2 kk + 1 of k
+  static __device__ __forceinline__ typename Frag<E>::type frag(const char* s, int plane, int row0, int kk, int lane) {
     const int half = lane >> 5;
+    s += plane * PLANE;
     if constexpr (KC) {
-      const int row = row0 + (lane & 31), c = 2 * kk + half;
-      return *(const typename Frag<T>::type*)(s + row * 128 + ((c ^ (row & 7)) << 4));
-    } else if constexpr (sizeof(T) == 2) {
+      const int row = row0 + (lane & 31);
+      return *(const typename Frag<E>::type*)(s + row * KB + (swizzle(row, 2 * kk + half) << 4));
+    } else if constexpr (sizeof(E) == 2) {
       const int t = lane & 15, k = kk * 16 + half * 8 + (t >> 2), m = row0 + ((lane >> 4) & 1) * 16 + (t & 3) * 4;
       typedef __attribute__((address_space(3))) s16x4 lds_s4;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(s + k * STRIDE + m * 2));
@@ -72,64 +133,86 @@ template <typename T, bool KC, int R> struct Tile {
   }
 };
 
-// 256 threads = 4 waves as 2 x 2; a wave owns BM / 2 x BN / 2 of C in 32 x 32 tiles.
-template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __launch_bounds__(256, 2) void k_product(const Product p) {
-  using TA = Tile<T, AK, BM>;
-  using TB = Tile<T, BK, BN>;
-  constexpr int V = Elem<T>::VEC, KT = TA::KT, WM = BM / 2, WN = BN / 2, MI = WM / 32, NI = WN / 32;
-  constexpr int BUF = TA::BYTES + TB::BYTES;
-  constexpr bool GATED = EPI == EPI_GATED;
-  constexpr int BNO = GATED ? BN / 2 : BN, HALF = WN / 2;  // output columns per workgroup; a gated wave owns HALF columns of both products
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-
+// The sum over k in [kbeg, kend) for the tile at (m0, n0): 4 waves as 2 x 2, each BM / 2 x BN / 2 in 32 x 32 tiles.  -> true if (SPLIT) a number had no sum.
+template <typename T, bool SPLIT, int KB, int BUFFERS, bool AK, bool BK, int BM, int BN, bool GATED>
+__device__ __forceinline__ bool product_tile(const Product& p, long long m0, long long n0, long long kbeg, long long kend, char* lds, f32x16 (&acc)[BM / 64][BN / 64]) {
+  using H = How<T, SPLIT, KB>;
+  using TA = Tile<T, SPLIT, KB, AK, BM>;
+  using TB = Tile<T, SPLIT, KB, BK, BN>;
+  using E = typename H::E;
+  constexpr int UE = H::UE, KT = H::KT, WM = BM / 2, WN = BN / 2, MI = WM / 32, NI = WN / 32, HALF = WN / 2, BUF = TA::BYTES + TB::BYTES;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
-  const long long tn = (p.N + BNO - 1) / BNO, tile = xcd_tile(blockIdx.x, gridDim.x);
-  const long long m0 = tile / tn * BM, n0 = tile % tn * BNO;
-  const long long kbeg = blockIdx.y * p.ksplit, kend = kbeg + p.ksplit < p.K ? kbeg + p.ksplit : p.K;
   const T *A = (const T*)p.A, *B = (const T*)p.B, *B2 = (const T*)p.B2;
+  // a tile that no row's end cuts (matters where rows are what is contiguous)
+  const bool inside = (AK || m0 + BM <= p.M) && (BK || n0 + BN <= p.N);
 
-  Chunk<T> ra[TA::NCH], rb[TB::NCH];
-  auto load = [&](long long k0) {
-#pragma unroll
-    for (int i = 0; i < TA::NCH; ++i) {
-      const int idx = tid + i * 256;
-      if constexpr (AK) {
-        const long long m = m0 + (idx >> 3), k = k0 + (idx & 7) * V;
-        ra[i] = load_part(A + m * p.lda + k, m < p.M ? kend - k : 0);
-      } else {
-        const long long k = k0 + idx / (BM / V), m = m0 + (idx % (BM / V)) * V;
-        ra[i] = load_part(A + k * p.lda + m, k < kend ? p.M - m : 0);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < TB::NCH; ++i) {
-      const int idx = tid + i * 256;
-      if constexpr (BK) {
-        const int row = idx >> 3;
-        const long long k = k0 + (idx & 7) * V;
-        if constexpr (GATED) {
-          const long long n = n0 + row / (2 * HALF) * HALF + row % HALF;
-          const bool up = (row / HALF) & 1;
-          rb[i] = load_part((up ? B2 + n * p.ldb2 : B + n * p.ldb) + k, n < p.N ? kend - k : 0);
-        } else {
-          const long long n = n0 + row;
-          rb[i] = load_part(B + n * p.ldb + k, n < p.N ? kend - k : 0);
-        }
-      } else {
-        const long long k = k0 + idx / (BN / V), n = n0 + (idx % (BN / V)) * V;
-        const T* row = k < p.kb2 ? B + k * p.ldb : B2 + (k - p.kb2) * p.ldb2;
-        rb[i] = load_part(row + n, k < kend ? p.N - n : 0);
-      }
+  Unit<T, UE> ra[TA::NU], rb[TB::NU];
+  const T *pa[TA::NU], *pb[TB::NU];  // where this thread's units lie at the present k-tile
+  auto a_at = [&](int i, long long k0) {
+    const int u = tid + i * 256, r = TA::row_of(u), c = TA::col_of(u);
+    if constexpr (AK) { const long long m = m0 + r < p.M ? m0 + r : p.M - 1; return A + m * p.lda + k0 + c; }
+    else return A + (k0 + r) * p.lda + m0 + c;
+  };
+  auto b_at = [&](int i, long long k0) {
+    const int u = tid + i * 256, r = TB::row_of(u), c = TB::col_of(u);
+    if constexpr (BK) {
+      long long n = GATED ? n0 + r / (2 * HALF) * HALF + r % HALF : n0 + r;
+      n = n < p.N ? n : p.N - 1;
+      return (GATED && (r / HALF & 1) ? B2 + n * p.ldb2 : B + n * p.ldb) + k0 + c;
+    } else {
+      const long long k = k0 + r;
+      return (k < p.kb2 ? B + k * p.ldb : B2 + (k - p.kb2) * p.ldb2) + n0 + c;
     }
   };
+  auto aim = [&](long long k0) {
+#pragma unroll
+    for (int i = 0; i < TA::NU; ++i) pa[i] = a_at(i, k0);
+#pragma unroll
+    for (int i = 0; i < TB::NU; ++i) pb[i] = b_at(i, k0);
+  };
+  auto load = [&](long long k0) {
+    if (inside && k0 + KT <= kend) {
+#pragma unroll
+      for (int i = 0; i < TA::NU; ++i) load_unit(ra[i], pa[i]);
+#pragma unroll
+      for (int i = 0; i < TB::NU; ++i) load_unit(rb[i], pb[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < TA::NU; ++i) {
+        const int u = tid + i * 256, r = TA::row_of(u), c = TA::col_of(u);
+        load_unit_part(ra[i], pa[i], AK ? kend - (k0 + c) : k0 + r < kend ? p.M - (m0 + c) : 0);
+      }
+#pragma unroll
+      for (int i = 0; i < TB::NU; ++i) {
+        const int u = tid + i * 256, r = TB::row_of(u), c = TB::col_of(u);
+        load_unit_part(rb[i], pb[i], BK ? kend - (k0 + c) : k0 + r < kend ? p.N - (n0 + c) : 0);
+      }
+    }
+    // on to the next k-tile; where B's rows change over to B2's, the pointers are formed anew
+#pragma unroll
+    for (int i = 0; i < TA::NU; ++i) pa[i] += AK ? KT : KT * p.lda;
+    if constexpr (BK) {
+#pragma unroll
+      for (int i = 0; i < TB::NU; ++i) pb[i] += KT;
+    } else {
+      const bool same = k0 + 2 * KT <= p.kb2 || k0 >= p.kb2;  // (uniform)
+#pragma unroll
+      for (int i = 0; i < TB::NU; ++i) pb[i] = same ? pb[i] + KT * (k0 < p.kb2 ? p.ldb : p.ldb2) : b_at(i, k0 + KT);
+    }
+  };
+  bool odd = false;
   auto stage = [&](char* s) {
 #pragma unroll
-    for (int i = 0; i < TA::NCH; ++i) *(Chunk<T>*)(s + TA::address(tid + i * 256)) = ra[i];
+    for (int i = 0; i < TA::NU; ++i) odd |= TA::put(s, tid + i * 256, ra[i]);
 #pragma unroll
-    for (int i = 0; i < TB::NCH; ++i) *(Chunk<T>*)(s + TA::BYTES + TB::address(tid + i * 256)) = rb[i];
+    for (int i = 0; i < TB::NU; ++i) odd |= TB::put(s + TA::BYTES, tid + i * 256, rb[i]);
   };
 
-  f32x16 acc[MI][NI] = {};
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j) acc[i][j] = f32x16{};
+  aim(kbeg);
   load(kbeg);
   stage(lds);
   __syncthreads();
@@ -139,20 +222,68 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
     if (more) load(k0 + KT);
     const char *sa = lds + cur * BUF, *sb = sa + TA::BYTES;
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk) {
-      typename Frag<T>::type fa[MI], fb[NI];
+    for (int kk = 0; kk < H::STEPS; ++kk) {
+      typename Frag<E>::type fa[MI][H::PLANES], fb[NI][H::PLANES];
 #pragma unroll
-      for (int i = 0; i < MI; ++i) fa[i] = TA::frag(sa, wm + i * 32, kk, lane);
+      for (int q = 0; q < H::PLANES; ++q) {
 #pragma unroll
-      for (int j = 0; j < NI; ++j) fb[j] = TB::frag(sb, wn + j * 32, kk, lane);
+        for (int i = 0; i < MI; ++i) fa[i][q] = TA::frag(sa, q, wm + i * 32, kk, lane);
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+        for (int j = 0; j < NI; ++j) fb[j][q] = TB::frag(sb, q, wn + j * 32, kk, lane);
+      }
 #pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = mma(fa[i], fb[j], acc[i][j], T());
+      for (int qa = 0; qa < H::PLANES; ++qa)
+#pragma unroll
+        for (int qb = 0; qa + qb < H::PLANES; ++qb)
+#pragma unroll
+          for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) acc[i][j] = mma(fa[i][qa], fb[j][qb], acc[i][j], E());
     }
-    if (more) stage(lds + (cur ^ 1) * BUF);
+    if (BUFFERS == 1) __syncthreads();
+    if (more) stage(lds + (BUFFERS == 2 ? (cur ^ 1) * BUF : 0));
     __syncthreads();
-    cur ^= 1;
+    if (BUFFERS == 2) cur ^= 1;
+  }
+  return odd;
+}
+
+// Sizes of a launch: the tile, and how T is multiplied in it.
+template <typename T, int BM_, int BN_> struct Shape {
+  static constexpr int BM = BM_, BN = BN_, KB = BM_ == 256 ? 64 : 128, BUFFERS = 2;
+  static constexpr bool SPLIT = false;
+};
+template <int BM_, int BN_> struct Shape<float, BM_, BN_> {
+  static constexpr int BM = BM_, BN = BN_, KB = 64, BUFFERS = BM_ == 64 ? 2 : 1;
+  static constexpr bool SPLIT = true;
+};
+
+template <typename T, bool AK, bool BK, int BM, int BN, int EPI> struct ProductLds {
+  using S = Shape<T, BM, BN>;
+  static constexpr int TILES = S::BUFFERS * (Tile<T, S::SPLIT, S::KB, AK, BM>::BYTES + Tile<T, S::SPLIT, S::KB, BK, BN>::BYTES);
+  static constexpr int AGAIN = Tile<T, false, 64, AK, BM>::BYTES + Tile<T, false, 64, BK, BN>::BYTES;  // (float's second try)
+  static constexpr int EPILOGUE = 4 * 32 * (BN / 2 + 4) * 4;
+  static constexpr int BYTES = TILES > EPILOGUE ? (TILES > AGAIN ? TILES : AGAIN) : (EPILOGUE > AGAIN ? EPILOGUE : AGAIN);
+};
+
+template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __launch_bounds__(256, 2) void k_product(const Product p) {
+  using S = Shape<T, BM, BN>;
+  constexpr int V = Elem<T>::VEC, WM = BM / 2, WN = BN / 2, MI = WM / 32, NI = WN / 32;
+  constexpr bool GATED = EPI == EPI_GATED;
+  constexpr int BNO = GATED ? BN / 2 : BN, HALF = WN / 2;  // output columns per workgroup; a gated wave owns HALF columns of both products
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
+  // Tiles go through the device in groups of 8 rows of tiles, column after column: neighbours in time share operand rows in L2.
+  const long long tm = (p.M + BM - 1) / BM, tn = (p.N + BNO - 1) / BNO, tile = xcd_tile(blockIdx.x, gridDim.x);
+  const long long g = tile / (8 * tn), in = tile % (8 * tn), gm = tm - 8 * g < 8 ? tm - 8 * g : 8;
+  const long long m0 = (8 * g + in % gm) * BM, n0 = in / gm * BNO;
+  const long long kbeg = blockIdx.y * p.ksplit, kend = kbeg + p.ksplit < p.K ? kbeg + p.ksplit : p.K;
+
+  f32x16 acc[MI][NI];
+  const bool odd = product_tile<T, S::SPLIT, S::KB, S::BUFFERS, AK, BK, BM, BN, GATED>(p, m0, n0, kbeg, kend, lds, acc);
+  if constexpr (S::SPLIT) {
+    if (__syncthreads_or(odd)) product_tile<T, false, 64, 1, AK, BK, BM, BN, GATED>(p, m0, n0, kbeg, kend, lds, acc);
   }
 
   // C leaves through LDS, 32 rows of the wave's own at a time: an accumulator holds one column per lane, memory wants 16 bytes of a row.
