@@ -111,9 +111,10 @@ hipError_t POLICY_NAME(mjlab_launch_layer_backward)(const mjlab_layer_grad_t* g,
     if (splits == 1 && !q.gated) return launch_product<false, false, EPI_STORE>(p, 1, st);
     if ((e = launch_product<false, false, EPI_PARTIAL>(p, splits, st)) != hipSuccess) return e;
     const long long n = f.out * f.in;
+    if ((n + 255) / 256 > MAX_BLOCKS) return hipErrorInvalidValue;
     for (int u = 0; u < (q.gated ? 2 : 1); ++u) {
       // (a gated layer's partials hold both matrices: 2 n floats per split)
-      hipLaunchKernelGGL(k_join_splits<T>, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, st, partial + u * n, (T*)(u ? g->dw_up : g->dw), n, q.ns * n, splits);
+      hipLaunchKernelGGL(k_join_splits<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, partial + u * n, (T*)(u ? g->dw_up : g->dw), n, q.ns * n, splits);
       if ((e = hipGetLastError()) != hipSuccess) return e;
     }
   }

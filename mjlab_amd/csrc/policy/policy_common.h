@@ -46,17 +46,41 @@ template <typename T> __device__ __forceinline__ void store_part(T* p, const Chu
     if (i < n) p[i] = c.e[i];
 }
 
-// ---- activations, in float.  NaN goes through every one of them.
-__device__ __forceinline__ float sigmoid_f(float z) { return 1.f / (1.f + __expf(-z)); }
+// ---- activations, in float.  NaN goes through every one of them.  The device library's erff, expm1f and tanhf cost a hundred instructions each; a layer's
+// epilogue runs one per output, which at 24576 x 1024 outputs took longer than the product (187 us together, 128 us with the forms below).
+__device__ __forceinline__ float rcp_f(float x) { return __builtin_amdgcn_rcpf(x); }  // 1 ulp
+__device__ __forceinline__ float sigmoid_f(float z) { return rcp_f(1.f + __expf(-z)); }
+
+// exp(z) - 1 for z <= 0: the series to z^7 above -1/4 (next term: 2^-16 / 40320 of z, below 2^-31), the difference below
+__device__ __forceinline__ float expm1_neg(float z) {
+  const float s = z * (1.f + z * (1.f / 2 + z * (1.f / 6 + z * (1.f / 24 + z * (1.f / 120 + z * (1.f / 720 + z * (1.f / 5040)))))));
+  const float d = __expf(z) - 1.f;
+  return z > -0.25f ? s : d;
+}
+
+// The odd series to z^9 below 1/4 (next term: 2^-20 * 0.0089 of z), 1 - 2 / (1 + exp 2z) above
+__device__ __forceinline__ float tanh_f(float z) {
+  const float q = z * z;
+  const float s = z * (1.f + q * (-1.f / 3 + q * (2.f / 15 + q * (-17.f / 315 + q * (62.f / 2835)))));
+  const float d = 1.f - 2.f * rcp_f(1.f + __expf(2.f * z));
+  return q < 0.0625f ? s : d;
+}
+
+// (1 + erf(z / sqrt 2)) / 2 with e = exp(-z^2 / 2): Abramowitz and Stegun 7.1.26, off by 0.75e-7 at most
+__device__ __forceinline__ float normal_cdf(float z, float e) {
+  const float t = rcp_f(1.f + 0.3275911f * 0.70710678f * __builtin_fabsf(z));
+  const float tail = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  return z < 0.f ? tail : 1.f - tail;
+}
 
 __device__ __forceinline__ float act_value(float z, int act) {
   switch (act) {
     case MJLAB_ACT_RELU: return z < 0.f ? 0.f : z;
-    case MJLAB_ACT_ELU: return z > 0.f ? z : expm1f(z);
-    case MJLAB_ACT_TANH: return tanhf(z);
+    case MJLAB_ACT_ELU: return z > 0.f ? z : expm1_neg(z);
+    case MJLAB_ACT_TANH: return tanh_f(z);
     case MJLAB_ACT_SIGMOID: return sigmoid_f(z);
     case MJLAB_ACT_SILU: return z * sigmoid_f(z);
-    case MJLAB_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678f));
+    case MJLAB_ACT_GELU: return z * normal_cdf(z, __expf(-0.5f * z * z));
     default: return z;
   }
 }
@@ -68,10 +92,10 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case MJLAB_ACT_RELU: return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
     case MJLAB_ACT_ELU: return z > 0.f ? 1.f : __expf(z);
-    case MJLAB_ACT_TANH: { const float t = tanhf(z); return 1.f - t * t; }
-    case MJLAB_ACT_SIGMOID: { const float s = sigmoid_f(z); return s * (1.f - s); }
+    case MJLAB_ACT_TANH: { const float e = __expf(-2.f * __builtin_fabsf(z)), r = rcp_f(1.f + e); return 4.f * e * r * r; }
+    case MJLAB_ACT_SIGMOID: { const float e = __expf(-__builtin_fabsf(z)), r = rcp_f(1.f + e); return e * r * r; }
     case MJLAB_ACT_SILU: { const float s = sigmoid_f(z); return s * (1.f + z * (1.f - s)); }
-    case MJLAB_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+    case MJLAB_ACT_GELU: { const float e = __expf(-0.5f * z * z); return normal_cdf(z, e) + z * 0.39894228f * e; }
     default: return 1.f;
   }
 }

@@ -7,8 +7,8 @@
 // A k-contiguous tile lies in LDS as rows of 64 or 128 bytes whose 16-byte chunks are exchanged by the row's low bits, so that the 32 rows one
 // fragment reads meet all banks evenly; the other kind lies as it is in memory, k rows of m elements, and 16-bit fragments are turned by the
 // transposing LDS read (ds_read_b64_tr_b16: four k of one m per lane).  Global loads go through registers one k-tile ahead of the matrix
-// instructions; rows behind the last are read from the last (their results are not stored), so only a tile that k or a row's end cuts pays
-// for bounds.
+// instructions.  What lies behind the last m or n may be anything, since its results are not stored: rows behind the last are read from the last,
+// and 16 bytes that a row's end cuts are read whole, on into the next row -- but for the last row of all.  So only a k-tile at the end of k pays for bounds.
 //
 // float: the bf16 matrix cores are sixteen times as fast as those for float.  A float is the sum of three bf16 h + m + l (each the nearest to what is
 // left: 3 x 8 bits and their signs hold all 24), so a b = hh + hm + mh + mm + hl + lh and terms below 2^-23 |a b|, which are left out: six products
@@ -68,18 +68,25 @@ template <typename T, int KB> struct How<T, false, KB> {
   static constexpr int PLANES = 1, UE = 16 / sizeof(T), KT = KB / sizeof(T), STEPS = KB / 32;
 };
 
-// h, m, l of eight floats; true if one of them has none
-__device__ __forceinline__ bool split3(const float* x, b16x8& h, b16x8& m, b16x8& l) {
-  bool odd = false;
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+
+// h, m, l of eight floats; `odd` becomes NaN if one of them has none (x - h is then infinite or NaN)
+__device__ __forceinline__ void split3(const float* x, b16x8& h, b16x8& m, b16x8& l, float& odd) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    h[i] = (__bf16)x[i];
-    const float hf = (float)h[i], r = x[i] - hf;
-    m[i] = (__bf16)r;
-    l[i] = (__bf16)(r - (float)m[i]);
-    odd |= (__float_as_uint(hf) & 0x7f800000u) == 0x7f800000u;
+  for (int i = 0; i < 8; i += 2) {
+    const f32x2 v = {x[i], x[i + 1]};
+    const b16x2 a = __builtin_convertvector(v, b16x2);
+    const unsigned ua = __builtin_bit_cast(unsigned, a);
+    const f32x2 r = {v[0] - __uint_as_float(ua << 16), v[1] - __uint_as_float(ua & 0xffff0000u)};
+    const b16x2 b = __builtin_convertvector(r, b16x2);
+    const unsigned ub = __builtin_bit_cast(unsigned, b);
+    const f32x2 q = {r[0] - __uint_as_float(ub << 16), r[1] - __uint_as_float(ub & 0xffff0000u)};
+    const b16x2 c = __builtin_convertvector(q, b16x2);
+    h[i] = a[0]; h[i + 1] = a[1]; m[i] = b[0]; m[i + 1] = b[1]; l[i] = c[0]; l[i + 1] = c[1];
+    odd = __builtin_fmaf(r[0], 0.f, odd);
+    odd = __builtin_fmaf(r[1], 0.f, odd);
   }
-  return odd;
 }
 
 // LDS layout of one operand tile of R rows (m or n)
@@ -95,19 +102,17 @@ template <typename T, bool SPLIT, int KB, bool KC, int R> struct Tile {
   static __device__ __forceinline__ int row_of(int u) { return u / UPR; }
   static __device__ __forceinline__ int col_of(int u) { return u % UPR * UE; }
 
-  static __device__ __forceinline__ bool put(char* s, int u, const Unit<T, UE>& x) {
+  static __device__ __forceinline__ void put(char* s, int u, const Unit<T, UE>& x, float& odd) {
     const int row = u / UPR, c = u % UPR;
     char* at = s + (KC ? row * KB + (swizzle(row, c) << 4) : row * STRIDE + c * 16);
     if constexpr (SPLIT) {
       b16x8 h, m, l;
-      const bool odd = split3(x.e, h, m, l);
+      split3(x.e, h, m, l, odd);
       *(b16x8*)at = h;
       *(b16x8*)(at + PLANE) = m;
       *(b16x8*)(at + 2 * PLANE) = l;
-      return odd;
     } else {
       *(Unit<T, UE>*)at = x;
-      return false;
     }
   }
 
@@ -143,15 +148,21 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
   constexpr int UE = H::UE, KT = H::KT, WM = BM / 2, WN = BN / 2, MI = WM / 32, NI = WN / 32, HALF = WN / 2, BUF = TA::BYTES + TB::BYTES;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
   const T *A = (const T*)p.A, *B = (const T*)p.B, *B2 = (const T*)p.B2;
-  // a tile that no row's end cuts (matters where rows are what is contiguous)
-  const bool inside = (AK || m0 + BM <= p.M) && (BK || n0 + BN <= p.N);
+  // Row-contiguous operands: a tile that no row's end cuts, or one whose rows lie far enough apart that a unit read beyond the end stays before the
+  // end of the row after the next one's start
+  const bool in_a = AK || m0 + BM <= p.M, in_b = BK || n0 + BN <= p.N;
+  const bool over_a = in_a || p.lda >= UE, over_b = in_b || (p.ldb >= UE && (p.kb2 == p.K || p.ldb2 >= UE));
+  auto whole = [&](long long k0) {  // (uniform) the k-tile at k0 can be read without bounds
+    const long long k1 = k0 + KT;
+    return k1 <= kend && over_a && over_b && (in_a || k1 < p.K) && (in_b || (k1 < p.K && (k1 < p.kb2 || k0 >= p.kb2)));
+  };
 
   Unit<T, UE> ra[TA::NU], rb[TB::NU];
   const T *pa[TA::NU], *pb[TB::NU];  // where this thread's units lie at the present k-tile
   auto a_at = [&](int i, long long k0) {
     const int u = tid + i * 256, r = TA::row_of(u), c = TA::col_of(u);
     if constexpr (AK) { const long long m = m0 + r < p.M ? m0 + r : p.M - 1; return A + m * p.lda + k0 + c; }
-    else return A + (k0 + r) * p.lda + m0 + c;
+    else return A + (k0 + r) * p.lda + (m0 + c < p.M ? m0 + c : 0);
   };
   auto b_at = [&](int i, long long k0) {
     const int u = tid + i * 256, r = TB::row_of(u), c = TB::col_of(u);
@@ -161,7 +172,7 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
       return (GATED && (r / HALF & 1) ? B2 + n * p.ldb2 : B + n * p.ldb) + k0 + c;
     } else {
       const long long k = k0 + r;
-      return (k < p.kb2 ? B + k * p.ldb : B2 + (k - p.kb2) * p.ldb2) + n0 + c;
+      return (k < p.kb2 ? B + k * p.ldb : B2 + (k - p.kb2) * p.ldb2) + (n0 + c < p.N ? n0 + c : 0);
     }
   };
   auto aim = [&](long long k0) {
@@ -171,7 +182,7 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
     for (int i = 0; i < TB::NU; ++i) pb[i] = b_at(i, k0);
   };
   auto load = [&](long long k0) {
-    if (inside && k0 + KT <= kend) {
+    if (whole(k0)) {
 #pragma unroll
       for (int i = 0; i < TA::NU; ++i) load_unit(ra[i], pa[i]);
 #pragma unroll
@@ -200,12 +211,12 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
       for (int i = 0; i < TB::NU; ++i) pb[i] = same ? pb[i] + KT * (k0 < p.kb2 ? p.ldb : p.ldb2) : b_at(i, k0 + KT);
     }
   };
-  bool odd = false;
+  float odd = 0.f;
   auto stage = [&](char* s) {
 #pragma unroll
-    for (int i = 0; i < TA::NU; ++i) odd |= TA::put(s, tid + i * 256, ra[i]);
+    for (int i = 0; i < TA::NU; ++i) TA::put(s, tid + i * 256, ra[i], odd);
 #pragma unroll
-    for (int i = 0; i < TB::NU; ++i) odd |= TB::put(s + TA::BYTES, tid + i * 256, rb[i]);
+    for (int i = 0; i < TB::NU; ++i) TB::put(s + TA::BYTES, tid + i * 256, rb[i], odd);
   };
 
 #pragma unroll
@@ -245,7 +256,7 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
     __syncthreads();
     if (BUFFERS == 2) cur ^= 1;
   }
-  return odd;
+  return odd != odd;
 }
 
 // Sizes of a launch: the tile, and how T is multiplied in it.
@@ -350,20 +361,14 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
   }
 }
 
-// out = sum over the splits, in the order of the splits
+// out = sum over the splits, in the order of the splits; one element per thread, eight loads in flight
 template <typename T> __global__ __launch_bounds__(256) void k_join_splits(const float* partial, T* out, long long n, long long stride, int splits) {
-  const long long i = (blockIdx.x * 256LL + threadIdx.x) * 4;
+  const long long i = blockIdx.x * 256LL + threadIdx.x;
   if (i >= n) return;
-  const long long left = n - i;
-  float s[4] = {};
-  for (int k = 0; k < splits; ++k) {
-    const Chunk<float> c = load_part(partial + k * stride + i, left);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) s[e] += c.e[e];
-  }
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (e < left) out[i + e] = (T)s[e];
+  float s = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < splits; ++k) s += partial[k * stride + i];
+  out[i] = (T)s;
 }
 
 // dz (rows, out | 2 out) from dy and the stored sums, and this row block's column sums for the bias gradient.
