@@ -8,6 +8,8 @@
 // nothing overflows.  A sequence is split into segments when there are few sequences: a first pass forms each segment's own contribution to R, a
 // scan along the segments turns these into the R each segment starts from, the second pass does the rest.
 #pragma once
+#include <type_traits>
+
 #include "policy_common.h"
 
 struct DecayPass {
@@ -61,71 +63,169 @@ __device__ __forceinline__ bool reset_at(const DecayPass& p, long long seq, long
   return p.reset_bytes == 1 ? ((const unsigned char*)p.reset)[i] != 0 : ((const int*)p.reset)[i] != 0;
 }
 
-template <typename T, int DA, int DC> struct DecayLds {
+template <typename T, int DA, int DC, bool STATE> struct DecayLds {
   using L = typename DecayCfg<T>::L;
   static constexpr int C = DecayCfg<T>::C, PAD = DecayCfg<T>::PAD, LA = DA + PAD, LC = DC + PAD, LP = C + PAD;
-  L a[C * LA], b[C * LA], bw[C * LA], c[C * LC], p[C * LP], r[DC * LA];
-  float power[C + 1];
+  L b[C * LA], c[C * LC], p[STATE ? 1 : C * LP], r[STATE ? 1 : DC * LA];
+  float weight[C], enter[C];  // of token j into R; of R into token i
 };
 
-// 256 threads per (sequence, head, segment).  STATE: the first pass of a split sequence, the segment's contribution to R alone.
-template <typename T, int DA, int DC, bool STATE> __global__ __launch_bounds__(256) void k_decay_chunks(const DecayPass p) {
+// VEC elements of T as elements of L, to an address aligned for them
+template <typename T, typename L> __device__ __forceinline__ void put_chunk(L* at, const Chunk<T>& x) {
+  if constexpr (sizeof(T) == sizeof(L)) *(Chunk<T>*)at = x;
+  else {
+    f32x4 lo, hi;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { lo[e] = (float)x.e[e]; hi[e] = (float)x.e[4 + e]; }
+    *(f32x4*)at = lo;
+    *(f32x4*)(at + 4) = hi;
+  }
+}
+__device__ __forceinline__ void put4(__bf16* at, const f32x4& x) {
+  typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
+  *(b16x4*)at = __builtin_convertvector(x, b16x4);
+}
+__device__ __forceinline__ void put4(float* at, const f32x4& x) { *(f32x4*)at = x; }
+
+// the weights of 16 / 4 tokens k on a fragment
+__device__ __forceinline__ s16x8 weigh(s16x8 f, const float* w, int k0, int lane) {
+  const b16x8 x = __builtin_bit_cast(b16x8, f);
+  b16x8 y;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float t = w[k0 + (lane >> 4) * 8 + i];
+    y[i] = (__bf16)(t == 0.f ? 0.f : t * (float)x[i]);
+  }
+  return __builtin_bit_cast(s16x8, y);
+}
+__device__ __forceinline__ float weigh(float x, const float* w, int k0, int lane) {
+  const float t = w[k0 + (lane >> 4)];
+  return t == 0.f ? 0.f : t * x;
+}
+
+// Elements col .. col + VEC - 1 of a row of d, zero from d on or where the row is not `live` (it exists all the same).  FULL: all of them are there.
+template <typename T, bool FULL> __device__ __forceinline__ Chunk<T> load_row(const T* row, int col, int d, bool live) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  if constexpr (FULL) {
+    const u32x4 w = __builtin_bit_cast(u32x4, load_chunk(row + col)), zero = {0, 0, 0, 0};
+    return __builtin_bit_cast(Chunk<T>, live ? w : zero);
+  }
+  return load_part(row + col, live ? d - col : 0);
+}
+
+// 256 or 512 threads per (sequence, head, segment).  FULL: da = DA and dc = DC.  STATE: the first pass of a split sequence, the segment's contribution to R alone.
+// Products are formed such that an accumulator's four rows are neighbours in memory: P^T and out^T (columns are tokens), R (rows are da).
+// The rows of a go from memory to the matrix cores' registers without LDS: with them in LDS a 128 x 128 workgroup took 114 KB, and one of them per CU
+// could not hide its loads (2 x 8192 tokens x 8 heads of 128, bf16: 130 us for this kernel then).
+constexpr int decay_threads(int da, int dc) { return da >= 64 && dc >= 64 ? 512 : 256; }
+
+template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch_bounds__(decay_threads(DA, DC), 2) void k_decay_chunks(const DecayPass p) {
   using Cfg = DecayCfg<T>;
   using L = typename Cfg::L;
-  using S = DecayLds<T, DA, DC>;
-  constexpr int C = Cfg::C, KS = Cfg::KS, LA = S::LA, LC = S::LC, LP = S::LP, V = Elem<T>::VEC;
-  constexpr int CT = C / 16, NO = CT * (DC / 16) / 4, NR = (DA / 16) * (DC / 16) / 4;  // 16 x 16 tiles per wave: of out, of R
-  constexpr int NA = (C * DA / V + 255) / 256, NC = (C * DC / V + 255) / 256;          // 16-byte chunks per thread
+  using S = DecayLds<T, DA, DC, STATE>;
+  constexpr int C = Cfg::C, KS = Cfg::KS, LA = S::LA, LC = S::LC, LP = S::LP, V = Elem<T>::VEC, CT = C / 16, KA = DA / KS;
+  constexpr int NT = decay_threads(DA, DC), NW = NT / 64, NB = (C * DA / V + NT - 1) / NT, NC = (C * DC / V + NT - 1) / NT;  // 16-byte chunks per thread
+  // Waves: of out, OR x OC waves of TR x TC tiles (tokens x dc); of R, RW x NW / RW waves of RR x RC tiles (da x dc)
+  constexpr int OC = CT == 4 ? NW / 2 : (DC / 16 < NW ? DC / 16 : NW);
+  constexpr int OR = NW / OC, TR = CT / OR, TC = DC / 16 / OC, RW = NW == 8 && DA >= 64 ? 4 : 2, RR = DA / 16 / RW, RC = DC / 16 * RW / NW;
+  static_assert(OR * OC == NW && OR * TR == CT && OC * TC == DC / 16 && RR >= 1 && RC >= 1 && RR * RW == DA / 16 && RC * (NW / RW) == DC / 16, "tiles do not cover");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   S& s = *(S*)lds;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row4 = (lane >> 4) * 4, colx = lane & 15;
+  const int t0 = (wave / OC) * TR, c0 = (wave % OC) * TC, r0 = wave / (NW / RW) * RR, rc0 = wave % (NW / RW) * RC;  // this wave's first tiles
   const int segs = STATE ? p.segments - 1 : p.segments;
   const long long sh = blockIdx.x / segs, seq = sh / p.heads;
   const int seg = (int)(blockIdx.x % segs), head = (int)(sh % p.heads);
-  const float g = p.log_decay[head];
-  for (int i = tid; i <= C; i += 256) s.power[i] = i ? expf(i * g) : 1.f;
+  // powers of the decay as 2^(n g2); a decay of zero (g2 = -infinity) stays finite here so that its power 0 is 1
+  float g2 = p.log_decay[head] * 1.44269504f;
+  g2 = g2 < -1e30f ? -1e30f : g2;
+  auto power = [&](int n) { return __builtin_amdgcn_exp2f(n * g2); };
   long long len = p.length;
   if (p.lengths) { const long long l = p.lengths[seq]; len = l < 0 ? 0 : (l < len ? l : len); }
   const T *ga = (const T*)p.a + seq * p.a_b + head * p.a_h, *gb = (const T*)p.b + seq * p.b_b + head * p.b_h, *gc = (const T*)p.c + seq * p.c_b + head * p.c_h;
   T* go = (T*)p.out + seq * p.o_b + head * p.o_h;
   auto token = [&](long long q) { return p.reverse && q < len ? len - 1 - q : q; };
+  auto there = [&](long long q) { return token(q < p.length ? q : p.length - 1); };  // a row that exists, for rows that are read but not used
 
-  Chunk<T> xa[NA], xb[NA], xc[NC];
+  Chunk<T> xb[NB], xc[NC];
   auto load = [&](long long q0) {
 #pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      const int idx = tid + i * 256, row = idx / (DA / V), col = idx % (DA / V) * V;
-      const long long q = q0 + row, t = token(q), left = row < C && q < len ? p.da - col : 0;
-      if constexpr (!STATE) xa[i] = load_part(ga + t * p.a_t + col, left);
-      xb[i] = load_part(gb + t * p.b_t + col, left);
+    for (int i = 0; i < NB; ++i) {
+      const int idx = tid + i * NT, row = idx / (DA / V), col = idx % (DA / V) * V;
+      const long long q = q0 + row;
+      xb[i] = load_row<T, FULL>(gb + there(q) * p.b_t, col, p.da, row < C && q < len);
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int idx = tid + i * 256, row = idx / (DC / V), col = idx % (DC / V) * V;
-      const long long q = q0 + row, t = token(q);
-      xc[i] = load_part(gc + t * p.c_t + col, row < C && q < len ? p.dc - col : 0);
+      const int idx = tid + i * NT, row = idx / (DC / V), col = idx % (DC / V) * V;
+      const long long q = q0 + row;
+      xc[i] = load_row<T, FULL>(gc + there(q) * p.c_t, col, p.dc, row < C && q < len);
     }
   };
+  // The rows of a of this wave's tokens.  16 bits: fragments as they are.  float: four k-steps come as 16 bytes, lane group by lane group, so the k order of
+  // the fragments is that of a_k(), not 4 step + (lane >> 4): the other operand of a product with `a` is read in the same order.
+  constexpr bool F32 = sizeof(L) == 4;
+  typename std::conditional<F32, f32x4, s16x8>::type fa[TR][F32 ? DA / 16 : KA];
+  auto a_k = [&](int i) { return sizeof(T) == 4 ? i * 16 + row4 : i / 2 * 32 + 2 * row4 + (i & 1) * 4; };  // first k of this lane in fa[.][i]
+  auto load_a = [&](long long q0) {
+#pragma unroll
+    for (int t = 0; t < TR; ++t) {
+      const long long q = q0 + (t0 + t) * 16 + colx;
+      const T* row = ga + there(q) * p.a_t;
+      if constexpr (!F32) {
+#pragma unroll
+        for (int k = 0; k < KA; ++k) fa[t][k] = __builtin_bit_cast(s16x8, load_row<T, FULL>(row, k * KS + (lane >> 4) * 8, p.da, q < len));
+      } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < DA / 16; ++i) fa[t][i] = __builtin_bit_cast(f32x4, load_row<T, FULL>(row, i * 16 + row4, p.da, q < len));
+      } else {
+#pragma unroll
+        for (int i = 0; i < DA / 32; ++i) {  // (a chunk of eight holds two neighbouring steps: the k order is that of with_a below)
+          const Chunk<T> c = load_row<T, FULL>(row, i * 32 + 2 * row4, p.da, q < len);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { fa[t][2 * i][e] = (float)c.e[e]; fa[t][2 * i + 1][e] = (float)c.e[4 + e]; }
+        }
+      }
+    }
+  };
+  // x += (rows r0 .. of s, k contiguous) (a's rows of token tile t)^T over all of da
+  auto with_a = [&](const L* rows, int row0, int t, f32x4 x) {
+    if constexpr (!F32) {
+#pragma unroll
+      for (int k = 0; k < KA; ++k) x = mma16(frag_kc(rows, LA, row0, k * KS, lane), fa[t][k], x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < DA / 16; ++i) {
+        const f32x4 o = *(const f32x4*)(rows + (row0 + colx) * LA + a_k(i));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x = mma16(o[e], fa[t][i][e], x);
+      }
+    }
+    return x;
+  };
 
-  // R, tile i of this wave: rows (of da) tr(i) * 16 + row4 .. + 3, column (of dc) tc(i) * 16 + colx
-  f32x4 acc[NR];
-  auto tr = [&](int i) { return (wave * NR + i) / (DC / 16); };
-  auto tc = [&](int i) { return (wave * NR + i) % (DC / 16); };
+  // R, tile (i, j) of this wave: rows (of da) (r0 + i) * 16 + row4 .. + 3, column (of dc) (rc0 + j) * 16 + colx
+  f32x4 acc[RR][RC];
   const float* start = STATE ? nullptr : seg ? p.seg_state + (sh * (p.segments - 1) + seg - 1) * p.da * p.dc : p.state_in ? p.state_in + sh * p.da * p.dc : nullptr;
   const int sr = seg ? p.dc : p.in_r, sc = seg ? 1 : p.in_c;
 #pragma unroll
-  for (int i = 0; i < NR; ++i)
+  for (int i = 0; i < RR; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = tr(i) * 16 + row4 + e, c = tc(i) * 16 + colx;
-      acc[i][e] = start && r < p.da && c < p.dc ? start[(long long)r * sr + c * sc] : 0.f;
-    }
+    for (int j = 0; j < RC; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = (r0 + i) * 16 + row4 + e, c = (rc0 + j) * 16 + colx;
+        acc[i][j][e] = start && (FULL || (r < p.da && c < p.dc)) ? start[(long long)r * sr + c * sc] : 0.f;
+      }
 
   const long long first = (long long)seg * p.seg_chunks * C;
   const long long last = first + (long long)p.seg_chunks * C < p.length ? first + (long long)p.seg_chunks * C : p.length;
   float factor = 1.f;
-  if (first < last) load(first);
+  if (first < last) {
+    load(first);
+    if constexpr (!STATE) load_a(first);
+  }
   for (long long q0 = first; q0 < last; q0 += C) {
     const int n = (int)(len - q0 < 0 ? 0 : (len - q0 < C ? len - q0 : C));  // live tokens of the chunk
     // cuts: bit i = the link between tokens i - 1 and i of the chunk (i = 0: the carry that comes in) is cut; out: the link to the carry that goes on
@@ -137,108 +237,144 @@ template <typename T, int DA, int DC, bool STATE> __global__ __launch_bounds__(2
       cut_out = p.reverse && reset_at(p, seq, token(q0 + n - 1));
     }
     auto episode = [&](int i) { return __popcll(cuts & ((2ULL << i) - 1)); };
+    const bool whole = (cuts >> 1) == 0;  // one episode, but perhaps for the carry
     const int e_last = n ? episode(n - 1) : 0;
     const bool carries = n == 0 || (e_last == 0 && !cut_out);  // R goes through the whole chunk
-    auto weight = [&](int j) { return j < n && !cut_out && episode(j) == e_last ? p.us * s.power[n - p.e0 - j] : 0.f; };
 
-    __syncthreads();  // the chunk before is done with LDS (and power[] is there)
+    __syncthreads();  // the chunk before is done with LDS
     bool odd = false;
 #pragma unroll
-    for (int i = 0; i < NA; ++i) {
-      const int idx = tid + i * 256, row = idx / (DA / V), col = idx % (DA / V) * V;
-      if (row >= C) continue;
-      const float w = weight(row);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if constexpr (!STATE) {
-          s.a[row * LA + col + e] = (L)(float)xa[i].e[e];
-          s.b[row * LA + col + e] = (L)(float)xb[i].e[e];
-        }
-        s.bw[row * LA + col + e] = w == 0.f ? (L)0.f : (L)(w * (float)xb[i].e[e]);
-      }
+    for (int i = 0; i < NB; ++i) {
+      const int idx = tid + i * NT, row = idx / (DA / V), col = idx % (DA / V) * V;
+      if (row < C) put_chunk(s.b + row * LA + col, xb[i]);
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int idx = tid + i * 256, row = idx / (DC / V), col = idx % (DC / V) * V;
-      if (row >= C) continue;
+      const int idx = tid + i * NT, row = idx / (DC / V), col = idx % (DC / V) * V;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        odd |= not_finite((float)xc[i].e[e]);
-        s.c[row * LC + col + e] = (L)(float)xc[i].e[e];
-      }
+      for (int e = 0; e < V; ++e) odd |= not_finite((float)xc[i].e[e]);
+      if (row < C) put_chunk(s.c + row * LC + col, xc[i]);
+    }
+    if (tid < C) {
+      s.weight[tid] = tid < n && !cut_out && episode(tid) == e_last ? p.us * power(n - p.e0 - tid) : 0.f;
+      s.enter[tid] = tid < n && episode(tid) == 0 ? p.is * power(tid + p.e0) : 0.f;
     }
     if constexpr (!STATE) {
 #pragma unroll
-      for (int i = 0; i < NR; ++i)
+      for (int i = 0; i < RR; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s.r[(tc(i) * 16 + colx) * LA + tr(i) * 16 + row4 + e] = (L)acc[i][e];
+        for (int j = 0; j < RC; ++j) put4(s.r + ((rc0 + j) * 16 + colx) * LA + (r0 + i) * 16 + row4, acc[i][j]);
     }
     // A zero weight times infinity would be NaN: a chunk whose c holds one goes term by term.
     const bool by_term = __syncthreads_or(odd);
     if (q0 + C < last) load(q0 + C);
 
     if constexpr (!STATE) {
-      // P, weighted: wave w has the row tile w of 4 (C = 64), or one tile of 2 x 2 (C = 32)
-      constexpr int NP = CT * CT / 4;
+      // P^T for this wave's tokens; the OC waves that share them take every OC-th tile of the columns
+      f32x4 x[TR][TC];
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        const int ti = (wave * NP + i) / CT, tj = (wave * NP + i) % CT;
-        f32x4 x = {};
-        if (tj <= ti)
-          for (int k = 0; k < DA; k += KS) x = mma16(frag_kc(s.a, LA, ti * 16, k, lane), frag_kc(s.b, LA, tj * 16, k, lane), x);
-        const int j = tj * 16 + colx, ej = episode(j);
+      for (int t = 0; t < TR; ++t) {
+        const int i = (t0 + t) * 16 + colx, ei = episode(i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = ti * 16 + row4 + e;
-          s.p[r * LP + j] = (L)(j <= r && r < n && ej == episode(r) ? p.ps * s.power[r - j] * x[e] : 0.f);
-        }
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < NO; ++i) {
-        const int ti = (wave * NO + i) / (DC / 16), tj = (wave * NO + i) % (DC / 16);
-        f32x4 x = {};
-        for (int k = 0; k < DA; k += KS) x = mma16(frag_kc(s.a, LA, ti * 16, k, lane), frag_kc(s.r, LA, tj * 16, k, lane), x);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = ti * 16 + row4 + e;
-          x[e] = r < n && episode(r) == 0 ? p.is * s.power[r + p.e0] * x[e] : 0.f;
-        }
-        if (!by_term) {
-          for (int k = 0; k < (ti + 1) * 16; k += KS) x = mma16(frag_kc(s.p, LP, ti * 16, k, lane), frag_kr(s.c, LC, tj * 16, k, lane), x);
-        } else {
-          for (int j = 0; j < n; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int r = ti * 16 + row4 + e;
-              if (j <= r && r < n && episode(j) == episode(r)) x[e] += (float)s.p[r * LP + j] * (float)s.c[j * LC + tj * 16 + colx];
-            }
-        }
-        if (tj * 16 + colx < p.dc) {
+        for (int jj = 0; jj < CT / OC + (CT % OC ? 1 : 0); ++jj) {
+          const int tj = jj * OC + wave % OC;
+          if (tj >= CT) continue;
+          f32x4 y = {};
+          if (tj <= t0 + t) y = with_a(s.b, tj * 16, t, y);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const long long q = q0 + ti * 16 + row4 + e;
-            if (q < p.length) go[token(q) * p.o_t + tj * 16 + colx] = (T)x[e];  // (behind the end x is 0)
+            const int j = tj * 16 + row4 + e;
+            y[e] = j <= i && i < n && (whole || episode(j) == ei) ? p.ps * power(i - j) * y[e] : 0.f;
+          }
+          put4(s.p + i * LP + tj * 16 + row4, y);
+        }
+#pragma unroll
+        for (int c = 0; c < TC; ++c) {
+          x[t][c] = with_a(s.r, (c0 + c) * 16, t, f32x4{});
+          const float f = s.enter[i];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[t][c][e] = f == 0.f ? 0.f : f * x[t][c][e];
+        }
+      }
+      if (q0 + C < last) load_a(q0 + C);
+      __syncthreads();
+      if (!by_term) {
+#pragma unroll
+        for (int t = 0; t < TR; ++t)
+          for (int k = 0; k < (t0 + t + 1) * 16; k += KS) {
+            const auto fp = frag_kc(s.p, LP, (t0 + t) * 16, k, lane);
+#pragma unroll
+            for (int c = 0; c < TC; ++c) x[t][c] = mma16(frag_kr(s.c, LC, (c0 + c) * 16, k, lane), fp, x[t][c]);
+          }
+      } else {
+#pragma unroll
+        for (int t = 0; t < TR; ++t) {
+          const int i = (t0 + t) * 16 + colx, ei = episode(i);
+          for (int j = 0; j <= i && i < n; ++j)
+            if (episode(j) == ei) {
+              const float w = (float)s.p[i * LP + j];
+#pragma unroll
+              for (int c = 0; c < TC; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[t][c][e] += w * (float)s.c[j * LC + (c0 + c) * 16 + row4 + e];
+            }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < TR; ++t) {
+        const long long q = q0 + (t0 + t) * 16 + colx;
+        if (q >= p.length) continue;
+        T* at = go + token(q) * p.o_t;  // (behind the end x is 0)
+#pragma unroll
+        for (int c = 0; c < TC; ++c) {
+          const int d = (c0 + c) * 16 + row4;
+          T o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = (T)x[t][c][e];
+          if (FULL || d + 4 <= p.dc) __builtin_memcpy(at + d, o, sizeof(o));
+          else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (d + e < p.dc) at[d + e] = o[e];
           }
         }
       }
     }
 
-    const float through = s.power[n];
-    factor = carries ? factor * through : 0.f;
+    const float through = carries ? power(n) : 0.f;
+    factor *= through;
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
+    for (int i = 0; i < RR; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[i][e] = carries ? through * acc[i][e] : 0.f;
-      if (!by_term) {
-        for (int k = 0; k < C; k += KS) acc[i] = mma16(frag_kr(s.bw, LA, tr(i) * 16, k, lane), frag_kr(s.c, LC, tc(i) * 16, k, lane), acc[i]);
-      } else {
-        for (int j = 0; j < n; ++j)
-          if (weight(j) != 0.f) {
+      for (int j = 0; j < RC; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (tr(i) * 16 + row4 + e < p.da) acc[i][e] += (float)s.bw[j * LA + tr(i) * 16 + row4 + e] * (float)s.c[j * LC + tc(i) * 16 + colx];
-          }
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = carries ? through * acc[i][j][e] : 0.f;
+    if (!by_term) {
+#pragma unroll 2
+      for (int k = 0; k < C; k += KS) {
+        decltype(frag_kr(s.b, LA, 0, 0, lane)) fb[RR];
+#pragma unroll
+        for (int i = 0; i < RR; ++i) fb[i] = weigh(frag_kr(s.b, LA, (r0 + i) * 16, k, lane), s.weight, k, lane);
+#pragma unroll
+        for (int j = 0; j < RC; ++j) {
+          const auto fc = frag_kr(s.c, LC, (rc0 + j) * 16, k, lane);
+#pragma unroll
+          for (int i = 0; i < RR; ++i) acc[i][j] = mma16(fb[i], fc, acc[i][j]);
+        }
+      }
+    } else {
+      for (int t = 0; t < n; ++t) {
+        const float w = s.weight[t];
+        if (w == 0.f) continue;
+#pragma unroll
+        for (int i = 0; i < RR; ++i)
+#pragma unroll
+          for (int j = 0; j < RC; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = (r0 + i) * 16 + row4 + e;
+              if (FULL || r < p.da) acc[i][j][e] += (float)(L)(w * (float)s.b[t * LA + r]) * (float)s.c[t * LC + (rc0 + j) * 16 + colx];
+            }
       }
     }
   }
@@ -246,12 +382,14 @@ template <typename T, int DA, int DC, bool STATE> __global__ __launch_bounds__(2
   float* end = STATE ? p.seg_state + (sh * (p.segments - 1) + seg) * p.da * p.dc : seg == p.segments - 1 && p.state_out ? p.state_out + sh * p.da * p.dc : nullptr;
   if (end) {
 #pragma unroll
-    for (int i = 0; i < NR; ++i)
+    for (int i = 0; i < RR; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = tr(i) * 16 + row4 + e, c = tc(i) * 16 + colx;
-        if (r < p.da && c < p.dc) end[(long long)r * p.dc + c] = acc[i][e];
-      }
+      for (int j = 0; j < RC; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = (r0 + i) * 16 + row4 + e, c = (rc0 + j) * 16 + colx;
+          if (FULL || (r < p.da && c < p.dc)) end[(long long)r * p.dc + c] = acc[i][j][e];
+        }
   }
   if (STATE && tid == 0) p.seg_factor[sh * (p.segments - 1) + seg] = factor;
 }

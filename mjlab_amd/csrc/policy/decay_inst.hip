@@ -22,22 +22,26 @@ Split split(long long batch, int heads, long long length) {
 long long up256(long long x) { return (x + 255) & ~255LL; }
 long long state_bytes(const mjlab_decay_t* d, const Split& s) { return up256(d->batch * d->heads * (s.segments - 1) * (long long)d->dk * d->dv * 4); }
 
-template <int DA, int DC> hipError_t launch_pass(const DecayPass& p, long long rows, hipStream_t st) {
-  constexpr int LDS = (int)sizeof(DecayLds<T, DA, DC>);
+template <int DA, int DC, bool FULL> hipError_t launch_sized(const DecayPass& p, long long rows, hipStream_t st) {
+  constexpr int LDS = (int)sizeof(DecayLds<T, DA, DC, false>), LDS_FIRST = (int)sizeof(DecayLds<T, DA, DC, true>);
   hipError_t e;
   if (rows * p.segments > MAX_BLOCKS) return hipErrorInvalidValue;
   if (p.segments > 1) {
-    auto first = k_decay_chunks<T, DA, DC, true>;
-    if ((e = allow_lds(first, LDS)) != hipSuccess) return e;
-    hipLaunchKernelGGL(first, dim3((unsigned)(rows * (p.segments - 1))), dim3(256), LDS, st, p);
+    auto first = k_decay_chunks<T, DA, DC, FULL, true>;
+    if ((e = allow_lds(first, LDS_FIRST)) != hipSuccess) return e;
+    hipLaunchKernelGGL(first, dim3((unsigned)(rows * (p.segments - 1))), dim3(decay_threads(DA, DC)), LDS_FIRST, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     hipLaunchKernelGGL(k_decay_scan<T>, dim3((unsigned)(rows * ((p.da * p.dc + 255) / 256))), dim3(256), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  auto kern = k_decay_chunks<T, DA, DC, false>;
+  auto kern = k_decay_chunks<T, DA, DC, FULL, false>;
   if ((e = allow_lds(kern, LDS)) != hipSuccess) return e;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(rows * p.segments)), dim3(256), LDS, st, p);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(rows * p.segments)), dim3(decay_threads(DA, DC)), LDS, st, p);
   return hipGetLastError();
+}
+
+template <int DA, int DC> hipError_t launch_pass(const DecayPass& p, long long rows, hipStream_t st) {
+  return p.da == DA && p.dc == DC ? launch_sized<DA, DC, true>(p, rows, st) : launch_sized<DA, DC, false>(p, rows, st);
 }
 
 template <int DA> hipError_t launch_dc(const DecayPass& p, long long rows, hipStream_t st) {

@@ -14,12 +14,14 @@ template <bool AK, bool BK, int BM, int BN, int EPI> hipError_t launch_tile(cons
   return hipGetLastError();
 }
 
-// The largest tile of which there is one per CU.
+// The tile by how many of them there are for the 256 CUs.  Measured (us; 256 x 128 / 128 x 128 / 64 x 64): bf16 16384 x 2048 x 2816 237 / 253 / 352,
+// 24576 x 1024 x 1024 (3 large tiles per CU) 78 / 76 / 104, 4096 x 1024 x 1024 35 / 22 / 24; float 24576 x 1024 x 1024 - / 278 / 368,
+// 4096 x 1024 x 1024 (1 per CU) - / 72 / 70, 4096 x 512 x 256 - / 36 / 19, 512 x 2048 x 2048 - / 116 / 52.
 template <bool AK, bool BK, int EPI> hipError_t launch_product(const Product& p, int splits, hipStream_t st) {
-  const long long nout = EPI == EPI_GATED ? 2 * p.N : p.N, tn = (nout + 127) / 128;
+  const long long nout = EPI == EPI_GATED ? 2 * p.N : p.N, tn = (nout + 127) / 128 * splits;
   if constexpr (sizeof(T) == 2)
-    if ((p.M + 255) / 256 * tn * splits >= CUS) return launch_tile<AK, BK, 256, 128, EPI>(p, splits, st);
-  if ((p.M + 127) / 128 * tn * splits >= CUS) return launch_tile<AK, BK, 128, 128, EPI>(p, splits, st);
+    if ((p.M + 255) / 256 * tn >= 4 * CUS) return launch_tile<AK, BK, 256, 128, EPI>(p, splits, st);
+  if ((p.M + 127) / 128 * tn * 2 >= 3 * CUS) return launch_tile<AK, BK, 128, 128, EPI>(p, splits, st);
   return launch_tile<AK, BK, 64, 64, EPI>(p, splits, st);
 }
 
@@ -83,7 +85,7 @@ hipError_t POLICY_NAME(mjlab_launch_layer_backward)(const mjlab_layer_grad_t* g,
     constexpr int V = Elem<T>::VEC;
     const long long colblocks = (f.out + 32 * V - 1) / (32 * V);
     if (colblocks * q.blocks > MAX_BLOCKS) return hipErrorInvalidValue;
-    auto kern = q.gated ? k_layer_slope<T, true> : k_layer_slope<T, false>;
+    auto kern = q.gated ? k_layer_slope<T, true, false> : f.z_is_y ? k_layer_slope<T, false, true> : k_layer_slope<T, false, false>;
     hipLaunchKernelGGL(kern, dim3((unsigned)(colblocks * q.blocks)), dim3(256), 0, st, (const T*)g->dy, g->ld_dy, (const T*)f.z, (const T*)f.z_up, q.slope ? dz : nullptr, sums, f.rows, f.out, (unsigned)colblocks, f.act);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     if (q.sums) {

@@ -1,4 +1,5 @@
 // policy.hip -- C ABI of include/mjlab_policy.h: argument checks and the choice of the element type; the kernels live in layer_inst.hip.
+#include "policy_common.h"
 #include "policy_launch.h"
 
 #include <cstdio>
@@ -58,6 +59,7 @@ int mjlab_layer_backward(const mjlab_layer_grad_t* g, void* stream) {
   const bool gated = g->f.w_up != nullptr;
   if (!g->dy) return fail(-2, "layer_backward: null dy");
   if ((gated || g->f.act != MJLAB_ACT_NONE) && !g->f.z) return fail(-2, "layer_backward: the sums before the activation (z) are missing");
+  if (g->f.z_is_y && (gated || !slope_from_output(g->f.act))) return fail(-2, "layer_backward: z_is_y: the output does not determine this layer's slope");
   if (gated && !g->f.z_up) return fail(-2, "layer_backward: z_up is missing");
   if (gated && ((g->dw != nullptr) != (g->dw_up != nullptr) || (g->db != nullptr) != (g->db_up != nullptr))) return fail(-2, "layer_backward: dw / dw_up and db / db_up come together");
   const long long need = BY_TYPE(g->f.dtype, mjlab_layer_backward_bytes, g);

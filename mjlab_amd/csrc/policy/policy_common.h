@@ -73,30 +73,51 @@ __device__ __forceinline__ float normal_cdf(float z, float e) {
   return z < 0.f ? tail : 1.f - tail;
 }
 
-__device__ __forceinline__ float act_value(float z, int act) {
-  switch (act) {
-    case MJLAB_ACT_RELU: return z < 0.f ? 0.f : z;
-    case MJLAB_ACT_ELU: return z > 0.f ? z : expm1_neg(z);
-    case MJLAB_ACT_TANH: return tanh_f(z);
-    case MJLAB_ACT_SIGMOID: return sigmoid_f(z);
-    case MJLAB_ACT_SILU: return z * sigmoid_f(z);
-    case MJLAB_ACT_GELU: return z * normal_cdf(z, __expf(-0.5f * z * z));
-    default: return z;
-  }
+template <int ACT> __device__ __forceinline__ float act_value(float z) {
+  if constexpr (ACT == MJLAB_ACT_RELU) return z < 0.f ? 0.f : z;
+  if constexpr (ACT == MJLAB_ACT_ELU) return z > 0.f ? z : expm1_neg(z);
+  if constexpr (ACT == MJLAB_ACT_TANH) return tanh_f(z);
+  if constexpr (ACT == MJLAB_ACT_SIGMOID) return sigmoid_f(z);
+  if constexpr (ACT == MJLAB_ACT_SILU) return z * sigmoid_f(z);
+  if constexpr (ACT == MJLAB_ACT_GELU) return z * normal_cdf(z, __expf(-0.5f * z * z));
+  return z;
 }
 
 // Derivative at z.  Beyond |z| = 100 the derivative of each is its limit to all 24 bits: z is cut there, so that a z that 16 bits hold
 // as infinite gives the limit and not infinity times zero.
-__device__ __forceinline__ float act_slope(float z, int act) {
+template <int ACT> __device__ __forceinline__ float act_slope(float z) {
   z = z > 100.f ? 100.f : (z < -100.f ? -100.f : z);
+  if constexpr (ACT == MJLAB_ACT_RELU) return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
+  if constexpr (ACT == MJLAB_ACT_ELU) return z > 0.f ? 1.f : __expf(z);
+  if constexpr (ACT == MJLAB_ACT_TANH) { const float e = __expf(-2.f * __builtin_fabsf(z)), r = rcp_f(1.f + e); return 4.f * e * r * r; }
+  if constexpr (ACT == MJLAB_ACT_SIGMOID) { const float e = __expf(-__builtin_fabsf(z)), r = rcp_f(1.f + e); return e * r * r; }
+  if constexpr (ACT == MJLAB_ACT_SILU) { const float s = sigmoid_f(z); return s * (1.f + z * (1.f - s)); }
+  if constexpr (ACT == MJLAB_ACT_GELU) { const float e = __expf(-0.5f * z * z); return normal_cdf(z, e) + z * 0.39894228f * e; }
+  return 1.f;
+}
+
+// The derivative from the output y of a layer without residual, where y determines it (off by 2^-24 of 1 where y is float)
+__host__ __device__ constexpr bool slope_from_output(int act) { return act == MJLAB_ACT_RELU || act == MJLAB_ACT_ELU || act == MJLAB_ACT_TANH || act == MJLAB_ACT_SIGMOID; }
+template <int ACT> __device__ __forceinline__ float act_slope_out(float y) {
+  if constexpr (ACT == MJLAB_ACT_RELU) return y > 0.f ? 1.f : (y <= 0.f ? 0.f : y);
+  if constexpr (ACT == MJLAB_ACT_ELU) return y > 0.f ? 1.f : 1.f + y;
+  if constexpr (ACT == MJLAB_ACT_TANH) return 1.f - y * y;
+  return y * (1.f - y);  // (sigmoid)
+}
+
+// One uniform branch for a whole block of elements: f(Act<..>) with the activation as a type
+template <int A> struct Act {
+  static constexpr int value = A;
+};
+template <typename F> __device__ __forceinline__ void with_act(int act, F f) {
   switch (act) {
-    case MJLAB_ACT_RELU: return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
-    case MJLAB_ACT_ELU: return z > 0.f ? 1.f : __expf(z);
-    case MJLAB_ACT_TANH: { const float e = __expf(-2.f * __builtin_fabsf(z)), r = rcp_f(1.f + e); return 4.f * e * r * r; }
-    case MJLAB_ACT_SIGMOID: { const float e = __expf(-__builtin_fabsf(z)), r = rcp_f(1.f + e); return e * r * r; }
-    case MJLAB_ACT_SILU: { const float s = sigmoid_f(z); return s * (1.f + z * (1.f - s)); }
-    case MJLAB_ACT_GELU: { const float e = __expf(-0.5f * z * z); return normal_cdf(z, e) + z * 0.39894228f * e; }
-    default: return 1.f;
+    case MJLAB_ACT_RELU: f(Act<MJLAB_ACT_RELU>()); break;
+    case MJLAB_ACT_ELU: f(Act<MJLAB_ACT_ELU>()); break;
+    case MJLAB_ACT_TANH: f(Act<MJLAB_ACT_TANH>()); break;
+    case MJLAB_ACT_SIGMOID: f(Act<MJLAB_ACT_SIGMOID>()); break;
+    case MJLAB_ACT_SILU: f(Act<MJLAB_ACT_SILU>()); break;
+    case MJLAB_ACT_GELU: f(Act<MJLAB_ACT_GELU>()); break;
+    default: f(Act<MJLAB_ACT_NONE>());
   }
 }
 

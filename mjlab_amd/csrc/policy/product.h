@@ -313,50 +313,77 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
       if (GATED && p.b_up && e < left) bias_up[e] = (float)((const T*)p.b_up)[n + e];
     }
   }
+  constexpr int PASSES = 32 / RPP;
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
+    // the residual's rows are on their way while C goes through LDS
+    Chunk<T> res[EPI == EPI_LAYER ? PASSES : 1];
+    if constexpr (EPI == EPI_LAYER) {
+      if (p.r) {
+#pragma unroll
+        for (int q = 0; q < PASSES; ++q) {
+          const long long m = m0 + wm + i * 32 + q * RPP + lane / LPR;
+          res[q] = load_part((const T*)p.r + m * p.ldr + n, m < p.M ? left : 0);
+        }
+      }
+    }
     if (i) __syncthreads();
 #pragma unroll
     for (int j = 0; j < NI; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) c[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * LD + j * 32 + (lane & 31)] = acc[i][j][e];
     __syncthreads();
+    float v[PASSES][OV], u[GATED ? PASSES : 1][OV];
 #pragma unroll
-    for (int q = 0; q < 32 / RPP; ++q) {
-      const int row = q * RPP + lane / LPR;
-      const long long m = m0 + wm + i * 32 + row;
-      if (m >= p.M || left <= 0) continue;
-      float v[OV];
+    for (int q = 0; q < PASSES; ++q)
 #pragma unroll
-      for (int e = 0; e < OV; ++e) v[e] = c[row * LD + col + e];
-      if constexpr (EPI == EPI_PARTIAL) {
+      for (int e = 0; e < OV; ++e) {
+        v[q][e] = c[(q * RPP + lane / LPR) * LD + col + e] + bias[e];
+        if constexpr (GATED) u[q][e] = c[(q * RPP + lane / LPR) * LD + HALF + col + e] + bias_up[e];
+      }
+    auto rows = [&](auto f) {  // f(pass, row of C) for the rows that there are
+#pragma unroll
+      for (int q = 0; q < PASSES; ++q) {
+        const long long m = m0 + wm + i * 32 + q * RPP + lane / LPR;
+        if (m < p.M && left > 0) f(q, m);
+      }
+    };
+    if constexpr (EPI == EPI_PARTIAL) {
+      rows([&](int q, long long m) {
         Chunk<float> out;
 #pragma unroll
-        for (int e = 0; e < OV; ++e) out.e[e] = v[e];
+        for (int e = 0; e < OV; ++e) out.e[e] = v[q][e];
         store_part(p.partial + ((long long)blockIdx.y * p.M + m) * p.N + n, out, left);
-      } else if constexpr (EPI == EPI_STORE) {
+      });
+    } else {
+      auto put = [&](void* base, long long ld, int q, long long m, const float (&x)[OV]) {
         Chunk<T> out;
 #pragma unroll
-        for (int e = 0; e < OV; ++e) out.e[e] = (T)v[e];
-        store_part((T*)p.y + m * p.ldy + n, out, left);
-      } else {
-        Chunk<T> out, zs;
+        for (int e = 0; e < OV; ++e) out.e[e] = (T)x[e];
+        store_part((T*)base + m * ld + n, out, left);
+      };
+      if constexpr (EPI != EPI_STORE) {
+        if (p.z) rows([&](int q, long long m) { put(p.z, p.N, q, m, v[q]); });
+        with_act(p.act, [&](auto act) {
 #pragma unroll
-        for (int e = 0; e < OV; ++e) { v[e] += bias[e]; zs.e[e] = (T)v[e]; v[e] = act_value(v[e], p.act); }
-        if (p.z) store_part((T*)p.z + m * p.N + n, zs, left);
+          for (int q = 0; q < PASSES; ++q)
+#pragma unroll
+            for (int e = 0; e < OV; ++e) v[q][e] = act_value<decltype(act)::value>(v[q][e]);
+        });
         if constexpr (GATED) {
+          if (p.z_up) rows([&](int q, long long m) { put(p.z_up, p.N, q, m, u[q]); });
 #pragma unroll
-          for (int e = 0; e < OV; ++e) { const float u = c[row * LD + HALF + col + e] + bias_up[e]; zs.e[e] = (T)u; v[e] *= u; }
-          if (p.z_up) store_part((T*)p.z_up + m * p.N + n, zs, left);
+          for (int q = 0; q < PASSES; ++q)
+#pragma unroll
+            for (int e = 0; e < OV; ++e) v[q][e] *= u[q][e];
         } else if (p.r) {
-          const Chunk<T> r = load_part((const T*)p.r + m * p.ldr + n, left);
 #pragma unroll
-          for (int e = 0; e < OV; ++e) v[e] += (float)r.e[e];
+          for (int q = 0; q < PASSES; ++q)
+#pragma unroll
+            for (int e = 0; e < OV; ++e) v[q][e] += (float)res[q].e[e];
         }
-#pragma unroll
-        for (int e = 0; e < OV; ++e) out.e[e] = (T)v[e];
-        store_part((T*)p.y + m * p.ldy + n, out, left);
       }
+      rows([&](int q, long long m) { put(p.y, p.ldy, q, m, v[q]); });
     }
   }
 }
@@ -372,44 +399,57 @@ template <typename T> __global__ __launch_bounds__(256) void k_join_splits(const
 }
 
 // dz (rows, out | 2 out) from dy and the stored sums, and this row block's column sums for the bias gradient.
-// 256 threads: 32 chunk columns x 8 rows at a time over SLOPE_ROWS rows; workgroups: row blocks x `colblocks`.  dz NULL: column sums of dy alone.
-#define SLOPE_ROWS 128
-template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_layer_slope(const T* dy, long long ld_dy, const T* z, const T* z_up, T* dz, float* sums,
-                                                                                        long long rows, long long out, unsigned colblocks, int act) {
-  constexpr int V = Elem<T>::VEC, NS = GATED ? 2 : 1;
+// 256 threads: 32 chunk columns x 8 rows, four rows of each thread in flight, over SLOPE_ROWS rows; workgroups: row blocks x `colblocks`.
+// dz NULL: column sums of dy alone.  FROM: what is stored is the layer's output.  Bound by memory: dense two reads and a write, gated three and two.
+#define SLOPE_ROWS 64
+template <typename T, bool GATED, bool FROM> __global__ __launch_bounds__(256) void k_layer_slope(const T* dy, long long ld_dy, const T* z, const T* z_up, T* dz,
+                                                                                                   float* sums, long long rows, long long out, unsigned colblocks, int act) {
+  constexpr int V = Elem<T>::VEC, NS = GATED ? 2 : 1, ROWS = GATED ? 1 : 2;
   __shared__ float part[NS][8][32 * V];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const unsigned bx = blockIdx.x % colblocks, by = blockIdx.x / colblocks;
   const long long n = (bx * 32LL + tx) * V, left = out - n, r0 = by * (long long)SLOPE_ROWS;
   float s[NS][V] = {};
-  if (left > 0)
-    for (int i = ty; i < SLOPE_ROWS && r0 + i < rows; i += 8) {
-      const long long m = r0 + i;
-      const Chunk<T> d = load_part(dy + m * ld_dy + n, left);
-      Chunk<T> o, o2;
-      if (dz && (GATED || act != MJLAB_ACT_NONE)) {
-        const Chunk<T> g = load_part(z + m * out + n, left);
-        Chunk<T> u;
-        if constexpr (GATED) u = load_part(z_up + m * out + n, left);
+  const bool slope = dz && (GATED || act != MJLAB_ACT_NONE);
+  for (int i = ty; i < SLOPE_ROWS && r0 + i < rows; i += 8 * ROWS) {
+    Chunk<T> d[ROWS], g[ROWS], u[ROWS];
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float v = (float)d.e[e] * act_slope((float)g.e[e], act);
-          if constexpr (GATED) {
-            v *= (float)u.e[e];
-            const float w = (float)d.e[e] * act_value((float)g.e[e], act);
-            s[NS - 1][e] += w;
-            o2.e[e] = (T)w;
+    for (int q = 0; q < ROWS; ++q) {
+      const long long m = r0 + i + 8 * q, have = m < rows ? left : 0;
+      d[q] = load_part(dy + m * ld_dy + n, have);
+      if (slope) g[q] = load_part(z + m * out + n, have);
+      if constexpr (GATED) u[q] = load_part(z_up + m * out + n, have);
+    }
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) {
+      const long long m = r0 + i + 8 * q;
+      if (slope) {
+        with_act(act, [&](auto a) {
+          constexpr int ACT = decltype(a)::value;
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float x = (float)g[q].e[e], t = (float)d[q].e[e];
+            float v = t * (FROM ? act_slope_out<ACT>(x) : act_slope<ACT>(x));
+            if constexpr (GATED) {
+              v *= (float)u[q].e[e];
+              const float w = t * act_value<ACT>(x);
+              s[NS - 1][e] += w;
+              u[q].e[e] = (T)w;
+            }
+            s[0][e] += v;
+            d[q].e[e] = (T)v;
           }
-          s[0][e] += v;
-          o.e[e] = (T)v;
+        });
+        if (m < rows && left > 0) {
+          store_part(dz + m * (NS * out) + n, d[q], left);
+          if constexpr (GATED) store_part(dz + m * (NS * out) + out + n, u[q], left);
         }
-        store_part(dz + m * (NS * out) + n, o, left);
-        if constexpr (GATED) store_part(dz + m * (NS * out) + out + n, o2, left);
       } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[0][e] += (float)d.e[e];
+        for (int e = 0; e < V; ++e) s[0][e] += (float)d[q].e[e];
       }
     }
+  }
   if (!sums) return;
 #pragma unroll
   for (int q = 0; q < NS; ++q)
@@ -436,6 +476,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_join_sums(const f
   const long long c = blockIdx.x * 16LL + tx;
   float s = 0.f;
   if (c < cols)
+#pragma unroll 4
     for (long long b = ty; b < blocks; b += 16) s += sums[b * cols + c];
   part[ty][tx] = s;
   __syncthreads();

@@ -28,7 +28,7 @@ ACTIVATIONS = {"none": 0, "relu": 1, "elu": 2, "tanh": 3, "sigmoid": 4, "silu": 
 
 
 class Layer(ctypes.Structure):  # mjlab_layer_t
-  _fields_ = [("dtype", ctypes.c_int), ("act", ctypes.c_int), ("rows", _ll), ("inp", _ll), ("out", _ll),
+  _fields_ = [("dtype", ctypes.c_int), ("act", ctypes.c_int), ("z_is_y", ctypes.c_int), ("pad_", ctypes.c_int), ("rows", _ll), ("inp", _ll), ("out", _ll),
               ("x", _vp), ("w", _vp), ("w_up", _vp), ("b", _vp), ("b_up", _vp), ("r", _vp),
               ("ldx", _ll), ("ldw", _ll), ("ldw_up", _ll), ("ldr", _ll), ("ldy", _ll), ("y", _vp), ("z", _vp), ("z_up", _vp)]  # fmt: skip
 
@@ -89,12 +89,20 @@ def _layer_struct(x, w, w_up, b, b_up, act: int) -> Layer:
   return f
 
 
+# float32 layers whose slope the output gives store nothing else for the backward pass (16 bits: 1 + y and 1 - y^2 would cancel)
+_FROM_OUTPUT = {ACTIVATIONS[a] for a in ("relu", "elu", "tanh", "sigmoid")}
+
+
+def _from_output(x, w_up, r, act: int) -> bool:
+  return x.dtype == torch.float32 and w_up is None and r is None and act in _FROM_OUTPUT
+
+
 def _forward(x, w, w_up, b, b_up, r, act: int, keep: bool, y=None):
   """-> y, z, z_up (z: the sums before the activation where the backward pass will want them)."""
   m, n = x.shape[0], w.shape[0]
   if y is None:
     y = x.new_empty((m, n))
-  z = x.new_empty((m, n)) if keep and (act or w_up is not None) else None
+  z = x.new_empty((m, n)) if keep and (act or w_up is not None) and not _from_output(x, w_up, r, act) else None
   z_up = x.new_empty((m, n)) if keep and w_up is not None else None
   if m:
     f = _layer_struct(x, w, w_up, b, b_up, act)
@@ -112,8 +120,9 @@ class _Layer(torch.autograd.Function):
   @staticmethod
   def forward(ctx, x, w, w_up, b, b_up, r, act):
     y, z, z_up = _forward(x, w, w_up, b, b_up, r, act, keep=True)
-    ctx.save_for_backward(x, w, w_up, z, z_up)
-    ctx.act, ctx.has_bias = act, (b is not None, b_up is not None)
+    ctx.z_is_y = _from_output(x, w_up, r, act)
+    ctx.save_for_backward(x, w, w_up, y if ctx.z_is_y else z, z_up)
+    ctx.act = act
     return y
 
   @staticmethod
@@ -137,6 +146,7 @@ class _Layer(torch.autograd.Function):
     elif dx is not None or dw is not None or db is not None:
       g = LayerGrad()
       g.f = _layer_struct(x, w, w_up, None, None, ctx.act)
+      g.f.z_is_y = ctx.z_is_y
       g.f.z = None if z is None else z.data_ptr()
       g.f.z_up = None if z_up is None else z_up.data_ptr()
       g.dy, g.ld_dy = dy.data_ptr(), _ld(dy)

@@ -52,7 +52,7 @@ def test_layer_forward_refuses(kw, text):
 @pytest.mark.parametrize("kw,text", [
   (dict(dy=None), "null dy"), (dict(f=dict(z=None)), "(z)"), (dict(f=dict(w_up=64, ldw_up=8)), "z_up"),
   (dict(f=dict(w_up=64, ldw_up=8, z_up=64), dw=64), "together"), (dict(workspace_bytes=16), "workspace"), (dict(workspace=None), "workspace"),
-  (dict(f=dict(rows=-1)), "sizes"),
+  (dict(f=dict(rows=-1)), "sizes"), (dict(f=dict(act=5, z_is_y=1)), "z_is_y"),
 ])  # fmt: skip
 def test_layer_backward_refuses(kw, text):
   lib = native.policy_lib()
