@@ -68,6 +68,7 @@ template <typename T, int DA, int DC, bool STATE> struct DecayLds {
   static constexpr int C = DecayCfg<T>::C, PAD = DecayCfg<T>::PAD, LA = DA + PAD, LC = DC + PAD, LP = C + PAD;
   L b[C * LA], c[C * LC], p[STATE ? 1 : C * LP], r[STATE ? 1 : DC * LA];
   float weight[C], enter[C];  // of token j into R; of R into token i
+  int odd[8];
 };
 
 // VEC elements of T as elements of L, to an address aligned for them
@@ -103,22 +104,18 @@ __device__ __forceinline__ float weigh(float x, const float* w, int k0, int lane
   return t == 0.f ? 0.f : t * x;
 }
 
-// Elements col .. col + VEC - 1 of a row of d, zero from d on or where the row is not `live` (it exists all the same).  FULL: all of them are there.
-template <typename T, bool FULL> __device__ __forceinline__ Chunk<T> load_row(const T* row, int col, int d, bool live) {
-  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-  if constexpr (FULL) {
-    const u32x4 w = __builtin_bit_cast(u32x4, load_chunk(row + col)), zero = {0, 0, 0, 0};
-    return __builtin_bit_cast(Chunk<T>, live ? w : zero);
-  }
-  return load_part(row + col, live ? d - col : 0);
+// Elements col .. col + VEC - 1 of a row of d, zero from d on.  FULL: all of them are there.
+template <typename T, bool FULL> __device__ __forceinline__ Chunk<T> load_row(const T* at, int col, int d) {
+  if constexpr (FULL) return load_chunk(at);
+  else return load_part(at, d - col);
 }
+
+constexpr int decay_threads(int da, int dc) { return da >= 64 && dc >= 64 ? 512 : 256; }
 
 // 256 or 512 threads per (sequence, head, segment).  FULL: da = DA and dc = DC.  STATE: the first pass of a split sequence, the segment's contribution to R alone.
 // Products are formed such that an accumulator's four rows are neighbours in memory: P^T and out^T (columns are tokens), R (rows are da).
 // The rows of a go from memory to the matrix cores' registers without LDS: with them in LDS a 128 x 128 workgroup took 114 KB, and one of them per CU
 // could not hide its loads (2 x 8192 tokens x 8 heads of 128, bf16: 130 us for this kernel then).
-constexpr int decay_threads(int da, int dc) { return da >= 64 && dc >= 64 ? 512 : 256; }
-
 template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch_bounds__(decay_threads(DA, DC), 2) void k_decay_chunks(const DecayPass p) {
   using Cfg = DecayCfg<T>;
   using L = typename Cfg::L;
@@ -126,7 +123,7 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
   constexpr int C = Cfg::C, KS = Cfg::KS, LA = S::LA, LC = S::LC, LP = S::LP, V = Elem<T>::VEC, CT = C / 16, KA = DA / KS;
   constexpr int NT = decay_threads(DA, DC), NW = NT / 64, NB = (C * DA / V + NT - 1) / NT, NC = (C * DC / V + NT - 1) / NT;  // 16-byte chunks per thread
   // Waves: of out, OR x OC waves of TR x TC tiles (tokens x dc); of R, RW x NW / RW waves of RR x RC tiles (da x dc)
-  constexpr int OC = CT == 4 ? NW / 2 : (DC / 16 < NW ? DC / 16 : NW);
+  constexpr int OC = CT == 4 ? 2 : (DC / 16 < NW ? DC / 16 : NW);
   constexpr int OR = NW / OC, TR = CT / OR, TC = DC / 16 / OC, RW = NW == 8 && DA >= 64 ? 4 : 2, RR = DA / 16 / RW, RC = DC / 16 * RW / NW;
   static_assert(OR * OC == NW && OR * TR == CT && OC * TC == DC / 16 && RR >= 1 && RC >= 1 && RR * RW == DA / 16 && RC * (NW / RW) == DC / 16, "tiles do not cover");
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -146,21 +143,32 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
   const T *ga = (const T*)p.a + seq * p.a_b + head * p.a_h, *gb = (const T*)p.b + seq * p.b_b + head * p.b_h, *gc = (const T*)p.c + seq * p.c_b + head * p.c_h;
   T* go = (T*)p.out + seq * p.o_b + head * p.o_h;
   auto token = [&](long long q) { return p.reverse && q < len ? len - 1 - q : q; };
-  auto there = [&](long long q) { return token(q < p.length ? q : p.length - 1); };  // a row that exists, for rows that are read but not used
 
+  // Where this thread's rows of the present chunk lie; one chunk on is `step` tokens on.
+  const long long first = (long long)seg * p.seg_chunks * C;
+  const long long last = first + (long long)p.seg_chunks * C < p.length ? first + (long long)p.seg_chunks * C : p.length;
+  const long long step = p.reverse ? -C : C;
   Chunk<T> xb[NB], xc[NC];
+  const T *pb[NB], *pc[NC];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) pb[i] = gb + token(first + (tid + i * NT) / (DA / V)) * p.b_t + (tid + i * NT) % (DA / V) * V;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) pc[i] = gc + token(first + (tid + i * NT) / (DC / V)) * p.c_t + (tid + i * NT) % (DC / V) * V;
   auto load = [&](long long q0) {
+    const bool all = q0 + C <= len;  // (uniform)
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      const int idx = tid + i * NT, row = idx / (DA / V), col = idx % (DA / V) * V;
-      const long long q = q0 + row;
-      xb[i] = load_row<T, FULL>(gb + there(q) * p.b_t, col, p.da, row < C && q < len);
+      const int row = (tid + i * NT) / (DA / V), col = (tid + i * NT) % (DA / V) * V;
+      if ((all && C * DA / V % NT == 0) || (row < C && q0 + row < len)) xb[i] = load_row<T, FULL>(pb[i], col, p.da);
+      else xb[i] = Chunk<T>{};
+      pb[i] += step * p.b_t;
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int idx = tid + i * NT, row = idx / (DC / V), col = idx % (DC / V) * V;
-      const long long q = q0 + row;
-      xc[i] = load_row<T, FULL>(gc + there(q) * p.c_t, col, p.dc, row < C && q < len);
+      const int row = (tid + i * NT) / (DC / V), col = (tid + i * NT) % (DC / V) * V;
+      if ((all && C * DC / V % NT == 0) || (row < C && q0 + row < len)) xc[i] = load_row<T, FULL>(pc[i], col, p.dc);
+      else xc[i] = Chunk<T>{};
+      pc[i] += step * p.c_t;
     }
   };
   // The rows of a of this wave's tokens.  16 bits: fragments as they are.  float: four k-steps come as 16 bytes, lane group by lane group, so the k order of
@@ -168,21 +176,34 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
   constexpr bool F32 = sizeof(L) == 4;
   typename std::conditional<F32, f32x4, s16x8>::type fa[TR][F32 ? DA / 16 : KA];
   auto a_k = [&](int i) { return sizeof(T) == 4 ? i * 16 + row4 : i / 2 * 32 + 2 * row4 + (i & 1) * 4; };  // first k of this lane in fa[.][i]
+  const T* pa[TR];
+  T* po[TR];
+#pragma unroll
+  for (int t = 0; t < TR; ++t) {
+    const long long k = token(first + (t0 + t) * 16 + colx);
+    pa[t] = ga + k * p.a_t;
+    po[t] = go + k * p.o_t + row4;
+  }
   auto load_a = [&](long long q0) {
 #pragma unroll
     for (int t = 0; t < TR; ++t) {
-      const long long q = q0 + (t0 + t) * 16 + colx;
-      const T* row = ga + there(q) * p.a_t;
+      const T* row = pa[t];
+      pa[t] += step * p.a_t;
+      const bool live = q0 + (t0 + t) * 16 + colx < len;
       if constexpr (!F32) {
 #pragma unroll
-        for (int k = 0; k < KA; ++k) fa[t][k] = __builtin_bit_cast(s16x8, load_row<T, FULL>(row, k * KS + (lane >> 4) * 8, p.da, q < len));
+        for (int k = 0; k < KA; ++k) {
+          const int col = k * KS + (lane >> 4) * 8;
+          fa[t][k] = live ? __builtin_bit_cast(s16x8, load_row<T, FULL>(row + col, col, p.da)) : s16x8{};
+        }
       } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < DA / 16; ++i) fa[t][i] = __builtin_bit_cast(f32x4, load_row<T, FULL>(row, i * 16 + row4, p.da, q < len));
+        for (int i = 0; i < DA / 16; ++i) fa[t][i] = live ? __builtin_bit_cast(f32x4, load_row<T, FULL>(row + i * 16 + row4, i * 16 + row4, p.da)) : f32x4{};
       } else {
 #pragma unroll
-        for (int i = 0; i < DA / 32; ++i) {  // (a chunk of eight holds two neighbouring steps: the k order is that of with_a below)
-          const Chunk<T> c = load_row<T, FULL>(row, i * 32 + 2 * row4, p.da, q < len);
+        for (int i = 0; i < DA / 32; ++i) {
+          const int col = i * 32 + 2 * row4;
+          const Chunk<T> c = live ? load_row<T, FULL>(row + col, col, p.da) : Chunk<T>{};
 #pragma unroll
           for (int e = 0; e < 4; ++e) { fa[t][2 * i][e] = (float)c.e[e]; fa[t][2 * i + 1][e] = (float)c.e[4 + e]; }
         }
@@ -219,8 +240,7 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
         acc[i][j][e] = start && (FULL || (r < p.da && c < p.dc)) ? start[(long long)r * sr + c * sc] : 0.f;
       }
 
-  const long long first = (long long)seg * p.seg_chunks * C;
-  const long long last = first + (long long)p.seg_chunks * C < p.length ? first + (long long)p.seg_chunks * C : p.length;
+  float* end = STATE ? p.seg_state + (sh * (p.segments - 1) + seg) * p.da * p.dc : seg == p.segments - 1 && p.state_out ? p.state_out + sh * p.da * p.dc : nullptr;
   float factor = 1.f;
   if (first < last) {
     load(first);
@@ -259,14 +279,21 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
       s.weight[tid] = tid < n && !cut_out && episode(tid) == e_last ? p.us * power(n - p.e0 - tid) : 0.f;
       s.enter[tid] = tid < n && episode(tid) == 0 ? p.is * power(tid + p.e0) : 0.f;
     }
-    if constexpr (!STATE) {
+    const bool carry = start || q0 > first;  // else R is zero so far
+    if (!STATE && carry) {
 #pragma unroll
       for (int i = 0; i < RR; ++i)
 #pragma unroll
         for (int j = 0; j < RC; ++j) put4(s.r + ((rc0 + j) * 16 + colx) * LA + (r0 + i) * 16 + row4, acc[i][j]);
     }
     // A zero weight times infinity would be NaN: a chunk whose c holds one goes term by term.
-    const bool by_term = __syncthreads_or(odd);
+    const bool mine = __ballot(odd) != 0;
+    if (lane == 0) s.odd[wave] = mine;
+    __syncthreads();
+    int any = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) any |= s.odd[i];
+    const bool by_term = __builtin_amdgcn_readfirstlane(any) != 0;
     if (q0 + C < last) load(q0 + C);
 
     if constexpr (!STATE) {
@@ -287,13 +314,17 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
             y[e] = j <= i && i < n && (whole || episode(j) == ei) ? p.ps * power(i - j) * y[e] : 0.f;
           }
           put4(s.p + i * LP + tj * 16 + row4, y);
+          __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int c = 0; c < TC; ++c) {
-          x[t][c] = with_a(s.r, (c0 + c) * 16, t, f32x4{});
+          x[t][c] = f32x4{};
+          if (!carry) continue;
+          x[t][c] = with_a(s.r, (c0 + c) * 16, t, x[t][c]);
           const float f = s.enter[i];
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[t][c][e] = f == 0.f ? 0.f : f * x[t][c][e];
+          __builtin_amdgcn_sched_barrier(0);  // (or the fragments of every column are loaded at once, and registers spill)
         }
       }
       if (q0 + C < last) load_a(q0 + C);
@@ -305,6 +336,7 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
             const auto fp = frag_kc(s.p, LP, (t0 + t) * 16, k, lane);
 #pragma unroll
             for (int c = 0; c < TC; ++c) x[t][c] = mma16(frag_kr(s.c, LC, (c0 + c) * 16, k, lane), fp, x[t][c]);
+            __builtin_amdgcn_sched_barrier(0);
           }
       } else {
 #pragma unroll
@@ -323,24 +355,27 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
 #pragma unroll
       for (int t = 0; t < TR; ++t) {
         const long long q = q0 + (t0 + t) * 16 + colx;
+        // behind the sequence's end x is 0, and the rows there are in order whatever the direction
+        T* at = p.reverse && q >= len ? go + q * p.o_t + row4 : po[t];
+        po[t] += step * p.o_t;
         if (q >= p.length) continue;
-        T* at = go + token(q) * p.o_t;  // (behind the end x is 0)
 #pragma unroll
         for (int c = 0; c < TC; ++c) {
-          const int d = (c0 + c) * 16 + row4;
+          const int d = (c0 + c) * 16;
           T o[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] = (T)x[t][c][e];
-          if (FULL || d + 4 <= p.dc) __builtin_memcpy(at + d, o, sizeof(o));
+          if (FULL || d + row4 + 4 <= p.dc) __builtin_memcpy(at + d, o, sizeof(o));
           else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (d + e < p.dc) at[d + e] = o[e];
+              if (d + row4 + e < p.dc) at[d + e] = o[e];
           }
         }
       }
     }
 
+    if (!STATE && !end && q0 + C >= last) break;  // nobody wants R any more
     const float through = carries ? power(n) : 0.f;
     factor *= through;
 #pragma unroll
@@ -361,6 +396,7 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
 #pragma unroll
           for (int i = 0; i < RR; ++i) acc[i][j] = mma16(fb[i], fc, acc[i][j]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     } else {
       for (int t = 0; t < n; ++t) {
@@ -379,7 +415,6 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
     }
   }
 
-  float* end = STATE ? p.seg_state + (sh * (p.segments - 1) + seg) * p.da * p.dc : seg == p.segments - 1 && p.state_out ? p.state_out + sh * p.da * p.dc : nullptr;
   if (end) {
 #pragma unroll
     for (int i = 0; i < RR; ++i)

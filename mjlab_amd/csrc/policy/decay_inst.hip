@@ -8,13 +8,13 @@ struct Split {
   int segments, seg_chunks;
 };
 
-// Segments per sequence: one where the sequences fill the device (a workgroup each), else as many as give it two workgroups per CU, of four chunks
-// at least: the first pass reads two of the operands again and moves R through memory once per segment.
-Split split(long long batch, int heads, long long length) {
+// Segments per sequence: one where the sequences fill the device (a workgroup each), else as many as give it a workgroup per CU (two for small
+// heads), of four chunks at least: the first pass reads two of the operands again and moves R through memory once per segment.
+Split split(const mjlab_decay_t* d) {
   constexpr int C = DecayCfg<T>::C;
-  const long long chunks = (length + C - 1) / C, rows = batch * heads;
-  if (rows >= CUS || chunks < 8) return {1, (int)chunks};
-  const long long want = (2 * CUS + rows - 1) / rows, most = chunks / 4, s = want < most ? want : most;
+  const long long chunks = (d->length + C - 1) / C, rows = d->batch * d->heads, slots = d->dk > 64 && d->dv > 64 ? CUS : 2 * CUS;
+  if (2 * rows >= slots || chunks < 8) return {1, (int)chunks};
+  const long long want = slots / rows, most = chunks / 4, s = want < most ? want : most;
   const long long per = (chunks + s - 1) / s;
   return {(int)((chunks + per - 1) / per), (int)per};
 }
@@ -51,7 +51,7 @@ template <int DA> hipError_t launch_dc(const DecayPass& p, long long rows, hipSt
 // out = the pass over a, b (heads of da) and c (of dc); see decay.h
 hipError_t launch(const mjlab_decay_t* d, const mjlab_decay_rows_t& a, const mjlab_decay_rows_t& b, const mjlab_decay_rows_t& c, const mjlab_decay_rows_t& out, int da,
                   int dc, bool reverse, const float* state_in, bool turned, float* state_out, hipStream_t st) {
-  const Split s = split(d->batch, d->heads, d->length);
+  const Split s = split(d);
   DecayPass p = {};
   p.a = a.p; p.a_b = a.batch; p.a_t = a.time; p.a_h = a.head;
   p.b = b.p; p.b_b = b.batch; p.b_t = b.time; p.b_h = b.head;
@@ -76,7 +76,7 @@ template <int LPR> hipError_t launch_step(const mjlab_decay_t* d, hipStream_t st
 }  // namespace
 
 long long POLICY_NAME(mjlab_decay_bytes)(const mjlab_decay_t* d) {
-  const Split s = split(d->batch, d->heads, d->length);
+  const Split s = split(d);
   return s.segments > 1 ? state_bytes(d, s) + up256(d->batch * d->heads * (s.segments - 1) * 4) : 0;
 }
 
