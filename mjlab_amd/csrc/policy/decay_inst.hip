@@ -81,11 +81,13 @@ long long POLICY_NAME(mjlab_decay_bytes)(const mjlab_decay_t* d) {
 }
 
 hipError_t POLICY_NAME(mjlab_launch_decay_forward)(const mjlab_decay_t* d, hipStream_t st) {
+  if (d->length <= 32) return POLICY_NAME(mjlab_launch_short_forward)(d, st);
   return launch(d, d->q, d->k, d->v, d->o, d->dk, d->dv, false, d->state, false, d->state_out, st);
 }
 
 hipError_t POLICY_NAME(mjlab_launch_decay_backward)(const mjlab_decay_grad_t* g, hipStream_t st) {
   const mjlab_decay_t* d = &g->f;
+  if (d->length <= 32) return POLICY_NAME(mjlab_launch_short_backward)(g, st);
   hipError_t e;
   if (g->dq.p && (e = launch(d, g->d_out, d->v, d->k, g->dq, d->dv, d->dk, false, d->state, true, nullptr, st)) != hipSuccess) return e;
   if (g->dk.p && (e = launch(d, d->v, g->d_out, d->q, g->dk, d->dv, d->dk, true, g->d_state_out, true, nullptr, st)) != hipSuccess) return e;

@@ -1,4 +1,4 @@
-// policy_launch.h -- the per-type launch functions that layer_inst.hip and decay_inst.hip define and policy.hip dispatches to.
+// policy_launch.h -- the per-type launch functions that layer_inst.hip, decay_inst.hip and short_inst.hip define and policy.hip dispatches to.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -11,6 +11,8 @@
   long long mjlab_decay_bytes_##T(const mjlab_decay_t* d);                                   \
   hipError_t mjlab_launch_decay_forward_##T(const mjlab_decay_t* d, hipStream_t st);         \
   hipError_t mjlab_launch_decay_backward_##T(const mjlab_decay_grad_t* g, hipStream_t st);   \
+  hipError_t mjlab_launch_short_forward_##T(const mjlab_decay_t* d, hipStream_t st);         \
+  hipError_t mjlab_launch_short_backward_##T(const mjlab_decay_grad_t* g, hipStream_t st);   \
   hipError_t mjlab_launch_decay_step_##T(const mjlab_decay_t* d, hipStream_t st);
 MJLAB_POLICY_DECLARE(f32)
 MJLAB_POLICY_DECLARE(f16)
