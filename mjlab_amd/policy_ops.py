@@ -16,6 +16,7 @@ with the eager stream inside the capture): capture from leaves of its own, as fo
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -53,17 +54,44 @@ class DecayGrad(ctypes.Structure):  # mjlab_decay_grad_t
   _fields_ = [("f", Decay), ("d_out", Rows), ("dq", Rows), ("dk", Rows), ("dv", Rows), ("d_state_out", _vp), ("d_state", _vp)]
 
 
-def _stream(dev: torch.device) -> int:
-  return torch.cuda.current_stream(dev).cuda_stream
+# A call's argument struct is packed in one go (setting two dozen ctypes fields one by one takes longer than a small layer's kernel): the layouts of the
+# mirrors above, which native.policy_lib() holds against the library's.
+_LAYER = struct.Struct("@4i3q6P5q3P")
+_LAYER_GRAD = struct.Struct("@4i3q6P5q3P" "Pq5PPq")
+_ROWS = "P3q"
+_DECAY = struct.Struct("@2i2q3if" + 4 * _ROWS + "3PP2q2Pq")
+_DECAY_GRAD = struct.Struct("@2i2q3if" + 4 * _ROWS + "3PP2q2Pq" + 4 * _ROWS + "2P")
+assert _LAYER.size == ctypes.sizeof(Layer) and _LAYER_GRAD.size == ctypes.sizeof(LayerGrad)
+assert _DECAY.size == ctypes.sizeof(Decay) and _DECAY_GRAD.size == ctypes.sizeof(DecayGrad)
+
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
-def _check(t: torch.Tensor, what: str, like: torch.Tensor, shape: tuple) -> torch.Tensor:
+def _call(fn: str, packed: bytes, dev: torch.device) -> None:
+  """Enqueue on torch's current stream of `dev`."""
+  lib = native.policy_lib()
+  index = dev.index
+  stream = _raw_stream(index) if _raw_stream else torch.cuda.current_stream(dev).cuda_stream
+  if torch.cuda.current_device() == index:
+    rc = getattr(lib, fn)(packed, stream)
+  else:
+    with torch.cuda.device(dev):
+      rc = getattr(lib, fn)(packed, stream)
+  if rc:
+    native.policy_check(rc, fn)
+
+
+def _ptr(t: torch.Tensor | None) -> int:
+  return 0 if t is None else t.data_ptr()
+
+
+def _check(t: torch.Tensor, what: str, name: str, like: torch.Tensor, shape: tuple) -> torch.Tensor:
   if t.dtype != like.dtype or t.device != like.device:
-    raise TypeError(f"{what}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
-  if tuple(t.shape) != shape:
-    raise ValueError(f"{what}: expected shape {shape}, got {tuple(t.shape)}")
-  if t.dim() and shape[-1] > 1 and t.stride(-1) != 1:
-    raise ValueError(f"{what}: the last dimension must be contiguous (shape {tuple(t.shape)}, strides {t.stride()})")
+    raise TypeError(f"{what}: {name}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
+  if t.shape != shape:
+    raise ValueError(f"{what}: {name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+  if shape and shape[-1] > 1 and t.stride(-1) != 1:
+    raise ValueError(f"{what}: {name}: the last dimension must be contiguous (shape {tuple(t.shape)}, strides {t.stride()})")
   return t
 
 
@@ -78,17 +106,6 @@ def _ld(t: torch.Tensor) -> int:
   return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _layer_struct(x, w, w_up, b, b_up, act: int) -> Layer:
-  f = Layer()
-  f.dtype, f.act, f.rows, f.inp, f.out = DTYPES[x.dtype], act, x.shape[0], x.shape[1], w.shape[0]
-  f.x, f.ldx, f.w, f.ldw = x.data_ptr(), _ld(x), w.data_ptr(), _ld(w)
-  if w_up is not None:
-    f.w_up, f.ldw_up = w_up.data_ptr(), _ld(w_up)
-  f.b = None if b is None else b.data_ptr()
-  f.b_up = None if b_up is None else b_up.data_ptr()
-  return f
-
-
 # float32 layers whose slope the output gives store nothing else for the backward pass (16 bits: 1 + y and 1 - y^2 would cancel)
 _FROM_OUTPUT = {ACTIVATIONS[a] for a in ("relu", "elu", "tanh", "sigmoid")}
 
@@ -99,20 +116,15 @@ def _from_output(x, w_up, r, act: int) -> bool:
 
 def _forward(x, w, w_up, b, b_up, r, act: int, keep: bool, y=None):
   """-> y, z, z_up (z: the sums before the activation where the backward pass will want them)."""
-  m, n = x.shape[0], w.shape[0]
+  (m, k), n = x.shape, w.shape[0]
   if y is None:
     y = x.new_empty((m, n))
   z = x.new_empty((m, n)) if keep and (act or w_up is not None) and not _from_output(x, w_up, r, act) else None
   z_up = x.new_empty((m, n)) if keep and w_up is not None else None
   if m:
-    f = _layer_struct(x, w, w_up, b, b_up, act)
-    f.y, f.ldy = y.data_ptr(), _ld(y)
-    f.z = None if z is None else z.data_ptr()
-    f.z_up = None if z_up is None else z_up.data_ptr()
-    if r is not None:
-      f.r, f.ldr = r.data_ptr(), _ld(r)
-    with torch.cuda.device(x.device):
-      native.policy_check(native.policy_lib().mjlab_layer_forward(ctypes.byref(f), _stream(x.device)), "mjlab_layer_forward")
+    _call("mjlab_layer_forward",
+          _LAYER.pack(DTYPES[x.dtype], act, 0, 0, m, k, n, x.data_ptr(), w.data_ptr(), _ptr(w_up), _ptr(b), _ptr(b_up), _ptr(r), _ld(x), _ld(w),
+                      0 if w_up is None else _ld(w_up), 0 if r is None else _ld(r), _ld(y), y.data_ptr(), _ptr(z), _ptr(z_up)), x.device)  # fmt: skip
   return y, z, z_up
 
 
@@ -144,21 +156,17 @@ class _Layer(torch.autograd.Function):
         if t is not None:
           t.zero_()
     elif dx is not None or dw is not None or db is not None:
-      g = LayerGrad()
-      g.f = _layer_struct(x, w, w_up, None, None, ctx.act)
-      g.f.z_is_y = ctx.z_is_y
-      g.f.z = None if z is None else z.data_ptr()
-      g.f.z_up = None if z_up is None else z_up.data_ptr()
-      g.dy, g.ld_dy = dy.data_ptr(), _ld(dy)
-      for name, t in (("dx", dx), ("dw", dw), ("dw_up", dwu), ("db", db), ("db_up", dbu)):
-        setattr(g, name, None if t is None else t.data_ptr())
-      lib = native.policy_lib()
-      need = lib.mjlab_layer_backward_workspace(ctypes.byref(g))
-      native.policy_check(min(0, need), "mjlab_layer_backward_workspace")
-      ws = torch.empty((max(need, 1),), dtype=torch.uint8, device=x.device)
-      g.workspace, g.workspace_bytes = ws.data_ptr(), need
-      with torch.cuda.device(x.device):
-        native.policy_check(lib.mjlab_layer_backward(ctypes.byref(g), _stream(x.device)), "mjlab_layer_backward")
+
+      def pack(workspace: int, size: int) -> bytes:
+        return _LAYER_GRAD.pack(DTYPES[x.dtype], ctx.act, ctx.z_is_y, 0, m, k, n, x.data_ptr(), w.data_ptr(), _ptr(w_up), 0, 0, 0, _ld(x), _ld(w),
+                                _ld(w_up) if gated else 0, 0, 0, 0, _ptr(z), _ptr(z_up), dy.data_ptr(), _ld(dy), _ptr(dx), _ptr(dw), _ptr(dwu), _ptr(db), _ptr(dbu),
+                                workspace, size)  # fmt: skip
+
+      need = native.policy_lib().mjlab_layer_backward_workspace(pack(0, 0))
+      if need < 0:
+        native.policy_check(need, "mjlab_layer_backward_workspace")
+      ws = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
+      _call("mjlab_layer_backward", pack(_ptr(ws), need), x.device)
     return dx, dw if need_w else None, dwu if need_wu else None, db if need_b else None, dbu if need_bu else None, dr, None
 
 
@@ -169,7 +177,7 @@ def _arguments(what: str, x: torch.Tensor, w: torch.Tensor, activation: str) -> 
     raise ValueError(f"{what}: unknown activation {activation!r} (one of {', '.join(ACTIVATIONS)})")
   if x.dim() < 1 or w.dim() != 2 or x.shape[-1] < 1 or w.shape[0] < 1:
     raise ValueError(f"{what}: x (..., in) and weight (out, in) with in, out >= 1, got {tuple(x.shape)} and {tuple(w.shape)}")
-  _check(w, f"{what}: weight", x, (w.shape[0], x.shape[-1]))
+  _check(w, what, "weight", x, (w.shape[0], x.shape[-1]))
   return ACTIVATIONS[activation], w.shape[0]
 
 
@@ -196,9 +204,9 @@ def dense(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = Non
   act, n = _arguments("dense", x, weight, activation)
   lead = tuple(x.shape[:-1])
   if bias is not None:
-    _check(bias, "dense: bias", x, (n,))
+    _check(bias, "dense", "bias", x, (n,))
   if residual is not None:
-    _check(residual, "dense: residual", x, (*lead, n))
+    _check(residual, "dense", "residual", x, (*lead, n))
   if out is not None:
     _check_out("dense", out, x, (*lead, n), (weight, bias), residual)
   return _run(x, weight, None, bias, None, residual, act, lead, out)
@@ -209,11 +217,11 @@ def gated(x: torch.Tensor, weight: torch.Tensor, weight_up: torch.Tensor, bias: 
   """``act(x weight^T + bias) * (x weight_up^T + bias_up)``: both products, the activation and the multiplication in one launch; weight and
   weight_up (out, in).  ``out`` as for dense()."""
   act, n = _arguments("gated", x, weight, activation)
-  _check(weight_up, "gated: weight_up", x, tuple(weight.shape))
+  _check(weight_up, "gated", "weight_up", x, weight.shape)
   lead = tuple(x.shape[:-1])
   for b, name in ((bias, "bias"), (bias_up, "bias_up")):
     if b is not None:
-      _check(b, f"gated: {name}", x, (n,))
+      _check(b, "gated", name, x, (n,))
   if out is not None:
     _check_out("gated", out, x, (*lead, n), (weight, weight_up, bias, bias_up))
   return _run(x, weight, weight_up, bias, bias_up, None, act, lead, out)
@@ -234,7 +242,7 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def _check_out(what: str, out: torch.Tensor, like: torch.Tensor, shape: tuple, others: tuple = (), same_as: torch.Tensor | None = None) -> None:
   """`out` is written while `like` and `others` are still read: it may share no memory with them.  `same_as` may be `out` itself."""
-  _check(out, f"{what}: out", like, shape)
+  _check(out, what, "out", like, shape)
   if not out.is_contiguous() or out.requires_grad:
     raise ValueError(f"{what}: out must be contiguous and must not require gradients")
   if same_as is not None and not (same_as.data_ptr() == out.data_ptr() and same_as.stride() == out.stride()):
@@ -251,12 +259,12 @@ def _decay_arguments(what: str, q, k, v, log_decay, state, reset, lead: tuple) -
   if q.dtype not in DTYPES or not q.is_cuda:
     raise TypeError(f"{what}: q must be a float32, float16 or bfloat16 device tensor, got {q.dtype} on {q.device} (there is no CPU fallback)")
   h, dk = q.shape[-2:]
-  _check(k, f"{what}: k", q, (*lead, h, dk))
+  _check(k, what, "k", q, (*lead, h, dk))
   if v.dim() != q.dim():
     raise ValueError(f"{what}: v must have the dimensions of q, got {tuple(v.shape)}")
   dv = v.shape[-1]
-  _check(q, f"{what}: q", q, (*lead, h, dk))
-  _check(v, f"{what}: v", q, (*lead, h, dv))
+  _check(q, what, "q", q, (*lead, h, dk))
+  _check(v, what, "v", q, (*lead, h, dv))
   if h < 1 or not 1 <= dk <= MAX_HEAD_DIM or not 1 <= dv <= MAX_HEAD_DIM:
     raise ValueError(f"{what}: at least one head, and head sizes in [1, {MAX_HEAD_DIM}], got {h} heads of {dk} and {dv}")
   if log_decay.dtype != torch.float32 or log_decay.device != q.device or tuple(log_decay.shape) != (h,) or not log_decay.is_contiguous():
@@ -269,23 +277,16 @@ def _decay_arguments(what: str, q, k, v, log_decay, state, reset, lead: tuple) -
     raise ValueError(f"{what}: reset must be a bool, uint8 or int32 tensor {lead} on {q.device}, got {reset.dtype} {tuple(reset.shape)} on {reset.device}")
 
 
-def _decay_struct(q, k, v, log_decay, scale: float, state, reset, lengths) -> Decay:
-  """q, k, v: (batch, length, heads, d)."""
-  d = Decay()
-  d.dtype, d.scale = DTYPES[q.dtype], scale
-  d.batch, d.length, d.heads, d.dk = q.shape
-  d.dv = v.shape[3]
-  d.q, d.k, d.v = _strided(q), _strided(k), _strided(v)
-  d.log_decay = log_decay.data_ptr()
-  d.state = None if state is None else state.data_ptr()
-  if reset is not None:
-    d.reset, d.reset_bytes, d.reset_batch, d.reset_time = reset.data_ptr(), reset.element_size(), reset.stride(0), reset.stride(1)
-  d.lengths = None if lengths is None else lengths.data_ptr()
-  return d
+def _decay_pack(q, k, v, o, log_decay, scale: float, state, state_out, reset, lengths) -> tuple:
+  """The values of a mjlab_decay_t up to its workspace; q, k, v, o: (batch, length, heads, d), o None: not used."""
+  b, n, h, dk = q.shape
+  r = (0, 0, 0, 0) if reset is None else (reset.element_size(), reset.data_ptr(), reset.stride(0), reset.stride(1))
+  return (DTYPES[q.dtype], r[0], b, n, h, dk, v.shape[3], scale, *_strided(q), *_strided(k), *_strided(v), *_strided(o), log_decay.data_ptr(), _ptr(state),
+          _ptr(state_out), *r[1:], _ptr(lengths))  # fmt: skip
 
 
-def _strided(t: torch.Tensor) -> Rows:
-  return Rows(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+def _strided(t: torch.Tensor | None) -> tuple:
+  return (0, 0, 0, 0) if t is None else (t.data_ptr(), *t.stride()[:3])
 
 
 def _rows_like(t: torch.Tensor, d: int) -> torch.Tensor:
@@ -294,17 +295,12 @@ def _rows_like(t: torch.Tensor, d: int) -> torch.Tensor:
   return t.new_empty((n, b, h, d)).transpose(0, 1) if b > 1 and n > 1 and t.stride(1) > t.stride(0) else t.new_empty((b, n, h, d))
 
 
-def _decay_launch(fn: str, struct: ctypes.Structure, d: Decay, dev: torch.device) -> None:
-  lib = native.policy_lib()
-  need = lib.mjlab_decay_workspace(ctypes.byref(d))
-  native.policy_check(min(0, need), "mjlab_decay_workspace")
+def _decay_launch(fn: str, layout: struct.Struct, head: tuple, tail: tuple, dev: torch.device) -> None:
+  need = native.policy_lib().mjlab_decay_workspace(_DECAY.pack(*head, 0, 0))
+  if need < 0:
+    native.policy_check(need, "mjlab_decay_workspace")
   ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-  if need:
-    d.workspace, d.workspace_bytes = ws.data_ptr(), need
-  if struct is not d:
-    struct.f = d
-  with torch.cuda.device(dev):
-    native.policy_check(getattr(lib, fn)(ctypes.byref(struct), _stream(dev)), fn)
+  _call(fn, layout.pack(*head, _ptr(ws), need, *tail), dev)
 
 
 def _decay_forward(q, k, v, state, log_decay, scale, reset, lengths):
@@ -314,9 +310,7 @@ def _decay_forward(q, k, v, state, log_decay, scale, reset, lengths):
     final = q.new_zeros((b, h, dk, v.shape[3]), dtype=torch.float32) if state is None else state.clone()
     return o, final
   final = torch.empty((b, h, dk, v.shape[3]), dtype=torch.float32, device=q.device)
-  d = _decay_struct(q, k, v, log_decay, scale, state, reset, lengths)
-  d.o, d.state_out = _strided(o), final.data_ptr()
-  _decay_launch("mjlab_decay_forward", d, d, q.device)
+  _decay_launch("mjlab_decay_forward", _DECAY, _decay_pack(q, k, v, o, log_decay, scale, state, final, reset, lengths), (), q.device)
   return o, final
 
 
@@ -346,17 +340,12 @@ class _DecayAttention(torch.autograd.Function):
     elif v.shape[3] > 1 and do.stride(3) != 1:
       do = do.contiguous()
     dfinal = None if dfinal is None else dfinal.contiguous()
-    g = DecayGrad()
     dq = _rows_like(q, dk) if need_q else None
     dk_ = _rows_like(k, dk) if need_k else None
     dv = _rows_like(v, v.shape[3]) if need_v or need_s else None
     ds = torch.empty_like(state) if need_s else None
-    for name, t in (("d_out", do), ("dq", dq), ("dk", dk_), ("dv", dv)):
-      if t is not None:
-        setattr(g, name, _strided(t))
-    g.d_state_out = None if dfinal is None else dfinal.data_ptr()
-    g.d_state = None if ds is None else ds.data_ptr()
-    _decay_launch("mjlab_decay_backward", g, _decay_struct(q, k, v, log_decay, ctx.scale, state, reset, lengths), q.device)
+    _decay_launch("mjlab_decay_backward", _DECAY_GRAD, _decay_pack(q, k, v, None, log_decay, ctx.scale, state, None, reset, lengths),
+                  (*_strided(do), *_strided(dq), *_strided(dk_), *_strided(dv), _ptr(dfinal), _ptr(ds)), q.device)
     return dq, dk_, dv if need_v else None, ds, None, None, None, None
 
 
@@ -407,13 +396,8 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
   else:
     _check_out("decay_attention_step", out, q, (b, h, dv), (k, v, state, out_state))
   if b:
-    d = Decay()
-    d.dtype, d.scale = DTYPES[q.dtype], dk**-0.5 if scale is None else float(scale)
-    d.batch, d.length, d.heads, d.dk, d.dv = b, 1, h, dk, dv
-    d.q, d.k, d.v, d.o = (Rows(t.data_ptr(), t.stride(0), 0, t.stride(1)) for t in (q, k, v, out))
-    d.log_decay, d.state, d.state_out = log_decay.data_ptr(), state.data_ptr(), out_state.data_ptr()
-    if reset is not None:
-      d.reset, d.reset_bytes, d.reset_batch = reset.data_ptr(), reset.element_size(), reset.stride(0)
-    with torch.cuda.device(q.device):
-      native.policy_check(native.policy_lib().mjlab_decay_step(ctypes.byref(d), _stream(q.device)), "mjlab_decay_step")
+    r = (0, 0, 0) if reset is None else (reset.element_size(), reset.data_ptr(), reset.stride(0))
+    rows = [x for t in (q, k, v, out) for x in (t.data_ptr(), t.stride(0), 0, t.stride(1))]
+    _call("mjlab_decay_step", _DECAY.pack(DTYPES[q.dtype], r[0], b, 1, h, dk, dv, dk**-0.5 if scale is None else scale, *rows, log_decay.data_ptr(), state.data_ptr(),
+                                          out_state.data_ptr(), r[1], r[2], 0, 0, 0, 0), q.device)  # fmt: skip
   return out, out_state
