@@ -24,18 +24,19 @@ long long state_bytes(const mjlab_decay_t* d, const Split& s) { return up256(d->
 
 template <int DA, int DC, bool FULL> hipError_t launch_sized(const DecayPass& p, long long rows, hipStream_t st) {
   constexpr int LDS = (int)sizeof(DecayLds<T, DA, DC, false>), LDS_FIRST = (int)sizeof(DecayLds<T, DA, DC, true>);
+  static std::atomic<unsigned long long> asked{0}, asked_first{0};
   hipError_t e;
   if (rows * p.segments > MAX_BLOCKS) return hipErrorInvalidValue;
   if (p.segments > 1) {
     auto first = k_decay_chunks<T, DA, DC, FULL, true>;
-    if ((e = allow_lds(first, LDS_FIRST)) != hipSuccess) return e;
+    if ((e = allow_lds(first, LDS_FIRST, asked_first)) != hipSuccess) return e;
     hipLaunchKernelGGL(first, dim3((unsigned)(rows * (p.segments - 1))), dim3(decay_threads(DA, DC)), LDS_FIRST, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     hipLaunchKernelGGL(k_decay_scan<T>, dim3((unsigned)(rows * ((p.da * p.dc + 255) / 256))), dim3(256), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   auto kern = k_decay_chunks<T, DA, DC, FULL, false>;
-  if ((e = allow_lds(kern, LDS)) != hipSuccess) return e;
+  if ((e = allow_lds(kern, LDS, asked)) != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3((unsigned)(rows * p.segments)), dim3(decay_threads(DA, DC)), LDS, st, p);
   return hipGetLastError();
 }

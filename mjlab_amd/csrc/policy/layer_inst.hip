@@ -9,26 +9,39 @@ template <bool AK, bool BK, int BM, int BN, int EPI> hipError_t launch_tile(cons
   const long long tiles = ((p.M + BM - 1) / BM) * ((p.N + BNO - 1) / BNO);
   if (tiles > MAX_BLOCKS) return hipErrorInvalidValue;
   auto kern = k_product<T, AK, BK, BM, BN, EPI>;
-  if (hipError_t e = allow_lds(kern, LDS); e != hipSuccess) return e;
+  static std::atomic<unsigned long long> asked{0};
+  if (hipError_t e = allow_lds(kern, LDS, asked); e != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3((unsigned)tiles, (unsigned)splits), dim3(256), LDS, st, p);
   return hipGetLastError();
 }
 
-// The tile by how many of them there are for the 256 CUs.  Measured (us; 256 x 128 / 128 x 128 / 64 x 64): bf16 16384 x 2048 x 2816 237 / 253 / 352,
-// 24576 x 1024 x 1024 (3 large tiles per CU) 78 / 76 / 104, 4096 x 1024 x 1024 35 / 22 / 24; float 24576 x 1024 x 1024 - / 278 / 368,
-// 4096 x 1024 x 1024 (1 per CU) - / 72 / 70, 4096 x 512 x 256 - / 36 / 19, 512 x 2048 x 2048 - / 116 / 52.
+// The tile, by an estimate of the time in units of a 256 x 128 tile's share of a CU: `n` tiles of cost `c` for the CU that gets most, of which R run there at
+// once; a round with fewer takes up to 0.4 of a tile longer than its share, since nothing hides what it waits for.  Per element of C a smaller tile costs
+// more: 128 x 128 12 % (24 % where an operand has to be turned), 64 x 64 60 % (124 %); float, whose matrix instructions take longer, 33 % over 128 x 128.
+// Measured (us; 256 x 128 / 128 x 128 / 64 x 64): bf16 y of 16384 x 2048 x 2816 226 / 234 / 351, 24576 x 512 x 1365 71 / 63 / 83,
+// 4096 x 1024 x 1024 30 / 20 / 24; dx of 24576 x 512 x 1365 66 / 77 / 90; float y of 24576 x 1024 x 1024 - / 278 / 368, 512 x 2048 x 2048 - / 116 / 52.
+float tile_cost(long long tiles, float cost, int at_once) {
+  const long long n = (tiles + CUS - 1) / CUS, rest = n % at_once;
+  return cost * (n + (rest ? 0.4f * (at_once - rest) / (at_once - 1) : 0.f));
+}
+
 template <bool AK, bool BK, int EPI> hipError_t launch_product(const Product& p, int splits, hipStream_t st) {
-  const long long nout = EPI == EPI_GATED ? 2 * p.N : p.N, tn = (nout + 127) / 128 * splits;
-  if constexpr (sizeof(T) == 2)
-    if ((p.M + 255) / 256 * tn >= 4 * CUS) return launch_tile<AK, BK, 256, 128, EPI>(p, splits, st);
-  if ((p.M + 127) / 128 * tn * 2 >= 3 * CUS) return launch_tile<AK, BK, 128, 128, EPI>(p, splits, st);
+  const long long nout = EPI == EPI_GATED ? 2 * p.N : p.N;
+  auto tiles = [&](int bm, int bn) { return (p.M + bm - 1) / bm * ((nout + bn - 1) / bn) * splits; };
+  constexpr bool F32 = sizeof(T) == 4;
+  const float small = tile_cost(tiles(64, 64), F32 ? 0.166f : BK ? 0.2f : 0.28f, F32 ? 3 : 5), mid = tile_cost(tiles(128, 128), F32 ? 0.5f : BK ? 0.56f : 0.62f, BK ? 3 : 2);
+  if constexpr (!F32) {
+    const float large = tile_cost(tiles(256, 128), 1.f, 2);
+    if (large < mid && large < small) return launch_tile<AK, BK, 256, 128, EPI>(p, splits, st);
+  }
+  if (mid < small) return launch_tile<AK, BK, 128, 128, EPI>(p, splits, st);
   return launch_tile<AK, BK, 64, 64, EPI>(p, splits, st);
 }
 
 // How many ways the sum over the rows is split in dw = dz^T x: few tiles, many rows.
 int weight_splits(long long out, long long in, long long rows) {
   const long long tiles = ((out + 127) / 128) * ((in + 127) / 128);
-  const long long most = (rows + 255) / 256, want = (2 * CUS + tiles - 1) / tiles;
+  const long long most = (rows + 255) / 256, want = 2 * CUS / tiles;
   const long long s = want < most ? want : most;
   return (int)(s < 1 ? 1 : s);
 }

@@ -1,5 +1,7 @@
 // policy_type.h -- the element type of this translation unit: -DMJLAB_POLICY_DTYPE=<0 f32 | 1 f16 | 2 bf16> (mjlab_amd/native.py).
 #pragma once
+#include <atomic>
+
 #include "policy_common.h"
 #include "policy_launch.h"
 
@@ -17,7 +19,14 @@ using T = __bf16;
 constexpr int CUS = 256;
 constexpr long long MAX_BLOCKS = (1LL << 24) - 1;  // of 256 threads: a launch counts its threads in 32 bits
 
-// Dynamic LDS beyond 64 KB has to be asked for, per device and kernel.
-template <typename K> inline hipError_t allow_lds(K* kern, int bytes) {
-  return bytes > 64 * 1024 ? hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) : hipSuccess;
+// Dynamic LDS beyond 64 KB has to be asked for, once per device and kernel.
+template <typename K> inline hipError_t allow_lds(K* kern, int bytes, std::atomic<unsigned long long>& asked) {
+  if (bytes <= 64 * 1024) return hipSuccess;
+  int dev = 0;
+  if (hipError_t e = hipGetDevice(&dev); e != hipSuccess) return e;
+  const unsigned long long bit = 1ULL << (dev & 63);
+  if (asked.load(std::memory_order_relaxed) & bit) return hipSuccess;
+  const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }

@@ -98,7 +98,7 @@ template <typename T, bool SPLIT, int KB, bool KC, int R> struct Tile {
   static constexpr int PLANE = KC ? R * KB : KT * STRIDE, BYTES = H::PLANES * PLANE;
   static constexpr int UPR = KC ? KT / UE : R / UE;                     // units per row of the tile (KC: m rows; else k rows)
 
-  static __device__ __forceinline__ int swizzle(int row, int c) { return KB == 128 ? c ^ (row & 7) : c ^ ((row >> 1) & 3); }
+  static __device__ __forceinline__ int swizzle(int row, int c) { return KB == 128 ? c ^ ((row >> 1) & 7) : c ^ ((row >> 2) & 3); }
   static __device__ __forceinline__ int row_of(int u) { return u / UPR; }
   static __device__ __forceinline__ int col_of(int u) { return u % UPR * UE; }
 
@@ -223,45 +223,72 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NI; ++j) acc[i][j] = f32x16{};
+  // Fragments of two k-steps: one is multiplied while the next comes from LDS.  (The scheduler would read into the registers of the step before and wait for
+  // every read; the barriers keep it from that.)
+  constexpr int SETS = SPLIT ? 1 : 2;
+  typename Frag<E>::type fa[SETS][MI][H::PLANES], fb[SETS][NI][H::PLANES];
+  auto fetch = [&](const char* sa, int kk) {
+#pragma unroll
+    for (int q = 0; q < H::PLANES; ++q) {
+#pragma unroll
+      for (int i = 0; i < MI; ++i) fa[kk % SETS][i][q] = TA::frag(sa, q, wm + i * 32, kk, lane);
+#pragma unroll
+      for (int j = 0; j < NI; ++j) fb[kk % SETS][j][q] = TB::frag(sa + TA::BYTES, q, wn + j * 32, kk, lane);
+    }
+  };
+  auto multiply = [&](int kk) {
+#pragma unroll
+    for (int qa = 0; qa < H::PLANES; ++qa)
+#pragma unroll
+      for (int qb = 0; qa + qb < H::PLANES; ++qb)
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+          for (int j = 0; j < NI; ++j) acc[i][j] = mma(fa[kk % SETS][i][qa], fb[kk % SETS][j][qb], acc[i][j], E());
+  };
   aim(kbeg);
   load(kbeg);
   stage(lds);
+  if (BUFFERS == 2 && kbeg + KT < kend) load(kbeg + KT);
   __syncthreads();
   int cur = 0;
   for (long long k0 = kbeg; k0 < kend; k0 += KT) {
-    const bool more = k0 + KT < kend;
-    if (more) load(k0 + KT);
-    const char *sa = lds + cur * BUF, *sb = sa + TA::BYTES;
+    const char* sa = lds + cur * BUF;
+    if constexpr (BUFFERS == 2) {
+      // The next k-tile, which came while the last was multiplied, goes to the other buffer before this one is multiplied, so that its way to LDS and the
+      // one after's way here lie behind the matrix instructions; what the first of those read is asked for ahead of it.
+      fetch(sa, 0);
+      cur ^= 1;
+      if (k0 + KT < kend) stage(lds + cur * BUF);
+      if (k0 + 2 * KT < kend) load(k0 + 2 * KT);
+    } else {
+      if (k0 + KT < kend) load(k0 + KT);
+      fetch(sa, 0);
+    }
 #pragma unroll
     for (int kk = 0; kk < H::STEPS; ++kk) {
-      typename Frag<E>::type fa[MI][H::PLANES], fb[NI][H::PLANES];
-#pragma unroll
-      for (int q = 0; q < H::PLANES; ++q) {
-#pragma unroll
-        for (int i = 0; i < MI; ++i) fa[i][q] = TA::frag(sa, q, wm + i * 32, kk, lane);
-#pragma unroll
-        for (int j = 0; j < NI; ++j) fb[j][q] = TB::frag(sb, q, wn + j * 32, kk, lane);
+      if constexpr (SETS == 1) {
+        if (kk) fetch(sa, kk);
+      } else {
+        if (kk + 1 < H::STEPS) fetch(sa, kk + 1);
+        __builtin_amdgcn_sched_barrier(0);
       }
-#pragma unroll
-      for (int qa = 0; qa < H::PLANES; ++qa)
-#pragma unroll
-        for (int qb = 0; qa + qb < H::PLANES; ++qb)
-#pragma unroll
-          for (int i = 0; i < MI; ++i)
-#pragma unroll
-            for (int j = 0; j < NI; ++j) acc[i][j] = mma(fa[i][qa], fb[j][qb], acc[i][j], E());
+      multiply(kk);
     }
-    if (BUFFERS == 1) __syncthreads();
-    if (more) stage(lds + (BUFFERS == 2 ? (cur ^ 1) * BUF : 0));
+    if constexpr (BUFFERS == 1) {
+      __syncthreads();
+      if (k0 + KT < kend) stage(lds);
+    }
     __syncthreads();
-    if (BUFFERS == 2) cur ^= 1;
   }
   return odd != odd;
 }
 
-// Sizes of a launch: the tile, and how T is multiplied in it.
+// Sizes of a launch: the tile, and how T is multiplied in it.  16 bits: 256 x 128 needs 48 KB of LDS with two buffers of 32 k, 128 x 128 32 KB with one of 64
+// (two and three workgroups per CU).  Other depths were no faster (16384 x 2048 x 2816 bf16, us: two buffers of 32 k 226, one of 64 k 239, registers two tiles
+// ahead 235): between the tiles' loads, fragments and matrix instructions none is the bound alone, and the library's own product takes 190 there.
 template <typename T, int BM_, int BN_> struct Shape {
-  static constexpr int BM = BM_, BN = BN_, KB = BM_ == 256 ? 64 : 128, BUFFERS = 2;
+  static constexpr int BM = BM_, BN = BN_, KB = BM_ == 256 ? 64 : 128, BUFFERS = BM_ == 128 ? 1 : 2;
   static constexpr bool SPLIT = false;
 };
 template <int BM_, int BN_> struct Shape<float, BM_, BN_> {

@@ -7,7 +7,8 @@ namespace {
 template <int DK, int DV, bool FULL, bool BACK> hipError_t launch_sized(const ShortArgs& p, hipStream_t st) {
   constexpr int LDS = (int)sizeof(ShortLds<DK, DV, BACK>);
   auto kern = k_decay_short<T, DK, DV, FULL, BACK>;
-  if (hipError_t e = allow_lds(kern, LDS); e != hipSuccess) return e;
+  static std::atomic<unsigned long long> asked{0};
+  if (hipError_t e = allow_lds(kern, LDS, asked); e != hipSuccess) return e;
   const long long rows = p.d.batch * p.d.heads;  // (below 2^24, and up to 512 threads each: below 2^32 in all is for the caller to check)
   if (rows * short_threads(DK, DV) > 0xffffffffLL) return hipErrorInvalidValue;
   hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(short_threads(DK, DV)), LDS, st, p);
