@@ -37,7 +37,10 @@ typedef struct mjlab_layer {
   const void *x, *w, *w_up, *b, *b_up, *r;
   long long ldx, ldw, ldw_up, ldr, ldy;
   void *y, *z, *z_up;
+  void* workspace; /* mjlab_layer_forward_workspace() bytes of device memory: 0 but for few rows, whose sums over `in` are split over the device */
+  long long workspace_bytes;
 } mjlab_layer_t;
+long long mjlab_layer_forward_workspace(const mjlab_layer_t* f); /* -1: bad arguments */
 int mjlab_layer_forward(const mjlab_layer_t* f, void* stream);
 int mjlab_sizeof_layer(void);
 

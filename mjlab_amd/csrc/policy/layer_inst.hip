@@ -25,18 +25,41 @@ float tile_cost(long long tiles, float cost, int at_once) {
   return cost * (n + (rest ? 0.4f * (at_once - rest) / (at_once - 1) : 0.f));
 }
 
-template <bool AK, bool BK, int EPI> hipError_t launch_product(const Product& p, int splits, hipStream_t st) {
-  const long long nout = EPI == EPI_GATED ? 2 * p.N : p.N;
-  auto tiles = [&](int bm, int bn) { return (p.M + bm - 1) / bm * ((nout + bn - 1) / bn) * splits; };
+struct Cost {
+  float small, mid, large, best;
+};
+template <bool BK> Cost costs(long long M, long long width, long long splits) {
+  auto tiles = [&](int bm, int bn) { return (M + bm - 1) / bm * ((width + bn - 1) / bn) * splits; };
   constexpr bool F32 = sizeof(T) == 4;
-  const float small = tile_cost(tiles(64, 64), F32 ? 0.166f : BK ? 0.2f : 0.28f, F32 ? 3 : 5), mid = tile_cost(tiles(128, 128), F32 ? 0.5f : BK ? 0.56f : 0.62f, BK ? 3 : 2);
-  if constexpr (!F32) {
-    const float large = tile_cost(tiles(256, 128), 1.f, 2);
-    if (large < mid && large < small) return launch_tile<AK, BK, 256, 128, EPI>(p, splits, st);
-  }
-  if (mid < small) return launch_tile<AK, BK, 128, 128, EPI>(p, splits, st);
-  return launch_tile<AK, BK, 64, 64, EPI>(p, splits, st);
+  Cost c;
+  c.small = tile_cost(tiles(64, 64), F32 ? 0.166f : BK ? 0.2f : 0.28f, F32 ? 3 : 5);
+  c.mid = tile_cost(tiles(128, 128), F32 ? 0.5f : BK ? 0.56f : 0.62f, BK ? 3 : 2);
+  c.large = F32 ? 1e30f : tile_cost(tiles(256, 128), 1.f, 2);
+  c.best = c.large < c.mid && c.large < c.small ? c.large : c.mid < c.small ? c.mid : c.small;
+  return c;
 }
+
+template <bool AK, bool BK, int EPI> hipError_t launch_product(const Product& p, int splits, hipStream_t st) {
+  const Cost c = costs<BK>(p.M, EPI == EPI_GATED ? 2 * p.N : p.N, splits);
+  if constexpr (sizeof(T) == 2)
+    if (c.best == c.large) return launch_tile<AK, BK, 256, 128, EPI>(p, splits, st);
+  return c.best == c.mid ? launch_tile<AK, BK, 128, 128, EPI>(p, splits, st) : launch_tile<AK, BK, 64, 64, EPI>(p, splits, st);
+}
+
+// Few rows leave most CUs idle: the sum over k is then split, each part's sums go through memory, and a second launch joins them.  The time of an unsplit unit of
+// tile_cost() is about 21 ns per k (float 80 ns), the second launch 4 us and what it reads at 3 TB/s.
+// (64 rows, 2048 x 2048: float 49 us unsplit, 12 + 4 us split; bf16 17 us, 6 + 3 us.)
+template <bool BK> int sum_splits(long long M, long long width, long long K) {
+  const float per_k = sizeof(T) == 4 ? 0.08f : 0.021f;
+  int best = 1;
+  float time = costs<BK>(M, width, 1).best * K * per_k;
+  for (int s = 2; s <= 32 && K / s >= 128; s *= 2) {
+    const float t = costs<BK>(M, width, s).best * K / s * per_k + 4.f + 4e-6f * M * width * s * 0.67f;
+    if (t < time) { time = t; best = s; }
+  }
+  return best;
+}
+long long per_split(long long K, int splits) { return ((K + splits - 1) / splits + 63) / 64 * 64; }
 
 // How many ways the sum over the rows is split in dw = dz^T x: few tiles, many rows.
 int weight_splits(long long out, long long in, long long rows) {
@@ -51,7 +74,7 @@ long long up256(long long x) { return (x + 255) & ~255LL; }
 struct Plan {
   bool gated, slope, sums, weights;
   long long ns, blocks, o_dz, o_sums, o_partial, bytes;
-  int splits;
+  int splits, x_splits;
 };
 
 Plan plan(const mjlab_layer_grad_t* g) {
@@ -69,20 +92,41 @@ Plan plan(const mjlab_layer_grad_t* g) {
   if (q.slope) at += up256(f.rows * q.ns * f.out * (long long)sizeof(T));
   q.o_sums = at;
   if (q.sums) at += up256(q.blocks * q.ns * f.out * 4);
-  q.o_partial = at;
-  if (q.weights && (q.splits > 1 || q.gated)) at += up256((long long)q.splits * q.ns * f.out * f.in * 4);
+  q.x_splits = g->dx ? sum_splits<false>(f.rows, f.in, q.ns * f.out) : 1;
+  q.o_partial = at;  // (dx's sums are joined before dw's are formed)
+  const long long w = q.weights && (q.splits > 1 || q.gated) ? q.splits * q.ns * f.out * f.in : 0, x = q.x_splits > 1 ? q.x_splits * f.rows * f.in : 0;
+  at += up256((w > x ? w : x) * 4);
   q.bytes = at;
   return q;
 }
+
+int forward_splits(const mjlab_layer_t* f) { return sum_splits<true>(f->rows, f->w_up ? 2 * f->out : f->out, f->in); }
 
 }  // namespace
 
 hipError_t POLICY_NAME(mjlab_launch_layer_forward)(const mjlab_layer_t* f, hipStream_t st) {
   Product p = {};
   p.A = f->x; p.lda = f->ldx; p.B = f->w; p.ldb = f->ldw; p.B2 = f->w_up; p.ldb2 = f->ldw_up;
-  p.M = f->rows; p.N = f->out; p.K = p.kb2 = p.ksplit = f->in;
+  p.M = f->rows; p.N = p.nb2 = f->out; p.K = p.kb2 = p.ksplit = f->in;
   p.act = f->act; p.b = f->b; p.b_up = f->b_up; p.r = f->r; p.ldr = f->ldr; p.y = f->y; p.ldy = f->ldy; p.z = f->z; p.z_up = f->z_up;
-  return f->w_up ? launch_product<true, true, EPI_GATED>(p, 1, st) : launch_product<true, true, EPI_LAYER>(p, 1, st);
+  const int s = forward_splits(f);
+  if (s == 1) return f->w_up ? launch_product<true, true, EPI_GATED>(p, 1, st) : launch_product<true, true, EPI_LAYER>(p, 1, st);
+  Product q = p;
+  q.N = f->w_up ? 2 * f->out : f->out;
+  q.ksplit = per_split(f->in, s);
+  q.partial = p.partial = (float*)f->workspace;
+  const int splits = (int)((f->in + q.ksplit - 1) / q.ksplit);
+  if (hipError_t e = launch_product<true, true, EPI_PARTIAL>(q, splits, st); e != hipSuccess) return e;
+  const long long blocks = (f->rows * f->out + 255) / 256;
+  if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
+  auto join = f->w_up ? k_join_layer<T, true> : k_join_layer<T, false>;
+  hipLaunchKernelGGL(join, dim3((unsigned)blocks), dim3(256), 0, st, p, splits);
+  return hipGetLastError();
+}
+
+long long POLICY_NAME(mjlab_layer_forward_bytes)(const mjlab_layer_t* f) {
+  const int s = forward_splits(f);
+  return s == 1 ? 0 : up256(s * f->rows * (f->w_up ? 2 : 1) * f->out * 4);
 }
 
 long long POLICY_NAME(mjlab_layer_backward_bytes)(const mjlab_layer_grad_t* g) { return plan(g).bytes; }
@@ -112,15 +156,25 @@ hipError_t POLICY_NAME(mjlab_launch_layer_backward)(const mjlab_layer_grad_t* g,
   if (g->dx) {
     Product p = {};
     p.A = d; p.lda = ldd; p.B = f.w; p.ldb = f.ldw; p.B2 = f.w_up; p.ldb2 = f.ldw_up;
-    p.M = f.rows; p.N = f.in; p.K = p.ksplit = q.ns * f.out; p.kb2 = f.out;
-    p.y = g->dx; p.ldy = f.in;
-    if ((e = launch_product<true, false, EPI_STORE>(p, 1, st)) != hipSuccess) return e;
+    p.M = f.rows; p.N = p.nb2 = f.in; p.K = p.ksplit = q.ns * f.out; p.kb2 = f.out;
+    p.y = g->dx; p.ldy = f.in; p.partial = partial;
+    if (q.x_splits == 1) {
+      if ((e = launch_product<true, false, EPI_STORE>(p, 1, st)) != hipSuccess) return e;
+    } else {
+      p.ksplit = per_split(p.K, q.x_splits);
+      const int splits = (int)((p.K + p.ksplit - 1) / p.ksplit);
+      const long long n = f.rows * f.in;
+      if ((n + 255) / 256 > MAX_BLOCKS) return hipErrorInvalidValue;
+      if ((e = launch_product<true, false, EPI_PARTIAL>(p, splits, st)) != hipSuccess) return e;
+      hipLaunchKernelGGL(k_join_splits<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, partial, (T*)g->dx, n, n, splits);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
   }
   if (g->dw) {
     Product p = {};
     p.A = d; p.lda = ldd; p.B = f.x; p.ldb = f.ldx;
-    p.M = q.ns * f.out; p.N = f.in; p.K = p.kb2 = f.rows;
-    p.ksplit = ((f.rows + q.splits - 1) / q.splits + 63) / 64 * 64;
+    p.M = q.ns * f.out; p.N = p.nb2 = f.in; p.K = p.kb2 = f.rows;
+    p.ksplit = per_split(f.rows, q.splits);
     const int splits = (int)((f.rows + p.ksplit - 1) / p.ksplit);
     p.y = g->dw; p.ldy = f.in; p.partial = partial;
     if (splits == 1 && !q.gated) return launch_product<false, false, EPI_STORE>(p, 1, st);

@@ -34,6 +34,12 @@ const char* mjlab_policy_last_error(void) { return g_error; }
 int mjlab_sizeof_layer(void) { return (int)sizeof(mjlab_layer_t); }
 int mjlab_sizeof_layer_grad(void) { return (int)sizeof(mjlab_layer_grad_t); }
 
+long long mjlab_layer_forward_workspace(const mjlab_layer_t* f) {
+  if (!f) return fail(-1, "layer_forward_workspace: null argument");
+  if (check_layer(*f)) return -1;
+  return BY_TYPE(f->dtype, mjlab_layer_forward_bytes, f);
+}
+
 int mjlab_layer_forward(const mjlab_layer_t* f, void* stream) {
   if (!f) return fail(-1, "layer_forward: null argument");
   int rc = check_layer(*f);
@@ -43,6 +49,8 @@ int mjlab_layer_forward(const mjlab_layer_t* f, void* stream) {
   if (f->r && f->w_up) return fail(-2, "layer_forward: a gated layer takes no residual");
   if (f->b_up && !f->w_up) return fail(-2, "layer_forward: b_up without w_up");
   if (f->z_up && !f->w_up) return fail(-2, "layer_forward: z_up without w_up");
+  const long long need = BY_TYPE(f->dtype, mjlab_layer_forward_bytes, f);
+  if (need > 0 && (!f->workspace || f->workspace_bytes < need)) return fail(-3, "layer_forward: workspace too small");
   return done(BY_TYPE(f->dtype, mjlab_launch_layer_forward, f, (hipStream_t)stream), "layer_forward launch failed");
 }
 

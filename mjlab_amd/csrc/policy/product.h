@@ -23,6 +23,7 @@ struct Product {
   const void *A, *B, *B2;      // B2: w_up (EPI_GATED: rows of both in turn; EPI_STORE: the rows k >= kb2 of B)
   long long lda, ldb, ldb2;
   long long M, N, K, kb2;      // kb2: where B's rows end and B2's begin (K where there is no B2)
+  long long nb2;               // the same for a k-contiguous B outside EPI_GATED (N where there is no B2)
   long long ksplit;            // k elements per blockIdx.y
   int act;
   const void *b, *b_up, *r;    // the epilogue's
@@ -169,6 +170,7 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
     if constexpr (BK) {
       long long n = GATED ? n0 + r / (2 * HALF) * HALF + r % HALF : n0 + r;
       n = n < p.N ? n : p.N - 1;
+      if (!GATED && n >= p.nb2) return B2 + (n - p.nb2) * p.ldb2 + k0 + c;
       return (GATED && (r / HALF & 1) ? B2 + n * p.ldb2 : B + n * p.ldb) + k0 + c;
     } else {
       const long long k = k0 + r;
@@ -423,6 +425,28 @@ template <typename T> __global__ __launch_bounds__(256) void k_join_splits(const
 #pragma unroll 8
   for (int k = 0; k < splits; ++k) s += partial[k * stride + i];
   out[i] = (T)s;
+}
+
+// What EPI_LAYER and EPI_GATED do, on sums that were split: partial (splits, rows, out | 2 out), one output per thread
+template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_join_layer(const Product p, int splits) {
+  const long long i = blockIdx.x * 256LL + threadIdx.x, n = p.M * p.N;
+  if (i >= n) return;
+  const long long m = i / p.N, c = i % p.N, width = GATED ? 2 * p.N : p.N;
+  float v = 0.f, u = 0.f;
+#pragma unroll 8
+  for (int k = 0; k < splits; ++k) {
+    v += p.partial[(k * p.M + m) * width + c];
+    if constexpr (GATED) u += p.partial[(k * p.M + m) * width + p.N + c];
+  }
+  if (p.b) v += (float)((const T*)p.b)[c];
+  if (p.z) ((T*)p.z)[i] = (T)v;
+  with_act(p.act, [&](auto act) { v = act_value<decltype(act)::value>(v); });
+  if constexpr (GATED) {
+    if (p.b_up) u += (float)((const T*)p.b_up)[c];
+    if (p.z_up) ((T*)p.z_up)[i] = (T)u;
+    v *= u;
+  } else if (p.r) v += (float)((const T*)p.r)[m * p.ldr + c];
+  ((T*)p.y)[m * p.ldy + c] = (T)v;
 }
 
 // dz (rows, out | 2 out) from dy and the stored sums, and this row block's column sums for the bias gradient.

@@ -31,7 +31,8 @@ ACTIVATIONS = {"none": 0, "relu": 1, "elu": 2, "tanh": 3, "sigmoid": 4, "silu": 
 class Layer(ctypes.Structure):  # mjlab_layer_t
   _fields_ = [("dtype", ctypes.c_int), ("act", ctypes.c_int), ("z_is_y", ctypes.c_int), ("pad_", ctypes.c_int), ("rows", _ll), ("inp", _ll), ("out", _ll),
               ("x", _vp), ("w", _vp), ("w_up", _vp), ("b", _vp), ("b_up", _vp), ("r", _vp),
-              ("ldx", _ll), ("ldw", _ll), ("ldw_up", _ll), ("ldr", _ll), ("ldy", _ll), ("y", _vp), ("z", _vp), ("z_up", _vp)]  # fmt: skip
+              ("ldx", _ll), ("ldw", _ll), ("ldw_up", _ll), ("ldr", _ll), ("ldy", _ll), ("y", _vp), ("z", _vp), ("z_up", _vp),
+              ("workspace", _vp), ("workspace_bytes", _ll)]  # fmt: skip
 
 
 class LayerGrad(ctypes.Structure):  # mjlab_layer_grad_t
@@ -56,8 +57,8 @@ class DecayGrad(ctypes.Structure):  # mjlab_decay_grad_t
 
 # A call's argument struct is packed in one go (setting two dozen ctypes fields one by one takes longer than a small layer's kernel): the layouts of the
 # mirrors above, which native.policy_lib() holds against the library's.
-_LAYER = struct.Struct("@4i3q6P5q3P")
-_LAYER_GRAD = struct.Struct("@4i3q6P5q3P" "Pq5PPq")
+_LAYER = struct.Struct("@4i3q6P5q3PPq")
+_LAYER_GRAD = struct.Struct("@4i3q6P5q3PPq" "Pq5PPq")
 _ROWS = "P3q"
 _DECAY = struct.Struct("@2i2q3if" + 4 * _ROWS + "3PP2q2Pq")
 _DECAY_GRAD = struct.Struct("@2i2q3if" + 4 * _ROWS + "3PP2q2Pq" + 4 * _ROWS + "2P")
@@ -122,9 +123,13 @@ def _forward(x, w, w_up, b, b_up, r, act: int, keep: bool, y=None):
   z = x.new_empty((m, n)) if keep and (act or w_up is not None) and not _from_output(x, w_up, r, act) else None
   z_up = x.new_empty((m, n)) if keep and w_up is not None else None
   if m:
-    _call("mjlab_layer_forward",
-          _LAYER.pack(DTYPES[x.dtype], act, 0, 0, m, k, n, x.data_ptr(), w.data_ptr(), _ptr(w_up), _ptr(b), _ptr(b_up), _ptr(r), _ld(x), _ld(w),
-                      0 if w_up is None else _ld(w_up), 0 if r is None else _ld(r), _ld(y), y.data_ptr(), _ptr(z), _ptr(z_up)), x.device)  # fmt: skip
+    args = (DTYPES[x.dtype], act, 0, 0, m, k, n, x.data_ptr(), w.data_ptr(), _ptr(w_up), _ptr(b), _ptr(b_up), _ptr(r), _ld(x), _ld(w),
+            0 if w_up is None else _ld(w_up), 0 if r is None else _ld(r), _ld(y), y.data_ptr(), _ptr(z), _ptr(z_up))  # fmt: skip
+    need = native.policy_lib().mjlab_layer_forward_workspace(_LAYER.pack(*args, 0, 0))
+    if need < 0:
+      native.policy_check(need, "mjlab_layer_forward_workspace")
+    ws = torch.empty((need,), dtype=torch.uint8, device=x.device) if need else None
+    _call("mjlab_layer_forward", _LAYER.pack(*args, _ptr(ws), need), x.device)
   return y, z, z_up
 
 
@@ -159,7 +164,7 @@ class _Layer(torch.autograd.Function):
 
       def pack(workspace: int, size: int) -> bytes:
         return _LAYER_GRAD.pack(DTYPES[x.dtype], ctx.act, ctx.z_is_y, 0, m, k, n, x.data_ptr(), w.data_ptr(), _ptr(w_up), 0, 0, 0, _ld(x), _ld(w),
-                                _ld(w_up) if gated else 0, 0, 0, 0, _ptr(z), _ptr(z_up), dy.data_ptr(), _ld(dy), _ptr(dx), _ptr(dw), _ptr(dwu), _ptr(db), _ptr(dbu),
+                                _ld(w_up) if gated else 0, 0, 0, 0, _ptr(z), _ptr(z_up), 0, 0, dy.data_ptr(), _ld(dy), _ptr(dx), _ptr(dw), _ptr(dwu), _ptr(db), _ptr(dbu),
                                 workspace, size)  # fmt: skip
 
       need = native.policy_lib().mjlab_layer_backward_workspace(pack(0, 0))

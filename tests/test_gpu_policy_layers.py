@@ -128,6 +128,14 @@ def test_many_rows_split_the_weight_gradient(dtype):
 
 
 @pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("m,k,n", [(1, 2048, 1024), (5, 1999, 333), (64, 1031, 517), (70, 300, 2049)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_few_rows_split_the_sums(m, k, n, dtype, gated):
+  check_layer(m, k, n, dtype, "silu", gated, bias=True, residual=not gated, seed=8)
+  check_layer(m, k, n, dtype, "elu", gated, bias=False, residual=False, seed=9)
+
+
+@pytest.mark.parametrize("dtype", list(U))
 def test_row_strides_and_odd_addresses(dtype):
   gen = torch.Generator(device="cuda").manual_seed(3)
   wide = rand(gen, 70, 61, dtype=dtype)

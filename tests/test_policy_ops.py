@@ -41,6 +41,7 @@ def _layer(**kw):
   (dict(dtype=3), "dtype"), (dict(act=7), "activation"), (dict(act=-1), "activation"), (dict(rows=0), "sizes"), (dict(inp=0), "sizes"), (dict(out=-1), "sizes"),
   (dict(inp=1 << 30), "sizes"), (dict(x=None), "null x or w"), (dict(w=None), "null x or w"), (dict(y=None), "null y"), (dict(ldx=-8), "negative"),
   (dict(ldy=2), "overlap"), (dict(w_up=64, ldw_up=8, r=64), "residual"), (dict(b_up=64), "b_up"), (dict(z_up=64), "z_up"),
+  (dict(rows=4, inp=2048, out=2048, ldy=2048), "workspace"),
 ])  # fmt: skip
 def test_layer_forward_refuses(kw, text):
   lib = native.policy_lib()
@@ -65,6 +66,15 @@ def test_layer_backward_refuses(kw, text):
     setattr(g, k, v)
   assert lib.mjlab_layer_backward(ctypes.byref(g), None) < 0
   assert text in lib.mjlab_policy_last_error().decode()
+
+
+def test_few_rows_of_a_wide_layer_split_their_sums():
+  lib = native.policy_lib()
+  for dtype in (0, 1, 2):
+    assert lib.mjlab_layer_forward_workspace(ctypes.byref(_layer(dtype=dtype, rows=4096, inp=512, out=512))) == 0
+    assert lib.mjlab_layer_forward_workspace(ctypes.byref(_layer(dtype=dtype, rows=16, inp=99, out=29))) == 0
+    assert lib.mjlab_layer_forward_workspace(ctypes.byref(_layer(dtype=dtype, rows=16, inp=2048, out=2048))) >= 2 * 16 * 2048 * 4
+  assert lib.mjlab_layer_forward_workspace(ctypes.byref(_layer(rows=0))) == -1
 
 
 def test_workspace_covers_what_the_backward_pass_stores():
