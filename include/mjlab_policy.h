@@ -29,10 +29,11 @@ const char* mjlab_policy_last_error(void);
  *   gated (w_up != NULL):  y = act(x w^T + b) * (x w_up^T + b_up)
  * x (rows, in), w and w_up (out, in), b and b_up (out) or NULL, r (rows, out) or NULL (dense only), y (rows, out); the innermost stride of
  * each is 1, ld* is the distance of rows.  All arrays hold `dtype`; sums are held in 32 bits and each output is rounded once.
- * z / z_up (rows, out), dense, or NULL: the sums before the activation, which the backward pass reads.  z_is_y (backward pass only): z points to the
- * dense output y instead, which determines the slope of relu, elu, tanh and sigmoid where no residual was added. */
+ * z / z_up (rows, out), dense, or NULL: the sums before the activation, which the backward pass reads: of `dtype` for a dense layer, floats (z and z_up
+ * alike) for a gated one, whose gradients multiply them.  z_bytes, their element size, has to say so.  z_is_y (backward pass only): z points to the dense
+ * output y instead, which determines the slope of relu, elu, tanh and sigmoid where no residual was added. */
 typedef struct mjlab_layer {
-  int dtype, act, z_is_y, pad_;
+  int dtype, act, z_is_y, z_bytes;
   long long rows, in, out;
   const void *x, *w, *w_up, *b, *b_up, *r;
   long long ldx, ldw, ldw_up, ldr, ldy;
@@ -44,7 +45,10 @@ long long mjlab_layer_forward_workspace(const mjlab_layer_t* f); /* -1: bad argu
 int mjlab_layer_forward(const mjlab_layer_t* f, void* stream);
 int mjlab_sizeof_layer(void);
 
-/* The backward pass of the layer `f` (x, w, w_up, z, z_up and the sizes are read; b, r, y are not) for the upstream gradient dy:
+/* 1: the backward pass of this (gated, 16-bit) layer forms the sums again when z and z_up are NULL, which is faster than storing them; 0: it needs them. */
+int mjlab_layer_recomputes(const mjlab_layer_t* f);
+
+/* The backward pass of the layer `f` (x, w, w_up, z, z_up and the sizes are read, b and b_up where the sums are formed again; r, y are not) for the upstream gradient dy:
  *   dense: dz = dy act'(z);                          dx = dz w;            dw = dz^T x;  db = sum over rows of dz
  *   gated: dg = dy z_up act'(z), du = dy act(z);     dx = dg w + du w_up;  dw = dg^T x, dw_up = du^T x;  db, db_up likewise
  * (the residual's gradient is dy itself).  A dense layer without activation needs no z.  Each output is dense and may be NULL (not wanted);

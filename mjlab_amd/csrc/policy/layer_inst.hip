@@ -5,7 +5,7 @@
 namespace {
 
 template <bool AK, bool BK, int BM, int BN, int EPI> hipError_t launch_tile(const Product& p, int splits, hipStream_t st) {
-  constexpr int BNO = EPI == EPI_GATED ? BN / 2 : BN, LDS = ProductLds<T, AK, BK, BM, BN, EPI>::BYTES;
+  constexpr int BNO = EPI == EPI_GATED || EPI == EPI_SLOPE ? BN / 2 : BN, LDS = ProductLds<T, AK, BK, BM, BN, EPI>::BYTES;
   const long long tiles = ((p.M + BM - 1) / BM) * ((p.N + BNO - 1) / BNO);
   if (tiles > MAX_BLOCKS) return hipErrorInvalidValue;
   auto kern = k_product<T, AK, BK, BM, BN, EPI>;
@@ -40,7 +40,7 @@ template <bool BK> Cost costs(long long M, long long width, long long splits) {
 }
 
 template <bool AK, bool BK, int EPI> hipError_t launch_product(const Product& p, int splits, hipStream_t st) {
-  const Cost c = costs<BK>(p.M, EPI == EPI_GATED ? 2 * p.N : p.N, splits);
+  const Cost c = costs<BK>(p.M, EPI == EPI_GATED || EPI == EPI_SLOPE ? 2 * p.N : p.N, splits);
   if constexpr (sizeof(T) == 2)
     if (c.best == c.large) return launch_tile<AK, BK, 256, 128, EPI>(p, splits, st);
   return c.best == c.mid ? launch_tile<AK, BK, 128, 128, EPI>(p, splits, st) : launch_tile<AK, BK, 64, 64, EPI>(p, splits, st);
@@ -72,7 +72,7 @@ int weight_splits(long long out, long long in, long long rows) {
 long long up256(long long x) { return (x + 255) & ~255LL; }
 
 struct Plan {
-  bool gated, slope, sums, weights;
+  bool gated, slope, sums, weights, again;
   long long ns, blocks, o_dz, o_sums, o_partial, bytes;
   int splits, x_splits;
 };
@@ -85,7 +85,13 @@ Plan plan(const mjlab_layer_grad_t* g) {
   q.slope = q.gated || f.act != MJLAB_ACT_NONE;
   q.sums = g->db != nullptr;
   q.weights = g->dw != nullptr;
+  q.again = q.gated && !f.z;
   q.blocks = (f.rows + SLOPE_ROWS - 1) / SLOPE_ROWS;
+  if (q.again) {  // two sets of column sums per tile of rows
+    const Cost c = costs<true>(f.rows, 2 * f.out, 1);
+    const int bm = c.best == c.large ? 256 : c.best == c.mid ? 128 : 64;
+    q.blocks = 2 * ((f.rows + bm - 1) / bm);
+  }
   q.splits = weight_splits(q.ns * f.out, f.in, f.rows);
   long long at = 0;
   q.o_dz = at;
@@ -102,13 +108,21 @@ Plan plan(const mjlab_layer_grad_t* g) {
 
 int forward_splits(const mjlab_layer_t* f) { return sum_splits<true>(f->rows, f->w_up ? 2 * f->out : f->out, f->in); }
 
-}  // namespace
-
-hipError_t POLICY_NAME(mjlab_launch_layer_forward)(const mjlab_layer_t* f, hipStream_t st) {
+Product forward_product(const mjlab_layer_t* f) {
   Product p = {};
   p.A = f->x; p.lda = f->ldx; p.B = f->w; p.ldb = f->ldw; p.B2 = f->w_up; p.ldb2 = f->ldw_up;
   p.M = f->rows; p.N = p.nb2 = f->out; p.K = p.kb2 = p.ksplit = f->in;
   p.act = f->act; p.b = f->b; p.b_up = f->b_up; p.r = f->r; p.ldr = f->ldr; p.y = f->y; p.ldy = f->ldy; p.z = f->z; p.z_up = f->z_up;
+  return p;
+}
+
+}  // namespace
+
+// 16-bit gated layers up to this many inputs form their sums again in the backward pass, inside the launch that turns dy into [dg | du].
+int POLICY_NAME(mjlab_layer_again)(const mjlab_layer_t* f) { return sizeof(T) == 2 && f->w_up && f->in <= 1024; }
+
+hipError_t POLICY_NAME(mjlab_launch_layer_forward)(const mjlab_layer_t* f, hipStream_t st) {
+  Product p = forward_product(f);
   const int s = forward_splits(f);
   if (s == 1) return f->w_up ? launch_product<true, true, EPI_GATED>(p, 1, st) : launch_product<true, true, EPI_LAYER>(p, 1, st);
   Product q = p;
@@ -138,18 +152,24 @@ hipError_t POLICY_NAME(mjlab_launch_layer_backward)(const mjlab_layer_grad_t* g,
   T* dz = (T*)(ws + q.o_dz);
   float *sums = q.sums ? (float*)(ws + q.o_sums) : nullptr, *partial = (float*)(ws + q.o_partial);
   hipError_t e = hipSuccess;
-  if (q.slope || q.sums) {
+  if (q.again) {
+    if constexpr (sizeof(T) == 2) {
+      Product p = forward_product(&f);
+      p.r = g->dy; p.ldr = g->ld_dy; p.y = dz; p.ldy = 2 * f.out; p.z = p.z_up = nullptr; p.partial = sums;
+      if ((e = launch_product<true, true, EPI_SLOPE>(p, 1, st)) != hipSuccess) return e;
+    } else return hipErrorInvalidValue;
+  } else if (q.slope || q.sums) {
     constexpr int V = Elem<T>::VEC;
     const long long colblocks = (f.out + 32 * V - 1) / (32 * V);
     if (colblocks * q.blocks > MAX_BLOCKS) return hipErrorInvalidValue;
     auto kern = q.gated ? k_layer_slope<T, true, false> : f.z_is_y ? k_layer_slope<T, false, true> : k_layer_slope<T, false, false>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(colblocks * q.blocks)), dim3(256), 0, st, (const T*)g->dy, g->ld_dy, (const T*)f.z, (const T*)f.z_up, q.slope ? dz : nullptr, sums, f.rows, f.out, (unsigned)colblocks, f.act);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(colblocks * q.blocks)), dim3(256), 0, st, (const T*)g->dy, g->ld_dy, f.z, (const float*)f.z_up, q.slope ? dz : nullptr, sums, f.rows, f.out, (unsigned)colblocks, f.act);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    if (q.sums) {
-      const long long cols = q.ns * f.out;
-      hipLaunchKernelGGL(k_join_sums<T>, dim3((unsigned)((cols + 15) / 16)), dim3(256), 0, st, sums, (T*)g->db, (T*)g->db_up, f.out, cols, q.blocks);
-      if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
+  }
+  if (q.sums) {
+    const long long cols = q.ns * f.out;
+    hipLaunchKernelGGL(k_join_sums<T>, dim3((unsigned)((cols + 15) / 16)), dim3(256), 0, st, sums, (T*)g->db, (T*)g->db_up, f.out, cols, q.blocks);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   const void* d = q.slope ? (const void*)dz : g->dy;
   const long long ldd = q.slope ? q.ns * f.out : g->ld_dy;

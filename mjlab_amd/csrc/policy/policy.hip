@@ -34,6 +34,16 @@ const char* mjlab_policy_last_error(void) { return g_error; }
 int mjlab_sizeof_layer(void) { return (int)sizeof(mjlab_layer_t); }
 int mjlab_sizeof_layer_grad(void) { return (int)sizeof(mjlab_layer_grad_t); }
 
+static int check_z(const mjlab_layer_t& f) {
+  if ((f.z || f.z_up) && f.z_bytes != (f.w_up || f.dtype == MJLAB_DTYPE_F32 ? 4 : 2)) return fail(-2, "layer: z_bytes: a gated layer's sums are floats, a dense layer's of its dtype");
+  return 0;
+}
+
+int mjlab_layer_recomputes(const mjlab_layer_t* f) {
+  if (!f || check_layer(*f)) return 0;
+  return BY_TYPE(f->dtype, mjlab_layer_again, f);
+}
+
 long long mjlab_layer_forward_workspace(const mjlab_layer_t* f) {
   if (!f) return fail(-1, "layer_forward_workspace: null argument");
   if (check_layer(*f)) return -1;
@@ -49,6 +59,7 @@ int mjlab_layer_forward(const mjlab_layer_t* f, void* stream) {
   if (f->r && f->w_up) return fail(-2, "layer_forward: a gated layer takes no residual");
   if (f->b_up && !f->w_up) return fail(-2, "layer_forward: b_up without w_up");
   if (f->z_up && !f->w_up) return fail(-2, "layer_forward: z_up without w_up");
+  if ((rc = check_z(*f))) return rc;
   const long long need = BY_TYPE(f->dtype, mjlab_layer_forward_bytes, f);
   if (need > 0 && (!f->workspace || f->workspace_bytes < need)) return fail(-3, "layer_forward: workspace too small");
   return done(BY_TYPE(f->dtype, mjlab_launch_layer_forward, f, (hipStream_t)stream), "layer_forward launch failed");
@@ -66,9 +77,11 @@ int mjlab_layer_backward(const mjlab_layer_grad_t* g, void* stream) {
   if (rc) return rc;
   const bool gated = g->f.w_up != nullptr;
   if (!g->dy) return fail(-2, "layer_backward: null dy");
-  if ((gated || g->f.act != MJLAB_ACT_NONE) && !g->f.z) return fail(-2, "layer_backward: the sums before the activation (z) are missing");
+  const bool again = gated && !g->f.z && !g->f.z_up && mjlab_layer_recomputes(&g->f);
+  if (!again && (gated || g->f.act != MJLAB_ACT_NONE) && !g->f.z) return fail(-2, "layer_backward: the sums before the activation (z) are missing");
   if (g->f.z_is_y && (gated || !slope_from_output(g->f.act))) return fail(-2, "layer_backward: z_is_y: the output does not determine this layer's slope");
-  if (gated && !g->f.z_up) return fail(-2, "layer_backward: z_up is missing");
+  if (gated && !again && !g->f.z_up) return fail(-2, "layer_backward: z_up is missing");
+  if ((rc = check_z(g->f))) return rc;
   if (gated && ((g->dw != nullptr) != (g->dw_up != nullptr) || (g->db != nullptr) != (g->db_up != nullptr))) return fail(-2, "layer_backward: dw / dw_up and db / db_up come together");
   const long long need = BY_TYPE(g->f.dtype, mjlab_layer_backward_bytes, g);
   if (need > 0 && (!g->workspace || g->workspace_bytes < need)) return fail(-3, "layer_backward: workspace too small");

@@ -17,7 +17,7 @@
 #pragma once
 #include "policy_common.h"
 
-enum { EPI_LAYER = 0, EPI_GATED = 1, EPI_STORE = 2, EPI_PARTIAL = 3 };
+enum { EPI_LAYER = 0, EPI_GATED = 1, EPI_STORE = 2, EPI_PARTIAL = 3, EPI_SLOPE = 4 };
 
 struct Product {
   const void *A, *B, *B2;      // B2: w_up (EPI_GATED: rows of both in turn; EPI_STORE: the rows k >= kb2 of B)
@@ -29,7 +29,8 @@ struct Product {
   const void *b, *b_up, *r;    // the epilogue's
   void *y, *z, *z_up;
   long long ldr, ldy;
-  float* partial;              // EPI_PARTIAL: (splits, M, N)
+  float* partial;              // EPI_PARTIAL: (splits, M, N); EPI_SLOPE: column sums of y, (2 M / BM, 2 N), or NULL
+                               // EPI_SLOPE: a gated layer's sums formed again; r = dy, y = [dg | du]
 };
 
 __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c, _Float16) {
@@ -309,7 +310,7 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> struct ProductL
 template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __launch_bounds__(256, 2) void k_product(const Product p) {
   using S = Shape<T, BM, BN>;
   constexpr int V = Elem<T>::VEC, WM = BM / 2, WN = BN / 2, MI = WM / 32, NI = WN / 32;
-  constexpr bool GATED = EPI == EPI_GATED;
+  constexpr bool SLOPE = EPI == EPI_SLOPE, GATED = EPI == EPI_GATED || SLOPE;
   constexpr int BNO = GATED ? BN / 2 : BN, HALF = WN / 2;  // output columns per workgroup; a gated wave owns HALF columns of both products
   extern __shared__ __attribute__((aligned(16))) char lds[];
 
@@ -331,6 +332,7 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
   float* c = (float*)lds + wave * 32 * LD;
   constexpr int OV = EPI == EPI_PARTIAL ? 4 : V, OW = GATED ? HALF : WN, LPR = OW / OV, RPP = 64 / LPR;  // output elements per lane, lanes per row, rows per pass
   const int col = (lane % LPR) * OV;
+  float sum[SLOPE ? OV : 1] = {}, sum_up[SLOPE ? OV : 1] = {};  // of this lane's rows
   const long long n = n0 + (GATED ? wn / 2 : wn) + col, left = p.N - n;
   float bias[OV], bias_up[OV];
 #pragma unroll
@@ -346,9 +348,9 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
     // the residual's rows are on their way while C goes through LDS
-    Chunk<T> res[EPI == EPI_LAYER ? PASSES : 1];
-    if constexpr (EPI == EPI_LAYER) {
-      if (p.r) {
+    Chunk<T> res[EPI == EPI_LAYER || SLOPE ? PASSES : 1];
+    if constexpr (EPI == EPI_LAYER || SLOPE) {
+      if (SLOPE || p.r) {
 #pragma unroll
         for (int q = 0; q < PASSES; ++q) {
           const long long m = m0 + wm + i * 32 + q * RPP + lane / LPR;
@@ -391,8 +393,31 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
         for (int e = 0; e < OV; ++e) out.e[e] = (T)x[e];
         store_part((T*)base + m * ld + n, out, left);
       };
-      if constexpr (EPI != EPI_STORE) {
-        if (p.z) rows([&](int q, long long m) { put(p.z, p.N, q, m, v[q]); });
+      auto put_float = [&](void* base, int q, long long m, const float (&x)[OV]) {
+#pragma unroll
+        for (int e = 0; e < OV; e += 4) store_part((float*)base + m * p.N + n + e, Chunk<float>{{x[e], x[e + 1], x[e + 2], x[e + 3]}}, left - e);
+      };
+      if constexpr (SLOPE) {
+        with_act(p.act, [&](auto act) {
+          constexpr int ACT = decltype(act)::value;
+#pragma unroll
+          for (int q = 0; q < PASSES; ++q)
+#pragma unroll
+            for (int e = 0; e < OV; ++e) {
+              const float d = (float)res[q].e[e], g = v[q][e];  // (d is 0 behind the last row)
+              v[q][e] = d * act_slope<ACT>(g) * u[q][e];
+              u[q][e] = d * act_value<ACT>(g);
+              const bool there = m0 + wm + i * 32 + q * RPP + lane / LPR < p.M;  // (what stands behind may be infinite)
+              sum[e] += there ? v[q][e] : 0.f;
+              sum_up[e] += there ? u[q][e] : 0.f;
+            }
+        });
+        rows([&](int q, long long m) { put((T*)p.y + p.N, p.ldy, q, m, u[q]); });
+      } else if constexpr (EPI != EPI_STORE) {
+        if (p.z) rows([&](int q, long long m) {
+          if constexpr (GATED) put_float(p.z, q, m, v[q]);
+          else put(p.z, p.N, q, m, v[q]);
+        });
         with_act(p.act, [&](auto act) {
 #pragma unroll
           for (int q = 0; q < PASSES; ++q)
@@ -400,7 +425,7 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
             for (int e = 0; e < OV; ++e) v[q][e] = act_value<decltype(act)::value>(v[q][e]);
         });
         if constexpr (GATED) {
-          if (p.z_up) rows([&](int q, long long m) { put(p.z_up, p.N, q, m, u[q]); });
+          if (p.z_up) rows([&](int q, long long m) { put_float(p.z_up, q, m, u[q]); });
 #pragma unroll
           for (int q = 0; q < PASSES; ++q)
 #pragma unroll
@@ -413,6 +438,23 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
         }
       }
       rows([&](int q, long long m) { put(p.y, p.ldy, q, m, v[q]); });
+    }
+  }
+  if constexpr (SLOPE) {
+    if (p.partial) {
+#pragma unroll
+      for (int e = 0; e < OV; ++e)
+#pragma unroll
+        for (int x = LPR; x < 64; x *= 2) {
+          sum[e] += __shfl_xor(sum[e], x);
+          sum_up[e] += __shfl_xor(sum_up[e], x);
+        }
+      if (lane < LPR) {
+        float* to = p.partial + (m0 / BM * 2 + (wave >> 1)) * 2 * p.N + n;
+#pragma unroll
+        for (int e = 0; e < OV; ++e)
+          if (e < left) { to[e] = sum[e]; to[p.N + e] = sum_up[e]; }
+      }
     }
   }
 }
@@ -439,11 +481,14 @@ template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_join_
     if constexpr (GATED) u += p.partial[(k * p.M + m) * width + p.N + c];
   }
   if (p.b) v += (float)((const T*)p.b)[c];
-  if (p.z) ((T*)p.z)[i] = (T)v;
+  if (p.z) {
+    if constexpr (GATED) ((float*)p.z)[i] = v;
+    else ((T*)p.z)[i] = (T)v;
+  }
   with_act(p.act, [&](auto act) { v = act_value<decltype(act)::value>(v); });
   if constexpr (GATED) {
     if (p.b_up) u += (float)((const T*)p.b_up)[c];
-    if (p.z_up) ((T*)p.z_up)[i] = (T)u;
+    if (p.z_up) ((float*)p.z_up)[i] = u;
     v *= u;
   } else if (p.r) v += (float)((const T*)p.r)[m * p.ldr + c];
   ((T*)p.y)[m * p.ldy + c] = (T)v;
@@ -453,7 +498,7 @@ template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_join_
 // 256 threads: 32 chunk columns x 8 rows, four rows of each thread in flight, over SLOPE_ROWS rows; workgroups: row blocks x `colblocks`.
 // dz NULL: column sums of dy alone.  FROM: what is stored is the layer's output.  Bound by memory: dense two reads and a write, gated three and two.
 #define SLOPE_ROWS 64
-template <typename T, bool GATED, bool FROM> __global__ __launch_bounds__(256) void k_layer_slope(const T* dy, long long ld_dy, const T* z, const T* z_up, T* dz,
+template <typename T, bool GATED, bool FROM> __global__ __launch_bounds__(256) void k_layer_slope(const T* dy, long long ld_dy, const void* z, const float* z_up, T* dz,
                                                                                                    float* sums, long long rows, long long out, unsigned colblocks, int act) {
   constexpr int V = Elem<T>::VEC, NS = GATED ? 2 : 1, ROWS = GATED ? 1 : 2;
   __shared__ float part[NS][8][32 * V];
@@ -463,29 +508,37 @@ template <typename T, bool GATED, bool FROM> __global__ __launch_bounds__(256) v
   float s[NS][V] = {};
   const bool slope = dz && (GATED || act != MJLAB_ACT_NONE);
   for (int i = ty; i < SLOPE_ROWS && r0 + i < rows; i += 8 * ROWS) {
-    Chunk<T> d[ROWS], g[ROWS], u[ROWS];
+    Chunk<T> d[ROWS], g[ROWS];
+    float z0[GATED ? ROWS : 1][V], z1[GATED ? ROWS : 1][V];  // (a gated layer's sums are floats)
 #pragma unroll
     for (int q = 0; q < ROWS; ++q) {
       const long long m = r0 + i + 8 * q, have = m < rows ? left : 0;
       d[q] = load_part(dy + m * ld_dy + n, have);
-      if (slope) g[q] = load_part(z + m * out + n, have);
-      if constexpr (GATED) u[q] = load_part(z_up + m * out + n, have);
+      if constexpr (GATED) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+          const Chunk<float> x = load_part((const float*)z + m * out + n + e, have - e), y = load_part(z_up + m * out + n + e, have - e);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) { z0[q][e + k] = x.e[k]; z1[q][e + k] = y.e[k]; }
+        }
+      } else if (slope) g[q] = load_part((const T*)z + m * out + n, have);
     }
 #pragma unroll
     for (int q = 0; q < ROWS; ++q) {
       const long long m = r0 + i + 8 * q;
       if (slope) {
+        Chunk<T> o;
         with_act(act, [&](auto a) {
           constexpr int ACT = decltype(a)::value;
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float x = (float)g[q].e[e], t = (float)d[q].e[e];
+            const float x = GATED ? z0[GATED ? q : 0][e] : (float)g[q].e[e], t = (float)d[q].e[e];
             float v = t * (FROM ? act_slope_out<ACT>(x) : act_slope<ACT>(x));
             if constexpr (GATED) {
-              v *= (float)u[q].e[e];
+              v *= z1[q][e];
               const float w = t * act_value<ACT>(x);
               s[NS - 1][e] += w;
-              u[q].e[e] = (T)w;
+              o.e[e] = (T)w;
             }
             s[0][e] += v;
             d[q].e[e] = (T)v;
@@ -493,7 +546,7 @@ template <typename T, bool GATED, bool FROM> __global__ __launch_bounds__(256) v
         });
         if (m < rows && left > 0) {
           store_part(dz + m * (NS * out) + n, d[q], left);
-          if constexpr (GATED) store_part(dz + m * (NS * out) + out + n, u[q], left);
+          if constexpr (GATED) store_part(dz + m * (NS * out) + out + n, o, left);
         }
       } else {
 #pragma unroll

@@ -29,7 +29,7 @@ ACTIVATIONS = {"none": 0, "relu": 1, "elu": 2, "tanh": 3, "sigmoid": 4, "silu": 
 
 
 class Layer(ctypes.Structure):  # mjlab_layer_t
-  _fields_ = [("dtype", ctypes.c_int), ("act", ctypes.c_int), ("z_is_y", ctypes.c_int), ("pad_", ctypes.c_int), ("rows", _ll), ("inp", _ll), ("out", _ll),
+  _fields_ = [("dtype", ctypes.c_int), ("act", ctypes.c_int), ("z_is_y", ctypes.c_int), ("z_bytes", ctypes.c_int), ("rows", _ll), ("inp", _ll), ("out", _ll),
               ("x", _vp), ("w", _vp), ("w_up", _vp), ("b", _vp), ("b_up", _vp), ("r", _vp),
               ("ldx", _ll), ("ldw", _ll), ("ldw_up", _ll), ("ldr", _ll), ("ldy", _ll), ("y", _vp), ("z", _vp), ("z_up", _vp),
               ("workspace", _vp), ("workspace_bytes", _ll)]  # fmt: skip
@@ -120,11 +120,16 @@ def _forward(x, w, w_up, b, b_up, r, act: int, keep: bool, y=None):
   (m, k), n = x.shape, w.shape[0]
   if y is None:
     y = x.new_empty((m, n))
-  z = x.new_empty((m, n)) if keep and (act or w_up is not None) and not _from_output(x, w_up, r, act) else None
-  z_up = x.new_empty((m, n)) if keep and w_up is not None else None
+  z = z_up = None
   if m:
-    args = (DTYPES[x.dtype], act, 0, 0, m, k, n, x.data_ptr(), w.data_ptr(), _ptr(w_up), _ptr(b), _ptr(b_up), _ptr(r), _ld(x), _ld(w),
-            0 if w_up is None else _ld(w_up), 0 if r is None else _ld(r), _ld(y), y.data_ptr(), _ptr(z), _ptr(z_up))  # fmt: skip
+    dtype, lds = DTYPES[x.dtype], (_ld(x), _ld(w), 0 if w_up is None else _ld(w_up), 0 if r is None else _ld(r), _ld(y))
+    inputs = (x.data_ptr(), w.data_ptr(), _ptr(w_up), _ptr(b), _ptr(b_up), _ptr(r))
+    if keep and w_up is not None:
+      if not native.policy_lib().mjlab_layer_recomputes(_LAYER.pack(dtype, act, 0, 0, m, k, n, *inputs, *lds, 0, 0, 0, 0, 0)):
+        z, z_up = (torch.empty((m, n), dtype=torch.float32, device=x.device) for _ in range(2))
+    elif keep and act and not _from_output(x, w_up, r, act):
+      z = x.new_empty((m, n))
+    args = (dtype, act, 0, 0 if z is None else z.element_size(), m, k, n, *inputs, *lds, y.data_ptr(), _ptr(z), _ptr(z_up))
     need = native.policy_lib().mjlab_layer_forward_workspace(_LAYER.pack(*args, 0, 0))
     if need < 0:
       native.policy_check(need, "mjlab_layer_forward_workspace")
@@ -138,14 +143,15 @@ class _Layer(torch.autograd.Function):
   def forward(ctx, x, w, w_up, b, b_up, r, act):
     y, z, z_up = _forward(x, w, w_up, b, b_up, r, act, keep=True)
     ctx.z_is_y = _from_output(x, w_up, r, act)
-    ctx.save_for_backward(x, w, w_up, y if ctx.z_is_y else z, z_up)
+    again = w_up is not None and z is None
+    ctx.save_for_backward(x, w, w_up, y if ctx.z_is_y else z, z_up, b if again else None, b_up if again else None)
     ctx.act = act
     return y
 
   @staticmethod
   @torch.autograd.function.once_differentiable
   def backward(ctx, dy):
-    x, w, w_up, z, z_up = ctx.saved_tensors
+    x, w, w_up, z, z_up, b, b_up = ctx.saved_tensors  # (the biases where the sums are formed again)
     need_x, need_w, need_wu, need_b, need_bu, need_r, _ = ctx.needs_input_grad
     (m, k), n, gated = x.shape, w.shape[0], w_up is not None
     dr = dy if need_r else None
@@ -163,7 +169,8 @@ class _Layer(torch.autograd.Function):
     elif dx is not None or dw is not None or db is not None:
 
       def pack(workspace: int, size: int) -> bytes:
-        return _LAYER_GRAD.pack(DTYPES[x.dtype], ctx.act, ctx.z_is_y, 0, m, k, n, x.data_ptr(), w.data_ptr(), _ptr(w_up), 0, 0, 0, _ld(x), _ld(w),
+        return _LAYER_GRAD.pack(DTYPES[x.dtype], ctx.act, ctx.z_is_y, 0 if z is None else z.element_size(), m, k, n, x.data_ptr(), w.data_ptr(), _ptr(w_up),
+                                _ptr(b), _ptr(b_up), 0, _ld(x), _ld(w),
                                 _ld(w_up) if gated else 0, 0, 0, 0, _ptr(z), _ptr(z_up), 0, 0, dy.data_ptr(), _ld(dy), _ptr(dx), _ptr(dw), _ptr(dwu), _ptr(db), _ptr(dbu),
                                 workspace, size)  # fmt: skip
 

@@ -53,19 +53,29 @@ def test_layer_forward_refuses(kw, text):
 @pytest.mark.parametrize("kw,text", [
   (dict(dy=None), "null dy"), (dict(f=dict(z=None)), "(z)"), (dict(f=dict(w_up=64, ldw_up=8)), "z_up"),
   (dict(f=dict(w_up=64, ldw_up=8, z_up=64), dw=64), "together"), (dict(workspace_bytes=16), "workspace"), (dict(workspace=None), "workspace"),
-  (dict(f=dict(rows=-1)), "sizes"), (dict(f=dict(act=5, z_is_y=1)), "z_is_y"),
+  (dict(f=dict(rows=-1)), "sizes"), (dict(f=dict(act=5, z_is_y=1)), "z_is_y"), (dict(f=dict(z_bytes=2)), "z_bytes"),
+  (dict(f=dict(w_up=64, ldw_up=8, z=None)), "(z)"), (dict(f=dict(dtype=2, w_up=64, ldw_up=2000, inp=2000, ldw=2000, z=None)), "(z)"),
 ])  # fmt: skip
 def test_layer_backward_refuses(kw, text):
   lib = native.policy_lib()
   g = policy_ops.LayerGrad()
   kw = dict(kw)
-  g.f = _layer(**{"z": 64, **kw.pop("f", {})})
+  g.f = _layer(**{"z": 64, "z_bytes": 4, **kw.pop("f", {})})
   vals = dict(dy=64, ld_dy=3, dx=64, workspace=64, workspace_bytes=1 << 30)
   vals.update(kw)
   for k, v in vals.items():
     setattr(g, k, v)
   assert lib.mjlab_layer_backward(ctypes.byref(g), None) < 0
   assert text in lib.mjlab_policy_last_error().decode()
+
+
+def test_which_gated_layers_form_their_sums_again():
+  lib = native.policy_lib()
+  gated = dict(w_up=64, ldw_up=512, inp=512, ldw=512)
+  assert lib.mjlab_layer_recomputes(ctypes.byref(_layer(dtype=2, **gated))) == 1
+  assert lib.mjlab_layer_recomputes(ctypes.byref(_layer(dtype=0, **gated))) == 0
+  assert lib.mjlab_layer_recomputes(ctypes.byref(_layer(dtype=2, **{**gated, "inp": 4096}))) == 0
+  assert lib.mjlab_layer_recomputes(ctypes.byref(_layer(dtype=2))) == 0
 
 
 def test_few_rows_of_a_wide_layer_split_their_sums():
