@@ -28,19 +28,21 @@ float tile_cost(long long tiles, float cost, int at_once) {
 struct Cost {
   float small, mid, large, best;
 };
-template <bool BK> Cost costs(long long M, long long width, long long splits) {
+// A layer's epilogue (BK: the products that have one) is hidden behind the other workgroups of a CU, of which the large tile leaves one: counted as 0.13 of the
+// large tile's time at 1024 k (gated bf16 24576 rows, us, large / mid: 512 x 1365 122 / 110, [dg | du] 187 / 158; 1024 x 2048 264 / 264).
+template <bool BK> Cost costs(long long M, long long width, long long K, long long splits) {
   auto tiles = [&](int bm, int bn) { return (M + bm - 1) / bm * ((width + bn - 1) / bn) * splits; };
   constexpr bool F32 = sizeof(T) == 4;
   Cost c;
   c.small = tile_cost(tiles(64, 64), F32 ? 0.166f : BK ? 0.2f : 0.28f, F32 ? 3 : 5);
   c.mid = tile_cost(tiles(128, 128), F32 ? 0.5f : BK ? 0.56f : 0.62f, BK ? 3 : 2);
-  c.large = F32 ? 1e30f : tile_cost(tiles(256, 128), 1.f, 2);
+  c.large = F32 ? 1e30f : tile_cost(tiles(256, 128), BK ? 1.f + 133.f / K : 1.f, 2);
   c.best = c.large < c.mid && c.large < c.small ? c.large : c.mid < c.small ? c.mid : c.small;
   return c;
 }
 
 template <bool AK, bool BK, int EPI> hipError_t launch_product(const Product& p, int splits, hipStream_t st) {
-  const Cost c = costs<BK>(p.M, EPI == EPI_GATED || EPI == EPI_SLOPE ? 2 * p.N : p.N, splits);
+  const Cost c = costs<BK>(p.M, EPI == EPI_GATED || EPI == EPI_SLOPE ? 2 * p.N : p.N, p.K, splits);
   if constexpr (sizeof(T) == 2)
     if (c.best == c.large) return launch_tile<AK, BK, 256, 128, EPI>(p, splits, st);
   return c.best == c.mid ? launch_tile<AK, BK, 128, 128, EPI>(p, splits, st) : launch_tile<AK, BK, 64, 64, EPI>(p, splits, st);
@@ -52,9 +54,9 @@ template <bool AK, bool BK, int EPI> hipError_t launch_product(const Product& p,
 template <bool BK> int sum_splits(long long M, long long width, long long K) {
   const float per_k = sizeof(T) == 4 ? 0.08f : 0.021f;
   int best = 1;
-  float time = costs<BK>(M, width, 1).best * K * per_k;
+  float time = costs<BK>(M, width, K, 1).best * K * per_k;
   for (int s = 2; s <= 32 && K / s >= 128; s *= 2) {
-    const float t = costs<BK>(M, width, s).best * K / s * per_k + 4.f + 4e-6f * M * width * s * 0.67f;
+    const float t = costs<BK>(M, width, K, s).best * K / s * per_k + 4.f + 4e-6f * M * width * s * 0.67f;
     if (t < time) { time = t; best = s; }
   }
   return best;
@@ -88,7 +90,7 @@ Plan plan(const mjlab_layer_grad_t* g) {
   q.again = q.gated && !f.z;
   q.blocks = (f.rows + SLOPE_ROWS - 1) / SLOPE_ROWS;
   if (q.again) {  // two sets of column sums per tile of rows
-    const Cost c = costs<true>(f.rows, 2 * f.out, 1);
+    const Cost c = costs<true>(f.rows, 2 * f.out, f.in, 1);
     const int bm = c.best == c.large ? 256 : c.best == c.mid ? 128 : 64;
     q.blocks = 2 * ((f.rows + bm - 1) / bm);
   }
