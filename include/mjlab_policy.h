@@ -105,6 +105,7 @@ typedef struct mjlab_decay_grad {
   mjlab_decay_rows_t d_out, dq, dk, dv;
   const float* d_state_out;
   float* d_state;
+  const void* segments; /* the forward pass's workspace as it left it, which saves a pass over long sequences, or NULL; not f.workspace, which is written */
 } mjlab_decay_grad_t;
 int mjlab_decay_backward(const mjlab_decay_grad_t* g, void* stream);
 int mjlab_sizeof_decay_grad(void);

@@ -20,12 +20,13 @@ struct DecayPass {
   const float* state_in;  // or NULL
   float* state_out;       // or NULL
   int in_r, in_c;         // strides of the rows (da) and columns (dc) of state_in; state_out is (da, dc) dense
+  int seg_given;          // the segments' states are there: those of the pass with da and dc exchanged
   const void* reset;
   int reset_bytes, heads, da, dc, e0, reverse, segments, seg_chunks;
   long long reset_b, reset_t, length;
   const int* lengths;
   float ps, is, us;
-  float *seg_state, *seg_factor;  // (sequences * heads, segments - 1, da, dc), (sequences * heads, segments - 1)
+  float *seg_state, *seg_factor;  // (seg_given: seg_state is read only) (sequences * heads, segments - 1, da, dc), (sequences * heads, segments - 1)
 };
 
 // What the matrix cores read: bf16 as it is; float, and fp16 turned into float (whose products and sums of keys and values may leave fp16's range).
@@ -66,9 +67,9 @@ __device__ __forceinline__ bool reset_at(const DecayPass& p, long long seq, long
 template <typename T, int DA, int DC, bool STATE> struct DecayLds {
   using L = typename DecayCfg<T>::L;
   static constexpr int C = DecayCfg<T>::C, PAD = DecayCfg<T>::PAD, LA = DA + PAD, LC = DC + PAD, LP = C + PAD;
-  L b[C * LA], c[C * LC], p[STATE ? 1 : C * LP], r[STATE ? 1 : DC * LA];
-  float weight[C], enter[C];  // of token j into R; of R into token i
-  int odd[8];
+  L b[STATE ? 8 : C * LA], bw[C * LA], c[C * LC], p[STATE ? 8 : C * LP], r[STATE ? 8 : DC * LA];  // bw: b times its tokens' weights into R
+  float enter[C];                 // of R into token i
+  int episode[C], odd[8];         // the episode a token belongs to, counted in the chunk
 };
 
 // VEC elements of T as elements of L, to an address aligned for them
@@ -88,20 +89,32 @@ __device__ __forceinline__ void put4(__bf16* at, const f32x4& x) {
 }
 __device__ __forceinline__ void put4(float* at, const f32x4& x) { *(f32x4*)at = x; }
 
-// the weights of 16 / 4 tokens k on a fragment
-__device__ __forceinline__ s16x8 weigh(s16x8 f, const float* w, int k0, int lane) {
-  const b16x8 x = __builtin_bit_cast(b16x8, f);
-  b16x8 y;
+// x times w (w 0: zeros, whatever x holds), as elements of L
+template <typename T, typename L> __device__ __forceinline__ void put_weighted(L* at, const Chunk<T>& x, float w) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = w[k0 + (lane >> 4) * 8 + i];
-    y[i] = (__bf16)(t == 0.f ? 0.f : t * (float)x[i]);
+  for (int h = 0; h < Elem<T>::VEC; h += 4) {
+    f32x4 y;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = w * (float)x.e[h + e];
+    put4(at + h, w == 0.f ? f32x4{} : y);
   }
-  return __builtin_bit_cast(s16x8, y);
 }
-__device__ __forceinline__ float weigh(float x, const float* w, int k0, int lane) {
-  const float t = w[k0 + (lane >> 4)];
-  return t == 0.f ? 0.f : t * x;
+
+// Whether a chunk held an infinity or a NaN: the largest magnitude's bits, two 16-bit elements at a time
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+template <typename T> __device__ __forceinline__ void see(unsigned& most, const Chunk<T>& x) {
+  unsigned w[4];
+  __builtin_memcpy(w, &x, 16);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) most = most > (w[i] & 0x7fffffffu) ? most : w[i] & 0x7fffffffu;
+    else most = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most), __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu)));
+  }
+}
+template <typename T> __device__ __forceinline__ bool seen_odd(unsigned most) {
+  if constexpr (sizeof(T) == 4) return most >= 0x7f800000u;
+  constexpr unsigned INF = Elem<T>::DTYPE == MJLAB_DTYPE_F16 ? 0x7c00u : 0x7f80u;
+  return (most >> 16) >= INF || (most & 0xffffu) >= INF;
 }
 
 // Elements col .. col + VEC - 1 of a row of d, zero from d on.  FULL: all of them are there.
@@ -138,6 +151,7 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
   float g2 = p.log_decay[head] * 1.44269504f;
   g2 = g2 < -1e30f ? -1e30f : g2;
   auto power = [&](int n) { return __builtin_amdgcn_exp2f(n * g2); };
+  const float decay = power(1);
   long long len = p.length;
   if (p.lengths) { const long long l = p.lengths[seq]; len = l < 0 ? 0 : (l < len ? l : len); }
   const T *ga = (const T*)p.a + seq * p.a_b + head * p.a_h, *gb = (const T*)p.b + seq * p.b_b + head * p.b_h, *gc = (const T*)p.c + seq * p.c_b + head * p.c_h;
@@ -229,7 +243,7 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
   // R, tile (i, j) of this wave: rows (of da) (r0 + i) * 16 + row4 .. + 3, column (of dc) (rc0 + j) * 16 + colx
   f32x4 acc[RR][RC];
   const float* start = STATE ? nullptr : seg ? p.seg_state + (sh * (p.segments - 1) + seg - 1) * p.da * p.dc : p.state_in ? p.state_in + sh * p.da * p.dc : nullptr;
-  const int sr = seg ? p.dc : p.in_r, sc = seg ? 1 : p.in_c;
+  const int sr = !seg ? p.in_r : p.seg_given ? 1 : p.dc, sc = !seg ? p.in_c : p.seg_given ? p.da : 1;
 #pragma unroll
   for (int i = 0; i < RR; ++i)
 #pragma unroll
@@ -262,22 +276,25 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
     const bool carries = n == 0 || (e_last == 0 && !cut_out);  // R goes through the whole chunk
 
     __syncthreads();  // the chunk before is done with LDS
-    bool odd = false;
+    unsigned most = 0;
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
-      const int idx = tid + i * NT, row = idx / (DA / V), col = idx % (DA / V) * V;
-      if (row < C) put_chunk(s.b + row * LA + col, xb[i]);
+      const int row = (tid + i * NT) / (DA / V), col = (tid + i * NT) % (DA / V) * V;
+      if (row >= C) continue;
+      const float w = row < n && !cut_out && (whole || episode(row) == e_last) ? p.us * power(n - p.e0 - row) : 0.f;
+      put_weighted(s.bw + row * LA + col, xb[i], w);
+      if constexpr (!STATE) put_chunk(s.b + row * LA + col, xb[i]);
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-      const int idx = tid + i * NT, row = idx / (DC / V), col = idx % (DC / V) * V;
-#pragma unroll
-      for (int e = 0; e < V; ++e) odd |= not_finite((float)xc[i].e[e]);
-      if (row < C) put_chunk(s.c + row * LC + col, xc[i]);
+      const int row = (tid + i * NT) / (DC / V), col = (tid + i * NT) % (DC / V) * V;
+      if (row >= C) continue;
+      see(most, xc[i]);
+      put_chunk(s.c + row * LC + col, xc[i]);
     }
-    if (tid < C) {
-      s.weight[tid] = tid < n && !cut_out && episode(tid) == e_last ? p.us * power(n - p.e0 - tid) : 0.f;
+    if (!STATE && tid < C) {
       s.enter[tid] = tid < n && episode(tid) == 0 ? p.is * power(tid + p.e0) : 0.f;
+      s.episode[tid] = episode(tid);
     }
     const bool carry = start || q0 > first;  // else R is zero so far
     if (!STATE && carry) {
@@ -287,7 +304,7 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
         for (int j = 0; j < RC; ++j) put4(s.r + ((rc0 + j) * 16 + colx) * LA + (r0 + i) * 16 + row4, acc[i][j]);
     }
     // A zero weight times infinity would be NaN: a chunk whose c holds one goes term by term.
-    const bool mine = __ballot(odd) != 0;
+    const bool mine = __ballot(seen_odd<T>(most)) != 0;
     if (lane == 0) s.odd[wave] = mine;
     __syncthreads();
     int any = 0;
@@ -301,17 +318,25 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
       f32x4 x[TR][TC];
 #pragma unroll
       for (int t = 0; t < TR; ++t) {
-        const int i = (t0 + t) * 16 + colx, ei = episode(i);
+        const int i = (t0 + t) * 16 + colx, ei = s.episode[i];
 #pragma unroll
         for (int jj = 0; jj < CT / OC + (CT % OC ? 1 : 0); ++jj) {
-          const int tj = jj * OC + wave % OC;
+          const int tj = jj * OC + wave % OC, j = tj * 16 + row4;
           if (tj >= CT) continue;
           f32x4 y = {};
-          if (tj <= t0 + t) y = with_a(s.b, tj * 16, t, y);
+          if (tj <= t0 + t) {
+            y = with_a(s.b, tj * 16, t, y);
+            float w[4];
+            if (tj == t0 + t) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int j = tj * 16 + row4 + e;
-            y[e] = j <= i && i < n && (whole || episode(j) == ei) ? p.ps * power(i - j) * y[e] : 0.f;
+              for (int e = 0; e < 4; ++e) w[e] = j + e <= i ? p.ps * power(i - j - e) : 0.f;
+            } else {  // (i > j + 3: neighbours' weights are a decay apart)
+              w[3] = p.ps * power(i - j - 3);
+#pragma unroll
+              for (int e = 2; e >= 0; --e) w[e] = decay * w[e + 1];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = (tj < t0 + t || j + e <= i) && i < n && (whole || s.episode[j + e] == ei) ? w[e] * y[e] : 0.f;
           }
           put4(s.p + i * LP + tj * 16 + row4, y);
           __builtin_amdgcn_sched_barrier(0);
@@ -341,9 +366,9 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
       } else {
 #pragma unroll
         for (int t = 0; t < TR; ++t) {
-          const int i = (t0 + t) * 16 + colx, ei = episode(i);
+          const int i = (t0 + t) * 16 + colx, ei = s.episode[i];
           for (int j = 0; j <= i && i < n; ++j)
-            if (episode(j) == ei) {
+            if (s.episode[j] == ei) {
               const float w = (float)s.p[i * LP + j];
 #pragma unroll
               for (int c = 0; c < TC; ++c)
@@ -378,18 +403,25 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
     if (!STATE && !end && q0 + C >= last) break;  // nobody wants R any more
     const float through = carries ? power(n) : 0.f;
     factor *= through;
+    if (carries) {
 #pragma unroll
-    for (int i = 0; i < RR; ++i)
+      for (int i = 0; i < RR; ++i)
 #pragma unroll
-      for (int j = 0; j < RC; ++j)
+        for (int j = 0; j < RC; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[i][j][e] = carries ? through * acc[i][j][e] : 0.f;
+          for (int e = 0; e < 4; ++e) acc[i][j][e] *= through;
+    } else {  // (whatever it holds)
+#pragma unroll
+      for (int i = 0; i < RR; ++i)
+#pragma unroll
+        for (int j = 0; j < RC; ++j) acc[i][j] = f32x4{};
+    }
     if (!by_term) {
 #pragma unroll 2
       for (int k = 0; k < C; k += KS) {
-        decltype(frag_kr(s.b, LA, 0, 0, lane)) fb[RR];
+        decltype(frag_kr(s.bw, LA, 0, 0, lane)) fb[RR];
 #pragma unroll
-        for (int i = 0; i < RR; ++i) fb[i] = weigh(frag_kr(s.b, LA, (r0 + i) * 16, k, lane), s.weight, k, lane);
+        for (int i = 0; i < RR; ++i) fb[i] = frag_kr(s.bw, LA, (r0 + i) * 16, k, lane);
 #pragma unroll
         for (int j = 0; j < RC; ++j) {
           const auto fc = frag_kr(s.c, LC, (rc0 + j) * 16, k, lane);
@@ -400,8 +432,7 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
       }
     } else {
       for (int t = 0; t < n; ++t) {
-        const float w = s.weight[t];
-        if (w == 0.f) continue;
+        if (cut_out || episode(t) != e_last) continue;
 #pragma unroll
         for (int i = 0; i < RR; ++i)
 #pragma unroll
@@ -409,7 +440,7 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = (r0 + i) * 16 + row4 + e;
-              if (FULL || r < p.da) acc[i][j][e] += (float)(L)(w * (float)s.b[t * LA + r]) * (float)s.c[t * LC + (rc0 + j) * 16 + colx];
+              if (FULL || r < p.da) acc[i][j][e] += (float)s.bw[t * LA + r] * (float)s.c[t * LC + (rc0 + j) * 16 + colx];
             }
       }
     }

@@ -12,7 +12,8 @@ struct Split {
 // heads), of four chunks at least: the first pass reads two of the operands again and moves R through memory once per segment.
 Split split(const mjlab_decay_t* d) {
   constexpr int C = DecayCfg<T>::C;
-  const long long chunks = (d->length + C - 1) / C, rows = d->batch * d->heads, slots = d->dk > 64 && d->dv > 64 ? CUS : 2 * CUS;
+  const long long chunks = (d->length + C - 1) / C, rows = d->batch * d->heads, least = d->dk < d->dv ? d->dk : d->dv, most_d = d->dk < d->dv ? d->dv : d->dk;
+  const long long slots = least > 32 && most_d > 64 ? CUS : 2 * CUS;  // workgroups that are resident: one of eight waves per CU, or two
   if (2 * rows >= slots || chunks < 8) return {1, (int)chunks};
   const long long want = slots / rows, most = chunks / 4, s = want < most ? want : most;
   const long long per = (chunks + s - 1) / s;
@@ -26,8 +27,8 @@ template <int DA, int DC, bool FULL> hipError_t launch_sized(const DecayPass& p,
   constexpr int LDS = (int)sizeof(DecayLds<T, DA, DC, false>), LDS_FIRST = (int)sizeof(DecayLds<T, DA, DC, true>);
   static std::atomic<unsigned long long> asked{0}, asked_first{0};
   hipError_t e;
-  if (rows * p.segments > MAX_BLOCKS) return hipErrorInvalidValue;
-  if (p.segments > 1) {
+  if (rows * p.segments * decay_threads(DA, DC) > 0xffffffffLL) return hipErrorInvalidValue;
+  if (p.segments > 1 && !p.seg_given) {
     auto first = k_decay_chunks<T, DA, DC, FULL, true>;
     if ((e = allow_lds(first, LDS_FIRST, asked_first)) != hipSuccess) return e;
     hipLaunchKernelGGL(first, dim3((unsigned)(rows * (p.segments - 1))), dim3(decay_threads(DA, DC)), LDS_FIRST, st, p);
@@ -51,7 +52,7 @@ template <int DA> hipError_t launch_dc(const DecayPass& p, long long rows, hipSt
 
 // out = the pass over a, b (heads of da) and c (of dc); see decay.h
 hipError_t launch(const mjlab_decay_t* d, const mjlab_decay_rows_t& a, const mjlab_decay_rows_t& b, const mjlab_decay_rows_t& c, const mjlab_decay_rows_t& out, int da,
-                  int dc, bool reverse, const float* state_in, bool turned, float* state_out, hipStream_t st) {
+                  int dc, bool reverse, const float* state_in, bool turned, float* state_out, hipStream_t st, const void* segments = nullptr) {
   const Split s = split(d);
   DecayPass p = {};
   p.a = a.p; p.a_b = a.batch; p.a_t = a.time; p.a_h = a.head;
@@ -64,7 +65,8 @@ hipError_t launch(const mjlab_decay_t* d, const mjlab_decay_rows_t& a, const mjl
   p.heads = d->heads; p.da = da; p.dc = dc; p.e0 = reverse ? 0 : 1; p.reverse = reverse; p.segments = s.segments; p.seg_chunks = s.seg_chunks;
   p.length = d->length; p.lengths = d->lengths;
   p.ps = d->scale; p.is = reverse ? 1.f : d->scale; p.us = reverse ? d->scale : 1.f;
-  p.seg_state = (float*)d->workspace; p.seg_factor = (float*)((char*)d->workspace + state_bytes(d, s));
+  p.seg_given = segments != nullptr;
+  p.seg_state = segments ? (float*)segments : (float*)d->workspace; p.seg_factor = (float*)((char*)d->workspace + state_bytes(d, s));
   const long long rows = d->batch * d->heads;
   return da <= 32 ? launch_dc<32>(p, rows, st) : da <= 64 ? launch_dc<64>(p, rows, st) : launch_dc<128>(p, rows, st);
 }
@@ -90,9 +92,10 @@ hipError_t POLICY_NAME(mjlab_launch_decay_backward)(const mjlab_decay_grad_t* g,
   const mjlab_decay_t* d = &g->f;
   if (d->length <= 32) return POLICY_NAME(mjlab_launch_short_backward)(g, st);
   hipError_t e;
-  if (g->dq.p && (e = launch(d, g->d_out, d->v, d->k, g->dq, d->dv, d->dk, false, d->state, true, nullptr, st)) != hipSuccess) return e;
-  if (g->dk.p && (e = launch(d, d->v, g->d_out, d->q, g->dk, d->dv, d->dk, true, g->d_state_out, true, nullptr, st)) != hipSuccess) return e;
+  // dq's R is the forward pass's transposed, dk's is dv's: the states of their segments serve both
+  if (g->dq.p && (e = launch(d, g->d_out, d->v, d->k, g->dq, d->dv, d->dk, false, d->state, true, nullptr, st, g->segments)) != hipSuccess) return e;
   if (g->dv.p && (e = launch(d, d->k, d->q, g->d_out, g->dv, d->dk, d->dv, true, g->d_state_out, false, g->d_state, st)) != hipSuccess) return e;
+  if (g->dk.p && (e = launch(d, d->v, g->d_out, d->q, g->dk, d->dv, d->dk, true, g->d_state_out, true, nullptr, st, g->dv.p ? d->workspace : nullptr)) != hipSuccess) return e;
   return hipSuccess;
 }
 

@@ -128,6 +128,7 @@ int mjlab_decay_backward(const mjlab_decay_grad_t* g, void* stream) {
   if (!g->d_out.p) return fail(-2, "decay_backward: null d_out");
   if (g->d_state && (!g->dv.p || g->d_state == g->d_state_out)) return fail(-2, "decay_backward: d_state comes with dv and must not be d_state_out");
   if ((rc = check_decay_workspace(g->f))) return rc;
+  if (g->segments && g->segments == g->f.workspace) return fail(-2, "decay_backward: segments must not be the workspace");
   return done(BY_TYPE(g->f.dtype, mjlab_launch_decay_backward, g, (hipStream_t)stream), "decay_backward launch failed");
 }
 

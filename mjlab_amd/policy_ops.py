@@ -52,7 +52,7 @@ class Decay(ctypes.Structure):  # mjlab_decay_t
 
 
 class DecayGrad(ctypes.Structure):  # mjlab_decay_grad_t
-  _fields_ = [("f", Decay), ("d_out", Rows), ("dq", Rows), ("dk", Rows), ("dv", Rows), ("d_state_out", _vp), ("d_state", _vp)]
+  _fields_ = [("f", Decay), ("d_out", Rows), ("dq", Rows), ("dk", Rows), ("dv", Rows), ("d_state_out", _vp), ("d_state", _vp), ("segments", _vp)]
 
 
 # A call's argument struct is packed in one go (setting two dozen ctypes fields one by one takes longer than a small layer's kernel): the layouts of the
@@ -61,7 +61,7 @@ _LAYER = struct.Struct("@4i3q6P5q3PPq")
 _LAYER_GRAD = struct.Struct("@4i3q6P5q3PPq" "Pq5PPq")
 _ROWS = "P3q"
 _DECAY = struct.Struct("@2i2q3if" + 4 * _ROWS + "3PP2q2Pq")
-_DECAY_GRAD = struct.Struct("@2i2q3if" + 4 * _ROWS + "3PP2q2Pq" + 4 * _ROWS + "2P")
+_DECAY_GRAD = struct.Struct("@2i2q3if" + 4 * _ROWS + "3PP2q2Pq" + 4 * _ROWS + "3P")
 assert _LAYER.size == ctypes.sizeof(Layer) and _LAYER_GRAD.size == ctypes.sizeof(LayerGrad)
 assert _DECAY.size == ctypes.sizeof(Decay) and _DECAY_GRAD.size == ctypes.sizeof(DecayGrad)
 
@@ -307,12 +307,14 @@ def _rows_like(t: torch.Tensor, d: int) -> torch.Tensor:
   return t.new_empty((n, b, h, d)).transpose(0, 1) if b > 1 and n > 1 and t.stride(1) > t.stride(0) else t.new_empty((b, n, h, d))
 
 
-def _decay_launch(fn: str, layout: struct.Struct, head: tuple, tail: tuple, dev: torch.device) -> None:
+def _decay_launch(fn: str, layout: struct.Struct, head: tuple, tail: tuple, dev: torch.device) -> torch.Tensor | None:
+  """-> the workspace, which the forward pass leaves the states of its segments in."""
   need = native.policy_lib().mjlab_decay_workspace(_DECAY.pack(*head, 0, 0))
   if need < 0:
     native.policy_check(need, "mjlab_decay_workspace")
   ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
   _call(fn, layout.pack(*head, _ptr(ws), need, *tail), dev)
+  return ws
 
 
 def _decay_forward(q, k, v, state, log_decay, scale, reset, lengths):
@@ -320,24 +322,25 @@ def _decay_forward(q, k, v, state, log_decay, scale, reset, lengths):
   o = _rows_like(q, v.shape[3])
   if b == 0 or n == 0:
     final = q.new_zeros((b, h, dk, v.shape[3]), dtype=torch.float32) if state is None else state.clone()
-    return o, final
+    return o, final, None
   final = torch.empty((b, h, dk, v.shape[3]), dtype=torch.float32, device=q.device)
-  _decay_launch("mjlab_decay_forward", _DECAY, _decay_pack(q, k, v, o, log_decay, scale, state, final, reset, lengths), (), q.device)
-  return o, final
+  ws = _decay_launch("mjlab_decay_forward", _DECAY, _decay_pack(q, k, v, o, log_decay, scale, state, final, reset, lengths), (), q.device)
+  return o, final, ws
 
 
 class _DecayAttention(torch.autograd.Function):
   @staticmethod
   def forward(ctx, q, k, v, state, log_decay, scale, reset, lengths):
-    ctx.save_for_backward(q, k, v, state, log_decay, reset, lengths)
+    o, final, segments = _decay_forward(q, k, v, state, log_decay, scale, reset, lengths)
+    ctx.save_for_backward(q, k, v, state, log_decay, reset, lengths, segments)
     ctx.scale = scale
     ctx.set_materialize_grads(False)
-    return _decay_forward(q, k, v, state, log_decay, scale, reset, lengths)
+    return o, final
 
   @staticmethod
   @torch.autograd.function.once_differentiable
   def backward(ctx, do, dfinal):
-    q, k, v, state, log_decay, reset, lengths = ctx.saved_tensors
+    q, k, v, state, log_decay, reset, lengths, segments = ctx.saved_tensors
     need_q, need_k, need_v, need_s = ctx.needs_input_grad[:4]
     if do is None and dfinal is None:
       return (None,) * 8
@@ -357,7 +360,7 @@ class _DecayAttention(torch.autograd.Function):
     dv = _rows_like(v, v.shape[3]) if need_v or need_s else None
     ds = torch.empty_like(state) if need_s else None
     _decay_launch("mjlab_decay_backward", _DECAY_GRAD, _decay_pack(q, k, v, None, log_decay, ctx.scale, state, None, reset, lengths),
-                  (*_strided(do), *_strided(dq), *_strided(dk_), *_strided(dv), _ptr(dfinal), _ptr(ds)), q.device)
+                  (*_strided(do), *_strided(dq), *_strided(dk_), *_strided(dv), _ptr(dfinal), _ptr(ds), _ptr(segments)), q.device)
     return dq, dk_, dv if need_v else None, ds, None, None, None, None
 
 
@@ -379,7 +382,7 @@ def decay_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay
   scale = q.shape[3] ** -0.5 if scale is None else float(scale)
   if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
     return _DecayAttention.apply(q, k, v, state, log_decay, scale, reset, lengths)
-  return _decay_forward(q, k, v, state, log_decay, scale, reset, lengths)
+  return _decay_forward(q, k, v, state, log_decay, scale, reset, lengths)[:2]
 
 
 def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_decay: torch.Tensor, state: torch.Tensor, scale: float | None = None,

@@ -283,6 +283,17 @@ def test_only_the_wanted_gradients():
   assert torch.equal(shared, ga + gb)
 
 
+def test_backward_twice():
+  from mjlab_amd import policy_ops
+
+  x = inputs(2, 1100, 2, 24, 40, torch.float32, seed=12, resets=0.01, carry=True)
+  leaves = [t.requires_grad_(True) for t in (x["q"], x["k"], x["v"], x["state"])]
+  outs = policy_ops.decay_attention(*leaves[:3], x["log_decay"], state=leaves[3], reset=x["reset"])
+  first = torch.autograd.grad(outs, leaves, [x["do"], x["dstate"]], retain_graph=True)
+  second = torch.autograd.grad(outs, leaves, [x["do"], x["dstate"]])
+  assert all(torch.equal(a, b) for a, b in zip(first, second, strict=True))
+
+
 def test_refusals_on_the_device():
   from mjlab_amd import policy_ops
 

@@ -141,8 +141,10 @@ def test_decay_backward_refuses():
   assert lib.mjlab_decay_backward(ctypes.byref(g), None) < 0 and "d_out" in lib.mjlab_policy_last_error().decode()
   g.d_out, g.d_state = policy_ops.Rows(64, 80, 16, 8), 64
   assert lib.mjlab_decay_backward(ctypes.byref(g), None) < 0 and "d_state" in lib.mjlab_policy_last_error().decode()
-  g.f.length = 100000
   g.d_state = None
+  g.segments = g.f.workspace = 64
+  assert lib.mjlab_decay_backward(ctypes.byref(g), None) < 0 and "segments" in lib.mjlab_policy_last_error().decode()
+  g.f.length = 100000
   assert lib.mjlab_decay_backward(ctypes.byref(g), None) < 0 and "workspace" in lib.mjlab_policy_last_error().decode()
 
 
