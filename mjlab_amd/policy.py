@@ -122,7 +122,7 @@ class Policy(torch.nn.Module):
     return qkv.view(*x.shape[:-1], 3, self.cfg.heads, self.cfg.head_dim).unbind(-3)
 
   def _close(self, block: torch.nn.Module, x: torch.Tensor, o: torch.Tensor) -> torch.Tensor:
-    x = policy_ops.dense(o.reshape(*x.shape[:-1], -1), block.out, residual=x)
+    x = policy_ops.dense(o.reshape(*x.shape[:-1], block.out.shape[1]), block.out, residual=x)
     return policy_ops.dense(policy_ops.gated(x, block.gate, block.up, activation=self.cfg.gated_activation), block.down, residual=x)
 
   @torch.no_grad()

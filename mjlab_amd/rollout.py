@@ -339,7 +339,8 @@ class PhysicsRollout:
       self.push = (float(lo_t), float(hi_t), rng6, time_left)
     self._graph: torch.cuda.CUDAGraph | None = None
     self._policy = None  # the policy whose control step capture_graph() recorded
-    self._memory: dict = {}  # a policy's memory of these environments (Policy.initial_state), by policy
+    self.policy_memory: torch.Tensor | None = None  # that policy's memory of these environments (Policy.initial_state())
+    self._cut: torch.Tensor | None = None  # the environments that the last control step reset; None: all of them were
     self._action_buf: torch.Tensor | None = None
     self._obs_buf: torch.Tensor | None = None
     # load balance of the control kernel (mjlab_control_t.world_order): see balance_worlds()
@@ -377,8 +378,9 @@ class PhysicsRollout:
   def reset_all(self) -> None:
     d = self.sim.data
     n = self.sim.num_envs
-    for _, memory in self._memory.values():
-      memory.zero_()
+    self._cut = None
+    if self.policy_memory is not None:
+      self.policy_memory.zero_()
     if self.motion is not None:
       torch.rand(self.motion["rnd"].shape, device=self.key_qpos.device, generator=self.gen, out=self.motion["rnd"])
       t_new = self._motion_rows()
@@ -413,17 +415,21 @@ class PhysicsRollout:
       if action is not None and action is not self._action_buf:  # random_action(out=...) / a policy may write the static buffer directly
         self._action_buf.copy_(action)
       self._graph.replay()
-      return self._reset_buf
-    return self._step_eager(action)
+      self._cut = self._reset_buf
+    else:
+      self._cut = self._step_eager(action)
+    return self._cut
 
   def capture_graph(self, policy=None) -> None:
     """Capture one control step into a hipGraph (the physics kernels are launched directly
     inside the capture, not through the Simulation's own step/forward graphs).  With a ``policy``
     (mjlab_amd.policy.Policy) the graph begins with its action: observation rows -> network -> physics, then
-    ``step()`` takes no action.  Its parameters are read at every replay, so an update in place takes effect."""
+    ``step()`` takes no action.  Its parameters are read at every replay, so an update in place takes effect; its
+    memory, empty at first, is ``policy_memory``."""
     self._graph = None
-    self._policy = policy
     n = self.sim.num_envs
+    self._policy = policy
+    self.policy_memory = None if policy is None else policy.initial_state(n)
     dev = self.key_qpos.device
     self._action_buf = torch.zeros((n, self.m.nu), device=dev)
     # with the fused reset the mask written by the library IS the result (int32, non-zero = reset): no conversion launch
@@ -447,7 +453,7 @@ class PhysicsRollout:
 
   def _capture_body(self) -> None:
     if self._policy is not None:
-      self.policy_action(self._policy, out=self._action_buf)
+      self._policy.act(self.observation_rows(), state=self.policy_memory, reset=self._reset_buf, out=self._action_buf)
     r = self._step_eager(self._action_buf)
     if r is not self._reset_buf:
       self._reset_buf.copy_(r)
@@ -528,8 +534,6 @@ class PhysicsRollout:
         self.motion["time_steps"].copy_(torch.where(reset, t_new, self.motion["time_steps"].long() + 1).to(torch.int32))
       d.qacc_warmstart[:] = torch.where(rm, torch.zeros_like(d.qacc_warmstart), torch.nan_to_num(d.qacc_warmstart))
       self.episode_length.copy_(torch.where(reset, torch.zeros_like(self.episode_length), self.episode_length))
-      if self._memory:  # a policy's memory is cut by the mask at its next step
-        self._reset_mask.copy_(reset)
     self.sim.forward(reset if self.masked_forward else None)
     if self.push is not None:  # interval events come after the reset's forward() (manager_based_rl_env.py:134-137)
       lo_t, hi_t, rng6, time_left = self.push
@@ -574,15 +578,14 @@ class PhysicsRollout:
       out = torch.empty((self.sim.num_envs, self.m.nu), device=self.key_qpos.device)
     return out.uniform_(-1.0, 1.0, generator=self.gen)
 
-  def policy_action(self, policy, out: torch.Tensor | None = None) -> torch.Tensor:
+  def policy_action(self, policy, memory: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """The action of a ``policy`` (mjlab_amd.policy.Policy) at the present observation rows; ``out=self.action_buffer`` writes the captured graph's input in
-    place.  A policy with memory carries one state per environment here, cut where the last control step reset it, emptied by reset_all()."""
-    memory = None
-    if policy.cfg.memory_blocks:
-      if id(policy) not in self._memory:
-        self._memory[id(policy)] = (policy, policy.initial_state(self.sim.num_envs))
-      memory = self._memory[id(policy)][1]
-    return policy.act(self.observation_rows(), state=memory, reset=self._reset_mask, out=out)
+    place.  ``memory``: of a policy with memory, what ``policy.initial_state(num_envs)`` returned, kept by the caller; it is updated in place, and cut where
+    the last control step, or reset_all(), reset an environment."""
+    cut = self._cut
+    if memory is not None and cut is None:
+      cut = torch.ones_like(self._reset_mask)
+    return policy.act(self.observation_rows(), state=memory, reset=cut, out=out)
 
   @property
   def action_buffer(self) -> torch.Tensor | None:

@@ -91,6 +91,16 @@ def test_control_steps_equal_the_update():
   assert (again.reshape(n * t, 1, 11) - alone).norm() <= TOL[torch.float32] * alone.norm()
 
 
+def test_no_environments_and_no_steps():
+  p = make()
+  for n, t in ((0, 3), (2, 0)):
+    actions, final = p(torch.zeros((n, t, 37), device="cuda"))
+    assert actions.shape == (n, t, 11) and final.shape == p.initial_state(n).shape and not final.any()
+    sum(x.sum() for x in (actions, final)).backward()
+  assert all(not x.grad.any() for x in p.parameters())
+  assert p.act(torch.zeros((0, 37), device="cuda"), state=p.initial_state(0)).shape == (0, 11)
+
+
 def test_from_mlp_equals_the_sequential():
   torch.manual_seed(3)
   act = torch.nn.ELU()
@@ -113,30 +123,42 @@ def _rollout(**kw):
 
 @pytest.mark.parametrize("memory_blocks", [0, 1])
 @pytest.mark.parametrize("fused_reset", [True, False])
-def test_rollout_with_a_policy_captured_equals_eager(memory_blocks, fused_reset):
-  """observation rows -> policy -> physics: the captured control step replays what separate calls compute, resets cut the memory in both."""
+@pytest.mark.parametrize("inside", [True, False])
+def test_rollout_with_a_policy_captured_equals_eager(memory_blocks, fused_reset, inside):
+  """observation rows -> policy -> physics: the captured control step, with the policy inside or before it, replays what separate calls compute; resets cut
+  the memory in both."""
   kw = dict(fused_reset=fused_reset, control_kernel=fused_reset, episode_length_s=0.2)
   a, b = _rollout(**kw), _rollout(**kw)
   p = make(memory_blocks, obs_dim=a.observation_rows().shape[1], action_dim=a.m.nu)
+  mine, other = p.initial_state(64), p.initial_state(64)
   with pytest.raises(ValueError, match="action"):
     a.step()
-  a.capture_graph(p)  # (runs one control step to warm up)
-  b.step(b.policy_action(p))
+  if inside:
+    a.capture_graph(p)  # (runs one control step to warm up)
+    b.step(b.policy_action(p, other))
+  else:
+    a.capture_graph()
+    b.step(torch.zeros((64, b.m.nu), device="cuda"))
   resets = 0
   for _ in range(25):
-    ra = a.step()
-    rb = b.step(b.policy_action(p))
+    ra = a.step(None if inside else a.policy_action(p, mine, out=a.action_buffer))
+    rb = b.step(b.policy_action(p, other))
     assert torch.equal(ra != 0, rb != 0)
     resets += int((ra != 0).sum())
     assert torch.equal(a.sim.data.qpos, b.sim.data.qpos)
     if memory_blocks:
-      ma, mb = a._memory[id(p)][1], b._memory[id(p)][1]
-      assert torch.equal(ma, mb) and ma.any()
+      memory = a.policy_memory if inside else mine
+      assert torch.equal(memory, other) and memory.any()
   assert resets > 64  # episodes of 10 steps: every environment was cut at least twice
+  if memory_blocks:  # reset_all() cuts every memory
+    b.reset_all()
+    assert torch.equal(b.policy_action(p, other), p.act(b.observation_rows(), p.initial_state(64)))
+  if not inside:
+    return
   with pytest.raises(ValueError, match="action"):
     a.step(torch.zeros((64, a.m.nu), device="cuda"))
   a.reset_all()
-  assert not memory_blocks or not a._memory[id(p)][1].any()
+  assert not memory_blocks or not a.policy_memory.any()
   # parameters are read at every replay
   with torch.no_grad():
     p.head_weight.zero_()
