@@ -70,7 +70,7 @@ int mjlab_sizeof_layer_grad(void);
  *   S_t = decay keep_t S_{t-1} + k_t v_t^T      (dk x dv, 32 bits)          o_t = scale * q_t S_t
  * reset[t] means that token t is the first of an episode.  q, k (batch, length, heads, dk), v, o (batch, length, heads, dv) of `dtype`, any strides
  * but 1 for the innermost; dk, dv <= MJLAB_DECAY_MAX_DIM.  state (the S before token 0; NULL = 0) and state_out (S after the last token; NULL =
- * not wanted) are dense (batch, heads, dk, dv) floats and may be the same memory.  reset (batch, length) of reset_bytes 1 or 4 per element, non-zero =
+ * not wanted) are dense (batch, heads, dk, dv) floats and not the same memory.  reset (batch, length) of reset_bytes 1 or 4 per element, non-zero =
  * reset, or NULL.  lengths (batch) ints or NULL: sequence b ends before token lengths[b] (clamped to [0, length]); the rows of o behind it are
  * written as zeros.  A NaN or infinity reaches only the tokens that the recurrence takes it to: not earlier ones, not other episodes.
  * workspace: mjlab_decay_workspace() bytes of device memory. */

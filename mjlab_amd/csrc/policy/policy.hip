@@ -20,8 +20,9 @@ static bool bad_type(int dtype) { return dtype < MJLAB_DTYPE_F32 || dtype > MJLA
 static int check_layer(const mjlab_layer_t& f) {
   if (bad_type(f.dtype)) return fail(-2, "layer: unknown dtype");
   if (f.act < 0 || f.act >= MJLAB_ACT_COUNT) return fail(-2, "layer: unknown activation");
-  // in, out < 2^31 and rows < 2^37 keep every product of two sizes and an element size inside 64 bits with room to spare
-  if (f.rows < 1 || f.in < 1 || f.out < 1 || f.in >= (1LL << 30) || f.out >= (1LL << 30) || f.rows >= (1LL << 31)) return fail(-2, "layer: sizes must be positive (in, out below 2^30, rows below 2^31)");
+  if (f.rows < 1 || f.in < 1 || f.out < 1 || f.in >= (1LL << 30) || f.out >= (1LL << 27) || f.rows >= (1LL << 31)) return fail(-2, "layer: sizes must be positive (in below 2^30, out below 2^27, rows below 2^31)");
+  // 2^44 elements are more than any memory holds: the sizes of workspaces (up to 512 times a matrix of floats) stay inside 64 bits
+  if (f.rows * f.in >= (1LL << 44) || f.rows * f.out >= (1LL << 44) || f.in * f.out >= (1LL << 44)) return fail(-2, "layer: the product of two sizes must be below 2^44");
   if (!f.x || !f.w) return fail(-2, "layer: null x or w");
   if ((f.rows > 1 && f.ldx < 0) || (f.out > 1 && f.ldw < 0) || (f.w_up && f.out > 1 && f.ldw_up < 0)) return fail(-2, "layer: negative row stride");
   return 0;

@@ -82,6 +82,10 @@ def _call(fn: str, packed: bytes, dev: torch.device) -> None:
     native.policy_check(rc, fn)
 
 
+# A tensor of the caller's that a kernel wrote: autograd is to notice where an earlier operation kept it for its backward pass.
+_written = torch.autograd.graph.increment_version
+
+
 def _ptr(t: torch.Tensor | None) -> int:
   return 0 if t is None else t.data_ptr()
 
@@ -203,6 +207,7 @@ def _run(x, w, w_up, b, b_up, r, act, lead: tuple, out):
       raise ValueError("out= takes no part in a graph of gradients: call it under torch.no_grad()")
     out2 = out.view(-1, out.shape[-1])
     _forward(x2, w, w_up, b, b_up, r, act, keep=False, y=out2)
+    _written(out)
     return out
   y = _Layer.apply(x2, w, w_up, b, b_up, r, act) if grad else _forward(x2, w, w_up, b, b_up, r, act, keep=False)[0]
   return y if x.dim() == 2 else y.view(*lead, w.shape[0])
@@ -406,7 +411,8 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
       raise ValueError("decay_attention_step: out_state overlaps state")
   if any(_overlap(out_state, t) for t in (q, k, v)):
     raise ValueError("decay_attention_step: the state overlaps an input")
-  if out is None:
+  own = out is None
+  if own:
     out = q.new_empty((b, h, dv))
   else:
     _check_out("decay_attention_step", out, q, (b, h, dv), (k, v, state, out_state))
@@ -415,4 +421,7 @@ def decay_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log_
     rows = [x for t in (q, k, v, out) for x in (t.data_ptr(), t.stride(0), 0, t.stride(1))]
     _call("mjlab_decay_step", _DECAY.pack(DTYPES[q.dtype], r[0], b, 1, h, dk, dv, dk**-0.5 if scale is None else scale, *rows, log_decay.data_ptr(), state.data_ptr(),
                                           out_state.data_ptr(), r[1], r[2], 0, 0, 0, 0), q.device)  # fmt: skip
+    _written(out_state)
+    if not own:
+      _written(out)
   return out, out_state

@@ -285,3 +285,14 @@ def test_refusals_on_the_device():
   for kind, call in bad:
     with pytest.raises(kind):
       call()
+
+
+def test_an_output_over_a_kept_input_is_noticed():
+  from mjlab_amd import policy_ops
+
+  x, w = torch.randn((6, 8), device="cuda"), torch.randn((8, 8), device="cuda", requires_grad=True)
+  y = policy_ops.dense(x, w)
+  with torch.no_grad():
+    policy_ops.dense(torch.ones_like(x), w, out=x)
+  with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+    y.sum().backward()

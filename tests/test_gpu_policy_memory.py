@@ -294,6 +294,19 @@ def test_backward_twice():
   assert all(torch.equal(a, b) for a, b in zip(first, second, strict=True))
 
 
+def test_a_state_kept_for_a_backward_pass_and_then_stepped_is_noticed():
+  from mjlab_amd import policy_ops
+
+  x = inputs(3, 5, 2, 16, 16, torch.float32, seed=13, carry=True)
+  q = x["q"].requires_grad_(True)
+  state = x["state"].clone()
+  o, _ = policy_ops.decay_attention(q, x["k"], x["v"], x["log_decay"], state=state)
+  with torch.no_grad():
+    policy_ops.decay_attention_step(q[:, 0], x["k"][:, 0], x["v"][:, 0], x["log_decay"], state)
+  with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+    o.sum().backward()
+
+
 def test_refusals_on_the_device():
   from mjlab_amd import policy_ops
 

@@ -39,7 +39,7 @@ def _layer(**kw):
 
 @pytest.mark.parametrize("kw,text", [
   (dict(dtype=3), "dtype"), (dict(act=7), "activation"), (dict(act=-1), "activation"), (dict(rows=0), "sizes"), (dict(inp=0), "sizes"), (dict(out=-1), "sizes"),
-  (dict(inp=1 << 30), "sizes"), (dict(x=None), "null x or w"), (dict(w=None), "null x or w"), (dict(y=None), "null y"), (dict(ldx=-8), "negative"),
+  (dict(inp=1 << 30), "sizes"), (dict(out=1 << 27), "sizes"), (dict(rows=1 << 30, out=1 << 20), "2^44"), (dict(x=None), "null x or w"), (dict(w=None), "null x or w"), (dict(y=None), "null y"), (dict(ldx=-8), "negative"),
   (dict(ldy=2), "overlap"), (dict(w_up=64, ldw_up=8, r=64), "residual"), (dict(b_up=64), "b_up"), (dict(z_up=64), "z_up"),
   (dict(rows=4, inp=2048, out=2048, ldy=2048), "workspace"),
 ])  # fmt: skip
