@@ -29,23 +29,34 @@ struct DecayPass {
   float *seg_state, *seg_factor;  // (seg_given: seg_state is read only) (sequences * heads, segments - 1, da, dc), (sequences * heads, segments - 1)
 };
 
-// What the matrix cores read: bf16 as it is; float, and fp16 turned into float (whose products and sums of keys and values may leave fp16's range).
+// What the matrix cores read.  float as it is.  bf16 as it is; what is formed on the way (weighted rows, pairs, R) is rounded to it, like the outputs.  fp16: a b^T
+// as it is, but sums of keys and values may leave fp16's range, so all else is multiplied as sums of bf16, each the nearest to what is left: two hold
+// an fp16 number and 16 bits of R and of a pair (outputs are rounded to 11), three a weighted row (which R, a float output in the end, is made of).
 template <typename T> struct DecayCfg {
   using L = float;
-  static constexpr int C = 32, KS = 4, PAD = 4;  // tokens per chunk, k per matrix instruction, padding of LDS rows
+  static constexpr int KS = 4, PAD = 4, A = 1, W = 1, N = 1;  // k per matrix instruction, padding of LDS rows, planes of a, of weighted b, of c, P and R
 };
 template <> struct DecayCfg<__bf16> {
   using L = __bf16;
-  static constexpr int C = 64, KS = 32, PAD = 8;
+  static constexpr int KS = 32, PAD = 8, A = 1, W = 1, N = 1;
 };
+template <> struct DecayCfg<_Float16> {
+  using L = __bf16;
+  static constexpr int KS = 32, PAD = 8, A = 2, W = 3, N = 2;
+};
+// tokens per chunk
+template <typename T> constexpr int decay_chunk(bool both_large) { return sizeof(T) == 4 || (DecayCfg<T>::N > 1 && both_large) ? 32 : 64; }
 
 __device__ __forceinline__ f32x4 mma16(s16x8 a, s16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
 }
+__device__ __forceinline__ f32x4 mma16h(s16x8 a, s16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
+}
 __device__ __forceinline__ f32x4 mma16(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 // fragments of 16 rows (or columns) x KS of k: k contiguous / k the row index of the tile
-__device__ __forceinline__ s16x8 frag_kc(const __bf16* s, int ld, int r0, int k0, int lane) { return *(const s16x8*)(s + (r0 + (lane & 15)) * ld + k0 + (lane >> 4) * 8); }
+template <typename L> __device__ __forceinline__ s16x8 frag_kc(const L* s, int ld, int r0, int k0, int lane) { return *(const s16x8*)(s + (r0 + (lane & 15)) * ld + k0 + (lane >> 4) * 8); }
 __device__ __forceinline__ float frag_kc(const float* s, int ld, int r0, int k0, int lane) { return s[(r0 + (lane & 15)) * ld + k0 + (lane >> 4)]; }
 __device__ __forceinline__ s16x8 frag_kr(const __bf16* s, int ld, int r0, int k0, int lane) {
   typedef __attribute__((address_space(3))) s16x4 lds_s4;
@@ -65,38 +76,53 @@ __device__ __forceinline__ bool reset_at(const DecayPass& p, long long seq, long
 }
 
 template <typename T, int DA, int DC, bool STATE> struct DecayLds {
-  using L = typename DecayCfg<T>::L;
-  static constexpr int C = DecayCfg<T>::C, PAD = DecayCfg<T>::PAD, LA = DA + PAD, LC = DC + PAD, LP = C + PAD;
-  L b[STATE ? 8 : C * LA], bw[C * LA], c[C * LC], p[STATE ? 8 : C * LP], r[STATE ? 8 : DC * LA];  // bw: b times its tokens' weights into R
+  using Cfg = DecayCfg<T>;
+  using L = typename Cfg::L;
+  static constexpr int C = decay_chunk<T>(DA > 64 && DC > 64), PAD = Cfg::PAD, LA = DA + PAD, LC = DC + PAD, LP = C + PAD;
+  static constexpr int SW = C * LA, SC = C * LC, SP = STATE ? 8 : C * LP, SR = STATE ? 8 : DC * LA;  // a plane of each
+  T b[STATE ? 8 : C * LA];
+  L bw[Cfg::W * SW], c[Cfg::N * SC], p[Cfg::N * SP], r[Cfg::N * SR];  // bw: b times its tokens' weights into R
   float enter[C];                 // of R into token i
   int episode[C], odd[8];         // the episode a token belongs to, counted in the chunk
 };
 
-// VEC elements of T as elements of L, to an address aligned for them
-template <typename T, typename L> __device__ __forceinline__ void put_chunk(L* at, const Chunk<T>& x) {
-  if constexpr (sizeof(T) == sizeof(L)) *(Chunk<T>*)at = x;
-  else {
-    f32x4 lo, hi;
+// N planes of four numbers, `plane` elements apart; and the number that they hold
+template <int N> __device__ __forceinline__ void put4(__bf16* at, int plane, f32x4 x) {
+  typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) { lo[e] = (float)x.e[e]; hi[e] = (float)x.e[4 + e]; }
-    *(f32x4*)at = lo;
-    *(f32x4*)(at + 4) = hi;
+  for (int i = 0; i < N; ++i) {
+    const b16x4 h = __builtin_convertvector(x, b16x4);
+    *(b16x4*)(at + i * plane) = h;
+    if (i + 1 < N) x -= __builtin_convertvector(h, f32x4);
   }
 }
-__device__ __forceinline__ void put4(__bf16* at, const f32x4& x) {
-  typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
-  *(b16x4*)at = __builtin_convertvector(x, b16x4);
+template <int N> __device__ __forceinline__ void put4(float* at, int, const f32x4& x) { *(f32x4*)at = x; }
+template <int N, typename L> __device__ __forceinline__ float get(const L* at, int plane) {
+  float x = (float)*at;
+  if (N > 1 && !not_finite(x)) {  // (nothing can be left of an infinity)
+#pragma unroll
+    for (int i = 1; i < N; ++i) x += (float)at[i * plane];
+  }
+  return x;
 }
-__device__ __forceinline__ void put4(float* at, const f32x4& x) { *(f32x4*)at = x; }
+// a b over planes: the terms that count
+template <int NA, int NB, typename F> __device__ __forceinline__ f32x4 mma_planes(const F* a, const F* b, f32x4 x) {
+#pragma unroll
+  for (int i = NA - 1; i >= 0; --i)
+#pragma unroll
+    for (int j = NB - 1; j >= 0; --j)
+      if (i + j < (NA > NB ? NA : NB)) x = mma16(a[i], b[j], x);
+  return x;
+}
 
-// x times w (w 0: zeros, whatever x holds), as elements of L
-template <typename T, typename L> __device__ __forceinline__ void put_weighted(L* at, const Chunk<T>& x, float w) {
+// VEC elements of T times w (w 0: zeros, whatever x holds), as N planes of L
+template <int N, typename T, typename L> __device__ __forceinline__ void put_weighted(L* at, int plane, const Chunk<T>& x, float w) {
 #pragma unroll
   for (int h = 0; h < Elem<T>::VEC; h += 4) {
     f32x4 y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = w * (float)x.e[h + e];
-    put4(at + h, w == 0.f ? f32x4{} : y);
+    put4<N>(at + h, plane, w == 0.f ? f32x4{} : y);
   }
 }
 
@@ -117,23 +143,27 @@ template <typename T> __device__ __forceinline__ bool seen_odd(unsigned most) {
   return (most >> 16) >= INF || (most & 0xffffu) >= INF;
 }
 
-// Elements col .. col + VEC - 1 of a row of d, zero from d on.  FULL: all of them are there.
-template <typename T, bool FULL> __device__ __forceinline__ Chunk<T> load_row(const T* at, int col, int d) {
-  if constexpr (FULL) return load_chunk(at);
+// How the heads fit the tiles of DA and DC columns: they fill them; they end between two chunks of 16 bytes; or anywhere.
+enum { FIT_ANY = 0, FIT_CHUNKS = 1, FIT_FULL = 2 };
+// Elements col .. col + VEC - 1 of a row of d, zero from d on.
+template <typename T, int FIT> __device__ __forceinline__ Chunk<T> load_row(const T* at, int col, int d) {
+  if constexpr (FIT == FIT_FULL) return load_chunk(at);
+  else if constexpr (FIT == FIT_CHUNKS) return col < d ? load_chunk(at) : Chunk<T>{};
   else return load_part(at, d - col);
 }
 
 constexpr int decay_threads(int da, int dc) { return da >= 64 && dc >= 64 ? 512 : 256; }
 
-// 256 or 512 threads per (sequence, head, segment).  FULL: da = DA and dc = DC.  STATE: the first pass of a split sequence, the segment's contribution to R alone.
+// 256 or 512 threads per (sequence, head, segment).  STATE: the first pass of a split sequence, the segment's contribution to R alone.
 // Products are formed such that an accumulator's four rows are neighbours in memory: P^T and out^T (columns are tokens), R (rows are da).
 // The rows of a go from memory to the matrix cores' registers without LDS: with them in LDS a 128 x 128 workgroup took 114 KB, and one of them per CU
 // could not hide its loads (2 x 8192 tokens x 8 heads of 128, bf16: 130 us for this kernel then).
-template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch_bounds__(decay_threads(DA, DC), 2) void k_decay_chunks(const DecayPass p) {
+template <typename T, int DA, int DC, int FIT, bool STATE> __global__ __launch_bounds__(decay_threads(DA, DC), 2) void k_decay_chunks(const DecayPass p) {
   using Cfg = DecayCfg<T>;
   using L = typename Cfg::L;
   using S = DecayLds<T, DA, DC, STATE>;
-  constexpr int C = Cfg::C, KS = Cfg::KS, LA = S::LA, LC = S::LC, LP = S::LP, V = Elem<T>::VEC, CT = C / 16, KA = DA / KS;
+  constexpr bool FULL = FIT == FIT_FULL, FENCE = DA * DC > 64 * 64;
+  constexpr int C = S::C, KS = Cfg::KS, NA = Cfg::A, PW = Cfg::W, NN = Cfg::N, LA = S::LA, LC = S::LC, LP = S::LP, V = Elem<T>::VEC, CT = C / 16, KA = DA / KS;
   constexpr int NT = decay_threads(DA, DC), NW = NT / 64, NB = (C * DA / V + NT - 1) / NT, NC = (C * DC / V + NT - 1) / NT;  // 16-byte chunks per thread
   // Waves: of out, OR x OC waves of TR x TC tiles (tokens x dc); of R, RW x NW / RW waves of RR x RC tiles (da x dc)
   constexpr int OC = CT == 4 ? 2 : (DC / 16 < NW ? DC / 16 : NW);
@@ -173,23 +203,23 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const int row = (tid + i * NT) / (DA / V), col = (tid + i * NT) % (DA / V) * V;
-      if ((all && C * DA / V % NT == 0) || (row < C && q0 + row < len)) xb[i] = load_row<T, FULL>(pb[i], col, p.da);
+      if ((all && C * DA / V % NT == 0) || (row < C && q0 + row < len)) xb[i] = load_row<T, FIT>(pb[i], col, p.da);
       else xb[i] = Chunk<T>{};
       pb[i] += step * p.b_t;
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int row = (tid + i * NT) / (DC / V), col = (tid + i * NT) % (DC / V) * V;
-      if ((all && C * DC / V % NT == 0) || (row < C && q0 + row < len)) xc[i] = load_row<T, FULL>(pc[i], col, p.dc);
+      if ((all && C * DC / V % NT == 0) || (row < C && q0 + row < len)) xc[i] = load_row<T, FIT>(pc[i], col, p.dc);
       else xc[i] = Chunk<T>{};
       pc[i] += step * p.c_t;
     }
   };
   // The rows of a of this wave's tokens.  16 bits: fragments as they are.  float: four k-steps come as 16 bytes, lane group by lane group, so the k order of
-  // the fragments is that of a_k(), not 4 step + (lane >> 4): the other operand of a product with `a` is read in the same order.
-  constexpr bool F32 = sizeof(L) == 4;
+  // the fragments is i * 16 + row4 + e, not 4 step + (lane >> 4): the other operand of a product with `a` is read in the same order.
+  constexpr bool F32 = sizeof(T) == 4;
   typename std::conditional<F32, f32x4, s16x8>::type fa[TR][F32 ? DA / 16 : KA];
-  auto a_k = [&](int i) { return sizeof(T) == 4 ? i * 16 + row4 : i / 2 * 32 + 2 * row4 + (i & 1) * 4; };  // first k of this lane in fa[.][i]
+  s16x8 fs[NN > 1 ? KA : 1][NA];  // (fp16) the planes of one tile's
   const T* pa[TR];
   T* po[TR];
 #pragma unroll
@@ -208,34 +238,43 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
 #pragma unroll
         for (int k = 0; k < KA; ++k) {
           const int col = k * KS + (lane >> 4) * 8;
-          fa[t][k] = live ? __builtin_bit_cast(s16x8, load_row<T, FULL>(row + col, col, p.da)) : s16x8{};
+          fa[t][k] = live ? __builtin_bit_cast(s16x8, load_row<T, FIT>(row + col, col, p.da)) : s16x8{};
         }
-      } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < DA / 16; ++i) fa[t][i] = live ? __builtin_bit_cast(f32x4, load_row<T, FULL>(row + i * 16 + row4, i * 16 + row4, p.da)) : f32x4{};
       } else {
 #pragma unroll
-        for (int i = 0; i < DA / 32; ++i) {
-          const int col = i * 32 + 2 * row4;
-          const Chunk<T> c = live ? load_row<T, FULL>(row + col, col, p.da) : Chunk<T>{};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { fa[t][2 * i][e] = (float)c.e[e]; fa[t][2 * i + 1][e] = (float)c.e[4 + e]; }
-        }
+        for (int i = 0; i < DA / 16; ++i) fa[t][i] = live ? __builtin_bit_cast(f32x4, load_row<T, FIT>(row + i * 16 + row4, i * 16 + row4, p.da)) : f32x4{};
       }
     }
   };
-  // x += (rows r0 .. of s, k contiguous) (a's rows of token tile t)^T over all of da
-  auto with_a = [&](const L* rows, int row0, int t, f32x4 x) {
-    if constexpr (!F32) {
-#pragma unroll
-      for (int k = 0; k < KA; ++k) x = mma16(frag_kc(rows, LA, row0, k * KS, lane), fa[t][k], x);
-    } else {
+  // (rows row0 .. of b or R, k contiguous) (a's rows of token tile t)^T over all of da.  R, fp16: of whole numbers where something is not finite, since a plane of
+  // zeros times infinity would be NaN.
+  auto with_a = [&](auto of_r, const auto* rows, int row0, int t, bool whole) {
+    f32x4 x = {};
+    if constexpr (F32) {
 #pragma unroll
       for (int i = 0; i < DA / 16; ++i) {
-        const f32x4 o = *(const f32x4*)(rows + (row0 + colx) * LA + a_k(i));
+        const f32x4 o = *(const f32x4*)(rows + (row0 + colx) * LA + i * 16 + row4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x = mma16(o[e], fa[t][i][e], x);
       }
+    } else if constexpr (NN == 1) {
+#pragma unroll
+      for (int k = 0; k < KA; ++k) x = mma16(frag_kc(rows, LA, row0, k * KS, lane), fa[t][k], x);
+    } else if constexpr (!decltype(of_r)::value) {
+#pragma unroll
+      for (int k = 0; k < KA; ++k) x = mma16h(frag_kc(rows, LA, row0, k * KS, lane), fa[t][k], x);
+    } else if (!whole) {
+#pragma unroll
+      for (int k = 0; k < KA; ++k) {
+        s16x8 o[NN];
+#pragma unroll
+        for (int i = 0; i < NN; ++i) o[i] = frag_kc(rows + i * S::SR, LA, row0, k * KS, lane);
+        x = mma_planes<NN, NA>(o, fs[k], x);
+      }
+    } else {
+      for (int k = 0; k < KA; ++k)
+        for (int e = 0; e < 8; ++e)
+          x = mma16(get<NN>(rows + (row0 + colx) * LA + k * KS + 2 * row4 + e, S::SR), (float)__builtin_bit_cast(h16x8, fa[t][k])[e], x);
     }
     return x;
   };
@@ -277,20 +316,23 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
 
     __syncthreads();  // the chunk before is done with LDS
     unsigned most = 0;
+    float odd = 0.f;  // NaN: R is not finite
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const int row = (tid + i * NT) / (DA / V), col = (tid + i * NT) % (DA / V) * V;
       if (row >= C) continue;
       const float w = row < n && !cut_out && (whole || episode(row) == e_last) ? p.us * power(n - p.e0 - row) : 0.f;
-      put_weighted(s.bw + row * LA + col, xb[i], w);
-      if constexpr (!STATE) put_chunk(s.b + row * LA + col, xb[i]);
+      put_weighted<PW>(s.bw + row * LA + col, S::SW, xb[i], w);
+      if constexpr (!STATE) *(Chunk<T>*)(s.b + row * LA + col) = xb[i];
+      if constexpr (NN > 1) see(most, xb[i]);
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int row = (tid + i * NT) / (DC / V), col = (tid + i * NT) % (DC / V) * V;
       if (row >= C) continue;
       see(most, xc[i]);
-      put_chunk(s.c + row * LC + col, xc[i]);
+      if constexpr (NN == 1) *(Chunk<T>*)(s.c + row * LC + col) = xc[i];
+      else put_weighted<NN>(s.c + row * LC + col, S::SC, xc[i], 1.f);
     }
     if (!STATE && tid < C) {
       s.enter[tid] = tid < n && episode(tid) == 0 ? p.is * power(tid + p.e0) : 0.f;
@@ -301,10 +343,20 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
 #pragma unroll
       for (int i = 0; i < RR; ++i)
 #pragma unroll
-        for (int j = 0; j < RC; ++j) put4(s.r + ((rc0 + j) * 16 + colx) * LA + (r0 + i) * 16 + row4, acc[i][j]);
+        for (int j = 0; j < RC; ++j) {
+          put4<NN>(s.r + ((rc0 + j) * 16 + colx) * LA + (r0 + i) * 16 + row4, S::SR, acc[i][j]);
+          if constexpr (NN > 1)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) odd = __builtin_fmaf(acc[i][j][e], 0.f, odd);
+        }
     }
-    // A zero weight times infinity would be NaN: a chunk whose c holds one goes term by term.
-    const bool mine = __ballot(seen_odd<T>(most)) != 0;
+    if constexpr (!STATE && NN > 1)
+#pragma unroll
+      for (int t = 0; t < TR; ++t)
+#pragma unroll
+        for (int k = 0; k < KA; ++k) see(most, __builtin_bit_cast(Chunk<T>, fa[t][k]));
+    // A zero weight times infinity would be NaN: a chunk whose c holds one goes term by term.  (fp16: any operand, since a plane may be zero.)
+    const bool mine = __ballot(seen_odd<T>(most) || odd != odd) != 0;
     if (lane == 0) s.odd[wave] = mine;
     __syncthreads();
     int any = 0;
@@ -319,13 +371,27 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
 #pragma unroll
       for (int t = 0; t < TR; ++t) {
         const int i = (t0 + t) * 16 + colx, ei = s.episode[i];
+        if constexpr (NN > 1) {  // a's rows as planes
+#pragma unroll
+          for (int k = 0; k < KA; ++k) {
+            const h16x8 v = __builtin_bit_cast(h16x8, fa[t][k]);
+            typedef float f32x8 __attribute__((ext_vector_type(8)));
+            f32x8 left = __builtin_convertvector(v, f32x8);
+#pragma unroll
+            for (int q = 0; q < NA; ++q) {
+              const b16x8 h = __builtin_convertvector(left, b16x8);
+              fs[k][q] = __builtin_bit_cast(s16x8, h);
+              left -= __builtin_convertvector(h, f32x8);
+            }
+          }
+        }
 #pragma unroll
         for (int jj = 0; jj < CT / OC + (CT % OC ? 1 : 0); ++jj) {
           const int tj = jj * OC + wave % OC, j = tj * 16 + row4;
           if (tj >= CT) continue;
           f32x4 y = {};
           if (tj <= t0 + t) {
-            y = with_a(s.b, tj * 16, t, y);
+            y = with_a(std::false_type(), s.b, tj * 16, t, false);
             float w[4];
             if (tj == t0 + t) {
 #pragma unroll
@@ -338,18 +404,18 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = (tj < t0 + t || j + e <= i) && i < n && (whole || s.episode[j + e] == ei) ? w[e] * y[e] : 0.f;
           }
-          put4(s.p + i * LP + tj * 16 + row4, y);
-          __builtin_amdgcn_sched_barrier(0);
+          put4<NN>(s.p + i * LP + tj * 16 + row4, S::SP, y);
+          if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int c = 0; c < TC; ++c) {
           x[t][c] = f32x4{};
           if (!carry) continue;
-          x[t][c] = with_a(s.r, (c0 + c) * 16, t, x[t][c]);
+          x[t][c] = with_a(std::true_type(), s.r, (c0 + c) * 16, t, by_term);
           const float f = s.enter[i];
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[t][c][e] = f == 0.f ? 0.f : f * x[t][c][e];
-          __builtin_amdgcn_sched_barrier(0);  // (or the fragments of every column are loaded at once, and registers spill)
+          if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);  // (or the fragments of every column are loaded at once, and registers spill)
         }
       }
       if (q0 + C < last) load_a(q0 + C);
@@ -358,10 +424,16 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
 #pragma unroll
         for (int t = 0; t < TR; ++t)
           for (int k = 0; k < (t0 + t + 1) * 16; k += KS) {
-            const auto fp = frag_kc(s.p, LP, (t0 + t) * 16, k, lane);
+            decltype(frag_kr(s.c, LC, 0, 0, lane)) fp[NN], fc[NN];
 #pragma unroll
-            for (int c = 0; c < TC; ++c) x[t][c] = mma16(frag_kr(s.c, LC, (c0 + c) * 16, k, lane), fp, x[t][c]);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int q = 0; q < NN; ++q) fp[q] = frag_kc(s.p + q * S::SP, LP, (t0 + t) * 16, k, lane);
+#pragma unroll
+            for (int c = 0; c < TC; ++c) {
+#pragma unroll
+              for (int q = 0; q < NN; ++q) fc[q] = frag_kr(s.c + q * S::SC, LC, (c0 + c) * 16, k, lane);
+              x[t][c] = mma_planes<NN, NN>(fc, fp, x[t][c]);
+            }
+            if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
           }
       } else {
 #pragma unroll
@@ -369,11 +441,11 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
           const int i = (t0 + t) * 16 + colx, ei = s.episode[i];
           for (int j = 0; j <= i && i < n; ++j)
             if (s.episode[j] == ei) {
-              const float w = (float)s.p[i * LP + j];
+              const float w = get<NN>(s.p + i * LP + j, S::SP);
 #pragma unroll
               for (int c = 0; c < TC; ++c)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[t][c][e] += w * (float)s.c[j * LC + (c0 + c) * 16 + row4 + e];
+                for (int e = 0; e < 4; ++e) x[t][c][e] += w * get<NN>(s.c + j * LC + (c0 + c) * 16 + row4 + e, S::SC);
             }
         }
       }
@@ -391,7 +463,7 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] = (T)x[t][c][e];
           if (FULL || d + row4 + 4 <= p.dc) __builtin_memcpy(at + d, o, sizeof(o));
-          else {
+          else if (FIT == FIT_ANY) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (d + row4 + e < p.dc) at[d + e] = o[e];
@@ -419,16 +491,19 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
     if (!by_term) {
 #pragma unroll 2
       for (int k = 0; k < C; k += KS) {
-        decltype(frag_kr(s.bw, LA, 0, 0, lane)) fb[RR];
+        decltype(frag_kr(s.bw, LA, 0, 0, lane)) fb[RR][PW], fc[NN];
 #pragma unroll
-        for (int i = 0; i < RR; ++i) fb[i] = frag_kr(s.bw, LA, (r0 + i) * 16, k, lane);
+        for (int i = 0; i < RR; ++i)
+#pragma unroll
+          for (int q = 0; q < PW; ++q) fb[i][q] = frag_kr(s.bw + q * S::SW, LA, (r0 + i) * 16, k, lane);
 #pragma unroll
         for (int j = 0; j < RC; ++j) {
-          const auto fc = frag_kr(s.c, LC, (rc0 + j) * 16, k, lane);
 #pragma unroll
-          for (int i = 0; i < RR; ++i) acc[i][j] = mma16(fb[i], fc, acc[i][j]);
+          for (int q = 0; q < NN; ++q) fc[q] = frag_kr(s.c + q * S::SC, LC, (rc0 + j) * 16, k, lane);
+#pragma unroll
+          for (int i = 0; i < RR; ++i) acc[i][j] = mma_planes<PW, NN>(fb[i], fc, acc[i][j]);
         }
-        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
       }
     } else {
       for (int t = 0; t < n; ++t) {
@@ -440,7 +515,7 @@ template <typename T, int DA, int DC, bool FULL, bool STATE> __global__ __launch
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = (r0 + i) * 16 + row4 + e;
-              if (FULL || r < p.da) acc[i][j][e] += (float)s.bw[t * LA + r] * (float)s.c[t * LC + (rc0 + j) * 16 + colx];
+              if (FULL || r < p.da) acc[i][j][e] += get<PW>(s.bw + t * LA + r, S::SW) * get<NN>(s.c + t * LC + (rc0 + j) * 16 + colx, S::SC);
             }
       }
     }

@@ -51,7 +51,7 @@ template <typename T, int DK, int DV, bool FULL, bool BACK> __global__ __launch_
     for (int i = 0; i < (int)(sizeof(c) / sizeof(c[0])); ++i) {
       const int u = tid + i * NT, row = u / per, col = u % per * V;
       c[i] = Chunk<T>{};
-      if (row < n) c[i] = load_row<T, FULL>(base + row * r.time + col, col, real);
+      if (row < n) c[i] = load_row<T, FULL ? FIT_FULL : FIT_ANY>(base + row * r.time + col, col, real);
     }
   };
   Chunk<T> cq[NK], ck[NK], cv[NV], cg[BACK ? NV : 1];
