@@ -155,14 +155,18 @@ template <typename T, int FIT> __device__ __forceinline__ Chunk<T> load_row(cons
 constexpr int decay_threads(int da, int dc) { return da >= 64 && dc >= 64 ? 512 : 256; }
 
 // 256 or 512 threads per (sequence, head, segment).  STATE: the first pass of a split sequence, the segment's contribution to R alone.
-// Products are formed such that an accumulator's four rows are neighbours in memory: P^T and out^T (columns are tokens), R (rows are da).
-// The rows of a go from memory to the matrix cores' registers without LDS: with them in LDS a 128 x 128 workgroup took 114 KB, and one of them per CU
-// could not hide its loads (2 x 8192 tokens x 8 heads of 128, bf16: 130 us for this kernel then).
+// Products are formed such that an accumulator's four rows are neighbours in memory: P^T and out^T (columns are tokens), R (rows are da).  The rows of a go
+// from memory to the matrix cores' registers without LDS, which holds one workgroup of 128 x 128 heads per CU (bf16 96 KB).
+// 256 sequences of 1024 tokens, forward: bf16 128 x 128 75 us (3.6 TB/s), 64 x 64 47 us, 32 x 32 45 us; fp16 64 x 64 63 us, 128 x 128 235 us; float 64 x 64
+// 128 us, 128 x 128 300 us.  Large bf16 heads are near the memory's rate; the others are bound by the chain of a chunk (stage, pairs, R, with a barrier
+// and LDS reads between): 2.5 us for a chunk of 64 at 32 x 32, 2.3 with every row in L2.  More workgroups per CU, where there are more sequences, hide it.
 template <typename T, int DA, int DC, int FIT, bool STATE> __global__ __launch_bounds__(decay_threads(DA, DC), 2) void k_decay_chunks(const DecayPass p) {
   using Cfg = DecayCfg<T>;
   using L = typename Cfg::L;
   using S = DecayLds<T, DA, DC, STATE>;
-  constexpr bool FULL = FIT == FIT_FULL, FENCE = DA * DC > 64 * 64;
+  constexpr bool FULL = FIT == FIT_FULL;
+  // The scheduler is kept from loading the fragments of every column at once: small heads have the registers for it (float 64 x 64 128 us without, 135 with)
+  constexpr bool FENCE = DA * DC > 64 * 64;
   constexpr int C = S::C, KS = Cfg::KS, NA = Cfg::A, PW = Cfg::W, NN = Cfg::N, LA = S::LA, LC = S::LC, LP = S::LP, V = Elem<T>::VEC, CT = C / 16, KA = DA / KS;
   constexpr int NT = decay_threads(DA, DC), NW = NT / 64, NB = (C * DA / V + NT - 1) / NT, NC = (C * DC / V + NT - 1) / NT;  // 16-byte chunks per thread
   // Waves: of out, OR x OC waves of TR x TC tiles (tokens x dc); of R, RW x NW / RW waves of RR x RC tiles (da x dc)
@@ -415,7 +419,7 @@ template <typename T, int DA, int DC, int FIT, bool STATE> __global__ __launch_b
           const float f = s.enter[i];
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[t][c][e] = f == 0.f ? 0.f : f * x[t][c][e];
-          if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);  // (or the fragments of every column are loaded at once, and registers spill)
+          if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
         }
       }
       if (q0 + C < last) load_a(q0 + C);

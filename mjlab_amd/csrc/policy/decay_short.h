@@ -28,8 +28,9 @@ struct ShortArgs {
   float* d_state;
 };
 
-template <typename T, int DK, int DV, bool FULL, bool BACK> __global__ __launch_bounds__(short_threads(DK, DV)) void k_decay_short(const ShortArgs p) {
+template <typename T, int DK, int DV, int FIT, bool BACK> __global__ __launch_bounds__(short_threads(DK, DV)) void k_decay_short(const ShortArgs p) {
   using S = ShortLds<DK, DV, BACK>;
+  constexpr bool FULL = FIT == FIT_FULL;
   constexpr int NT = short_threads(DK, DV), NW = NT / 64, V = Elem<T>::VEC, LK = S::LK, LV = S::LV, LP = S::LP, KT = DK / 16, VT = DV / 16;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   S& s = *(S*)lds;
@@ -51,7 +52,7 @@ template <typename T, int DK, int DV, bool FULL, bool BACK> __global__ __launch_
     for (int i = 0; i < (int)(sizeof(c) / sizeof(c[0])); ++i) {
       const int u = tid + i * NT, row = u / per, col = u % per * V;
       c[i] = Chunk<T>{};
-      if (row < n) c[i] = load_row<T, FULL ? FIT_FULL : FIT_ANY>(base + row * r.time + col, col, real);
+      if (row < n) c[i] = load_row<T, FIT>(base + row * r.time + col, col, real);
     }
   };
   Chunk<T> cq[NK], ck[NK], cv[NV], cg[BACK ? NV : 1];
@@ -66,7 +67,7 @@ template <typename T, int DK, int DV, bool FULL, bool BACK> __global__ __launch_
   auto at = [&](const float* m, int r, int c) { return FULL || (r < d.dk && c < d.dv) ? m[r * d.dv + c] : 0.f; };
   auto state_frag = [&](const float* m, bool turned, int g) {
     f32x4 f;
-    if (!turned && FULL) f = __builtin_bit_cast(f32x4, load_chunk(m + (r0 + colx) * d.dv + g * 16 + row4));
+    if (!turned && FIT != FIT_ANY) f = __builtin_bit_cast(f32x4, load_row<float, FIT>(m + (r0 + colx) * d.dv + g * 16 + row4, g * 16 + row4, r0 + colx < d.dk ? d.dv : 0));
     else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) f[e] = turned ? at(m, g * 16 + row4 + e, r0 + colx) : at(m, r0 + colx, g * 16 + row4 + e);
@@ -231,7 +232,7 @@ template <typename T, int DK, int DV, bool FULL, bool BACK> __global__ __launch_
       for (int e = 0; e < 4; ++e) o[e] = (T)x[t][e];
       T* to = base + i * r.time;
       if (FULL || row0 + row4 + 4 <= real) __builtin_memcpy(to, o, sizeof(o));
-      else {
+      else if (FIT == FIT_ANY) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           if (row0 + row4 + e < real) to[e] = o[e];

@@ -46,8 +46,9 @@ template <typename T> __device__ __forceinline__ void store_part(T* p, const Chu
     if (i < n) p[i] = c.e[i];
 }
 
-// ---- activations, in float.  NaN goes through every one of them.  The device library's erff, expm1f and tanhf cost a hundred instructions each; a layer's
-// epilogue runs one per output, which at 24576 x 1024 outputs took longer than the product (187 us together, 128 us with the forms below).
+// ---- activations, in float.  NaN goes through every one of them.  The device library's erff, expm1f and tanhf cost a hundred instructions each, and a layer's
+// epilogue runs one per output: a gated layer of 24576 x 512 x 1365 (bf16, silu) with its backward pass took 815 us with them, 555 us with the forms below
+// (and wider stores).
 __device__ __forceinline__ float rcp_f(float x) { return __builtin_amdgcn_rcpf(x); }  // 1 ulp
 __device__ __forceinline__ float sigmoid_f(float z) { return rcp_f(1.f + __expf(-z)); }
 

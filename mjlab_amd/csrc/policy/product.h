@@ -12,7 +12,8 @@
 //
 // float: the bf16 matrix cores are sixteen times as fast as those for float.  A float is the sum of three bf16 h + m + l (each the nearest to what is
 // left: 3 x 8 bits and their signs hold all 24), so a b = hh + hm + mh + mm + hl + lh and terms below 2^-23 |a b|, which are left out: six products
-// of 16 bits, summed in 32, for one of float -- the error of a float product's own rounding, at up to twice the float instruction's rate.  A number that has no
+// of 16 bits, summed in 32, for one of float -- the error of a float product's own rounding, at more than the float instruction's rate (24576 x 1024 x 1024: 190 TFLOP/s; the library's float product
+// 128).  A number that has no
 // such sum (infinite, NaN, or so large that h overflows) sets a flag, and its workgroup's product is formed again with the float instruction.
 #pragma once
 #include "policy_common.h"
@@ -150,8 +151,7 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
   constexpr int UE = H::UE, KT = H::KT, WM = BM / 2, WN = BN / 2, MI = WM / 32, NI = WN / 32, HALF = WN / 2, BUF = TA::BYTES + TB::BYTES;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
   const T *A = (const T*)p.A, *B = (const T*)p.B, *B2 = (const T*)p.B2;
-  // Row-contiguous operands: a tile that no row's end cuts, or one whose rows lie far enough apart that a unit read beyond the end stays before the
-  // end of the row after the next one's start
+  // Row-contiguous operands: no row's end cuts the tile, or rows are at least a unit apart, so that a unit read beyond a row's end stays inside the next row
   const bool in_a = AK || m0 + BM <= p.M, in_b = BK || n0 + BN <= p.N;
   const bool over_a = in_a || p.lda >= UE, over_b = in_b || (p.ldb >= UE && (p.kb2 == p.K || p.ldb2 >= UE));
   auto whole = [&](long long k0) {  // (uniform) the k-tile at k0 can be read without bounds
@@ -289,7 +289,9 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
 
 // Sizes of a launch: the tile, and how T is multiplied in it.  16 bits: 256 x 128 needs 48 KB of LDS with two buffers of 32 k, 128 x 128 32 KB with one of 64
 // (two and three workgroups per CU).  Other depths were no faster (16384 x 2048 x 2816 bf16, us: two buffers of 32 k 226, one of 64 k 239, registers two tiles
-// ahead 235): between the tiles' loads, fragments and matrix instructions none is the bound alone, and the library's own product takes 190 there.
+// ahead 235), nor was a loop without bounds checks (220), other orders of its instructions (220 .. 224) or a wave priority (220); 256 x 256 tiles, one workgroup
+// per CU, gain where k is long (8192 x 8192 x 8192: 1040 instead of 1140) and lose where it is not, since nothing hides their ends (24576 x 1024 x 1024: 100
+// instead of 74).  The library's product takes 190 in the first and 52 in the last.
 template <typename T, int BM_, int BN_> struct Shape {
   static constexpr int BM = BM_, BN = BN_, KB = BM_ == 256 ? 64 : 128, BUFFERS = BM_ == 128 ? 1 : 2;
   static constexpr bool SPLIT = false;

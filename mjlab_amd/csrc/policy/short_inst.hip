@@ -4,9 +4,9 @@
 
 namespace {
 
-template <int DK, int DV, bool FULL, bool BACK> hipError_t launch_sized(const ShortArgs& p, hipStream_t st) {
+template <int DK, int DV, int FIT, bool BACK> hipError_t launch_sized(const ShortArgs& p, hipStream_t st) {
   constexpr int LDS = (int)sizeof(ShortLds<DK, DV, BACK>);
-  auto kern = k_decay_short<T, DK, DV, FULL, BACK>;
+  auto kern = k_decay_short<T, DK, DV, FIT, BACK>;
   static std::atomic<unsigned long long> asked{0};
   if (hipError_t e = allow_lds(kern, LDS, asked); e != hipSuccess) return e;
   const long long rows = p.d.batch * p.d.heads;  // (below 2^24, and up to 512 threads each: below 2^32 in all is for the caller to check)
@@ -16,7 +16,9 @@ template <int DK, int DV, bool FULL, bool BACK> hipError_t launch_sized(const Sh
 }
 
 template <int DK, int DV, bool BACK> hipError_t launch_pass(const ShortArgs& p, hipStream_t st) {
-  return p.d.dk == DK && p.d.dv == DV ? launch_sized<DK, DV, true, BACK>(p, st) : launch_sized<DK, DV, false, BACK>(p, st);
+  constexpr int V = Elem<T>::VEC;
+  if (p.d.dk == DK && p.d.dv == DV) return launch_sized<DK, DV, FIT_FULL, BACK>(p, st);
+  return p.d.dk % V || p.d.dv % V ? launch_sized<DK, DV, FIT_ANY, BACK>(p, st) : launch_sized<DK, DV, FIT_CHUNKS, BACK>(p, st);
 }
 
 template <int DK, bool BACK> hipError_t launch_dv(const ShortArgs& p, hipStream_t st) {
