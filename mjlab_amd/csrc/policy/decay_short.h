@@ -76,7 +76,7 @@ template <typename T, int DK, int DV, int FIT, bool BACK> __global__ __launch_bo
   };
   const float* st = d.state ? d.state + sh * d.dk * d.dv : nullptr;
   const float* ds = BACK && p.d_state_out ? p.d_state_out + sh * d.dk * d.dv : nullptr;
-  constexpr bool EARLY = DK <= 64 && DV <= 64;
+  constexpr bool EARLY = BACK ? DK <= 64 && DV <= 64 : true;
   f32x4 fx[EARLY ? (BACK ? VT : KT) : 1], fy[EARLY && BACK ? VT : 1], fz[EARLY && BACK ? KT : 1], acc_state[VT];
   auto early = [&](auto& f, const float* m, bool turned) {
 #pragma unroll
