@@ -36,7 +36,8 @@ int mjlab_sizeof_layer(void) { return (int)sizeof(mjlab_layer_t); }
 int mjlab_sizeof_layer_grad(void) { return (int)sizeof(mjlab_layer_grad_t); }
 
 static int check_z(const mjlab_layer_t& f) {
-  if ((f.z || f.z_up) && f.z_bytes != (f.w_up || f.dtype == MJLAB_DTYPE_F32 ? 4 : 2)) return fail(-2, "layer: z_bytes: a gated layer's sums are floats, a dense layer's of its dtype");
+  if ((f.z || f.z_up) && f.z_bytes != 4 && (f.w_up || f.dtype == MJLAB_DTYPE_F32 || f.z_bytes != 2)) return fail(-2, "layer: z_bytes: a gated layer's sums are floats, a dense layer's floats or of its dtype");
+  if (f.z && f.z_is_y && f.z_bytes != (f.dtype == MJLAB_DTYPE_F32 ? 4 : 2)) return fail(-2, "layer: z_bytes: y is of the layer's dtype");
   return 0;
 }
 

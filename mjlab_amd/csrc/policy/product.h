@@ -26,7 +26,7 @@ struct Product {
   long long M, N, K, kb2;      // kb2: where B's rows end and B2's begin (K where there is no B2)
   long long nb2;               // the same for a k-contiguous B outside EPI_GATED (N where there is no B2)
   long long ksplit;            // k elements per blockIdx.y
-  int act;
+  int act, z_float;            // z_float: z holds floats (a gated layer's always)
   const void *b, *b_up, *r;    // the epilogue's
   void *y, *z, *z_up;
   long long ldr, ldy;
@@ -417,7 +417,7 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
         rows([&](int q, long long m) { put((T*)p.y + p.N, p.ldy, q, m, u[q]); });
       } else if constexpr (EPI != EPI_STORE) {
         if (p.z) rows([&](int q, long long m) {
-          if constexpr (GATED) put_float(p.z, q, m, v[q]);
+          if (GATED || p.z_float) put_float(p.z, q, m, v[q]);
           else put(p.z, p.N, q, m, v[q]);
         });
         with_act(p.act, [&](auto act) {
@@ -484,7 +484,7 @@ template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_join_
   }
   if (p.b) v += (float)((const T*)p.b)[c];
   if (p.z) {
-    if constexpr (GATED) ((float*)p.z)[i] = v;
+    if (GATED || p.z_float) ((float*)p.z)[i] = v;
     else ((T*)p.z)[i] = (T)v;
   }
   with_act(p.act, [&](auto act) { v = act_value<decltype(act)::value>(v); });
@@ -498,10 +498,12 @@ template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_join_
 
 // dz (rows, out | 2 out) from dy and the stored sums, and this row block's column sums for the bias gradient.
 // 256 threads: 32 chunk columns x 8 rows, four rows of each thread in flight, over SLOPE_ROWS rows; workgroups: row blocks x `colblocks`.
-// dz NULL: column sums of dy alone.  FROM: what is stored is the layer's output.  Bound by memory: dense two reads and a write, gated three and two.
+// dz NULL: column sums of dy alone.  FROM: what is stored is the layer's output.  WIDE: the sums are floats.  Bound by memory: dense two reads and a write, gated
+// three and two.
 #define SLOPE_ROWS 64
-template <typename T, bool GATED, bool FROM> __global__ __launch_bounds__(256) void k_layer_slope(const T* dy, long long ld_dy, const void* z, const float* z_up, T* dz,
+template <typename T, bool GATED, bool FROM, bool WIDE> __global__ __launch_bounds__(256) void k_layer_slope(const T* dy, long long ld_dy, const void* z, const float* z_up, T* dz,
                                                                                                    float* sums, long long rows, long long out, unsigned colblocks, int act) {
+  static_assert(WIDE || !GATED, "a gated layer's sums are floats");
   constexpr int V = Elem<T>::VEC, NS = GATED ? 2 : 1, ROWS = GATED ? 1 : 2;
   __shared__ float part[NS][8][32 * V];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -511,17 +513,20 @@ template <typename T, bool GATED, bool FROM> __global__ __launch_bounds__(256) v
   const bool slope = dz && (GATED || act != MJLAB_ACT_NONE);
   for (int i = ty; i < SLOPE_ROWS && r0 + i < rows; i += 8 * ROWS) {
     Chunk<T> d[ROWS], g[ROWS];
-    float z0[GATED ? ROWS : 1][V], z1[GATED ? ROWS : 1][V];  // (a gated layer's sums are floats)
+    float z0[WIDE ? ROWS : 1][V], z1[GATED ? ROWS : 1][V];
 #pragma unroll
     for (int q = 0; q < ROWS; ++q) {
       const long long m = r0 + i + 8 * q, have = m < rows ? left : 0;
       d[q] = load_part(dy + m * ld_dy + n, have);
-      if constexpr (GATED) {
+      if constexpr (WIDE) {
 #pragma unroll
         for (int e = 0; e < V; e += 4) {
-          const Chunk<float> x = load_part((const float*)z + m * out + n + e, have - e), y = load_part(z_up + m * out + n + e, have - e);
+          const Chunk<float> x = load_part((const float*)z + m * out + n + e, slope ? have - e : 0), y = load_part(z_up + m * out + n + e, GATED ? have - e : 0);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) { z0[q][e + k] = x.e[k]; z1[q][e + k] = y.e[k]; }
+          for (int k = 0; k < 4; ++k) {
+            z0[q][e + k] = x.e[k];
+            if constexpr (GATED) z1[q][e + k] = y.e[k];
+          }
         }
       } else if (slope) g[q] = load_part((const T*)z + m * out + n, have);
     }
@@ -534,7 +539,7 @@ template <typename T, bool GATED, bool FROM> __global__ __launch_bounds__(256) v
           constexpr int ACT = decltype(a)::value;
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float x = GATED ? z0[GATED ? q : 0][e] : (float)g[q].e[e], t = (float)d[q].e[e];
+            const float x = WIDE ? z0[WIDE ? q : 0][e] : (float)g[q].e[e], t = (float)d[q].e[e];
             float v = t * (FROM ? act_slope_out<ACT>(x) : act_slope<ACT>(x));
             if constexpr (GATED) {
               v *= z1[q][e];
