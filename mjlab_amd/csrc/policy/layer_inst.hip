@@ -73,9 +73,14 @@ int weight_splits(long long out, long long in, long long rows) {
 
 long long up256(long long x) { return (x + 255) & ~255LL; }
 
+// dz is rounded to the type, which small layers in 16 bits need not bear: up to 2^28 multiplications per product, dz is two numbers of the type (its rounding and
+// what that left), and the products with it are formed for both.  That takes the device 5 us more at 2^28 (a call takes the host 70), and gradients are then
+// as exact as their own rounding: off by 1.00 times it instead of 1.41, which few rows or columns make 2 now and then.
+bool two_planes(const mjlab_layer_t& f, long long ns) { return sizeof(T) == 2 && f.rows * f.in < (1LL << 28) && f.rows * f.in * ns <= (1LL << 28) / f.out; }
+
 struct Plan {
   bool gated, slope, sums, weights, again;
-  long long ns, blocks, o_dz, o_sums, o_partial, bytes;
+  long long ns, planes, blocks, o_dz, o_sums, o_partial, bytes;
   int splits, x_splits;
 };
 
@@ -85,6 +90,7 @@ Plan plan(const mjlab_layer_grad_t* g) {
   q.gated = f.w_up != nullptr;
   q.ns = q.gated ? 2 : 1;
   q.slope = q.gated || f.act != MJLAB_ACT_NONE;
+  q.planes = q.slope && two_planes(f, q.ns) ? 2 : 1;
   q.sums = g->db != nullptr;
   q.weights = g->dw != nullptr;
   q.again = q.gated && !f.z;
@@ -94,15 +100,16 @@ Plan plan(const mjlab_layer_grad_t* g) {
     const int bm = c.best == c.large ? 256 : c.best == c.mid ? 128 : 64;
     q.blocks = 2 * ((f.rows + bm - 1) / bm);
   }
-  q.splits = weight_splits(q.ns * f.out, f.in, f.rows);
+  q.splits = weight_splits(q.planes * q.ns * f.out, f.in, f.rows);
   long long at = 0;
   q.o_dz = at;
-  if (q.slope) at += up256(f.rows * q.ns * f.out * (long long)sizeof(T));
+  if (q.slope) at += up256(f.rows * q.planes * q.ns * f.out * (long long)sizeof(T));
   q.o_sums = at;
   if (q.sums) at += up256(q.blocks * q.ns * f.out * 4);
-  q.x_splits = g->dx ? sum_splits<false>(f.rows, f.in, q.ns * f.out) : 1;
+  q.x_splits = g->dx ? sum_splits<false>(f.rows, f.in, q.gated ? 2 * f.out : q.planes * f.out) : 1;
   q.o_partial = at;  // (dx's sums are joined before dw's are formed)
-  const long long w = q.weights && (q.splits > 1 || q.gated) ? q.splits * q.ns * f.out * f.in : 0, x = q.x_splits > 1 ? q.x_splits * f.rows * f.in : 0;
+  const long long w = q.weights && (q.splits > 1 || q.gated || q.planes > 1) ? q.splits * q.planes * q.ns * f.out * f.in : 0;
+  const long long x_parts = q.x_splits * (q.gated ? q.planes : 1), x = x_parts > 1 ? x_parts * f.rows * f.in : 0;
   at += up256((w > x ? w : x) * 4);
   q.bytes = at;
   return q;
@@ -157,7 +164,7 @@ hipError_t POLICY_NAME(mjlab_launch_layer_backward)(const mjlab_layer_grad_t* g,
   if (q.again) {
     if constexpr (sizeof(T) == 2) {
       Product p = forward_product(&f);
-      p.r = g->dy; p.ldr = g->ld_dy; p.y = dz; p.ldy = 2 * f.out; p.z = p.z_up = nullptr; p.partial = sums;
+      p.r = g->dy; p.ldr = g->ld_dy; p.y = dz; p.ldy = q.planes * 2 * f.out; p.low = q.planes > 1 ? 2 * f.out : 0; p.z = p.z_up = nullptr; p.partial = sums;
       if ((e = launch_product<true, true, EPI_SLOPE>(p, 1, st)) != hipSuccess) return e;
     } else return hipErrorInvalidValue;
   } else if (q.slope || q.sums) {
@@ -168,7 +175,8 @@ hipError_t POLICY_NAME(mjlab_launch_layer_backward)(const mjlab_layer_grad_t* g,
                 : f.z_is_y ? k_layer_slope<T, false, true, false>
                 : sizeof(T) == 2 && f.z_bytes == 4 ? k_layer_slope<T, false, false, sizeof(T) == 2>
                                                    : k_layer_slope<T, false, false, false>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(colblocks * q.blocks)), dim3(256), 0, st, (const T*)g->dy, g->ld_dy, f.z, (const float*)f.z_up, q.slope ? dz : nullptr, sums, f.rows, f.out, (unsigned)colblocks, f.act);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(colblocks * q.blocks)), dim3(256), 0, st, (const T*)g->dy, g->ld_dy, f.z, (const float*)f.z_up, q.slope ? dz : nullptr, q.planes * q.ns * f.out,
+                       q.planes > 1 ? q.ns * f.out : 0, sums, f.rows, f.out, (unsigned)colblocks, f.act);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (q.sums) {
@@ -177,38 +185,43 @@ hipError_t POLICY_NAME(mjlab_launch_layer_backward)(const mjlab_layer_grad_t* g,
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   const void* d = q.slope ? (const void*)dz : g->dy;
-  const long long ldd = q.slope ? q.ns * f.out : g->ld_dy;
+  const long long ldd = q.slope ? q.planes * q.ns * f.out : g->ld_dy;
   if (g->dx) {
+    // a dense layer's planes are one sum over 2 out of k, with w in turn; a gated layer's two products
     Product p = {};
-    p.A = d; p.lda = ldd; p.B = f.w; p.ldb = f.ldw; p.B2 = f.w_up; p.ldb2 = f.ldw_up;
-    p.M = f.rows; p.N = p.nb2 = f.in; p.K = p.ksplit = q.ns * f.out; p.kb2 = f.out;
+    p.A = d; p.lda = ldd; p.B = f.w; p.ldb = f.ldw; p.B2 = q.gated ? f.w_up : f.w; p.ldb2 = q.gated ? f.ldw_up : f.ldw;
+    p.M = f.rows; p.N = p.nb2 = f.in; p.K = p.ksplit = q.gated ? 2 * f.out : q.planes * f.out; p.kb2 = f.out;
     p.y = g->dx; p.ldy = f.in; p.partial = partial;
-    if (q.x_splits == 1) {
+    const long long parts = q.gated ? q.planes : 1;
+    if (q.x_splits * parts == 1) {
       if ((e = launch_product<true, false, EPI_STORE>(p, 1, st)) != hipSuccess) return e;
     } else {
       p.ksplit = per_split(p.K, q.x_splits);
       const int splits = (int)((p.K + p.ksplit - 1) / p.ksplit);
       const long long n = f.rows * f.in;
       if ((n + 255) / 256 > MAX_BLOCKS) return hipErrorInvalidValue;
-      if ((e = launch_product<true, false, EPI_PARTIAL>(p, splits, st)) != hipSuccess) return e;
-      hipLaunchKernelGGL(k_join_splits<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, partial, (T*)g->dx, n, n, splits);
+      for (int part = 0; part < parts; ++part) {
+        p.A = (const T*)d + part * q.ns * f.out; p.partial = partial + part * splits * n;
+        if ((e = launch_product<true, false, EPI_PARTIAL>(p, splits, st)) != hipSuccess) return e;
+      }
+      hipLaunchKernelGGL(k_join_splits<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, partial, (T*)g->dx, n, n, splits * (int)parts);
       if ((e = hipGetLastError()) != hipSuccess) return e;
     }
   }
   if (g->dw) {
     Product p = {};
     p.A = d; p.lda = ldd; p.B = f.x; p.ldb = f.ldx;
-    p.M = q.ns * f.out; p.N = p.nb2 = f.in; p.K = p.kb2 = f.rows;
+    p.M = q.planes * q.ns * f.out; p.N = p.nb2 = f.in; p.K = p.kb2 = f.rows;
     p.ksplit = per_split(f.rows, q.splits);
     const int splits = (int)((f.rows + p.ksplit - 1) / p.ksplit);
     p.y = g->dw; p.ldy = f.in; p.partial = partial;
-    if (splits == 1 && !q.gated) return launch_product<false, false, EPI_STORE>(p, 1, st);
+    if (splits == 1 && !q.gated && q.planes == 1) return launch_product<false, false, EPI_STORE>(p, 1, st);
     if ((e = launch_product<false, false, EPI_PARTIAL>(p, splits, st)) != hipSuccess) return e;
     const long long n = f.out * f.in;
     if ((n + 255) / 256 > MAX_BLOCKS) return hipErrorInvalidValue;
     for (int u = 0; u < (q.gated ? 2 : 1); ++u) {
-      // (a gated layer's partials hold both matrices: 2 n floats per split)
-      hipLaunchKernelGGL(k_join_splits<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, partial + u * n, (T*)(u ? g->dw_up : g->dw), n, q.ns * n, splits);
+      // (partials: splits x planes x a gated layer's two matrices)
+      hipLaunchKernelGGL(k_join_splits<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, partial + u * n, (T*)(u ? g->dw_up : g->dw), n, q.ns * n, splits * (int)q.planes);
       if ((e = hipGetLastError()) != hipSuccess) return e;
     }
   }

@@ -32,6 +32,7 @@ struct Product {
   long long ldr, ldy;
   float* partial;              // EPI_PARTIAL: (splits, M, N); EPI_SLOPE: column sums of y, (2 M / BM, 2 N), or NULL
                                // EPI_SLOPE: a gated layer's sums formed again; r = dy, y = [dg | du]
+  long long low;               // EPI_SLOPE: columns from y to what its rounding left, or 0 (not wanted)
 };
 
 __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c, _Float16) {
@@ -309,6 +310,12 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> struct ProductL
   static constexpr int BYTES = TILES > EPILOGUE ? (TILES > AGAIN ? TILES : AGAIN) : (EPILOGUE > AGAIN ? EPILOGUE : AGAIN);
 };
 
+// What rounding x to T left, as T (a second plane of dz); 0 where nothing can be left
+template <typename T> __device__ __forceinline__ T rest(float x, T h) {
+  const float r = x - (float)h;
+  return (T)(__builtin_fabsf(r) < 1e38f ? r : 0.f);
+}
+
 template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __launch_bounds__(256, 2) void k_product(const Product p) {
   using S = Shape<T, BM, BN>;
   constexpr int V = Elem<T>::VEC, WM = BM / 2, WN = BN / 2, MI = WM / 32, NI = WN / 32;
@@ -415,6 +422,15 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
             }
         });
         rows([&](int q, long long m) { put((T*)p.y + p.N, p.ldy, q, m, u[q]); });
+        if (p.low) {
+          rows([&](int q, long long m) {
+            float x[OV], y[OV];
+#pragma unroll
+            for (int e = 0; e < OV; ++e) { x[e] = (float)rest<T>(v[q][e], (T)v[q][e]); y[e] = (float)rest<T>(u[q][e], (T)u[q][e]); }
+            put((T*)p.y + p.low, p.ldy, q, m, x);
+            put((T*)p.y + p.low + p.N, p.ldy, q, m, y);
+          });
+        }
       } else if constexpr (EPI != EPI_STORE) {
         if (p.z) rows([&](int q, long long m) {
           if (GATED || p.z_float) put_float(p.z, q, m, v[q]);
@@ -496,13 +512,14 @@ template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_join_
   ((T*)p.y)[m * p.ldy + c] = (T)v;
 }
 
-// dz (rows, out | 2 out) from dy and the stored sums, and this row block's column sums for the bias gradient.
+// dz (rows, out | 2 out) from dy and the stored sums, and this row block's column sums for the bias gradient.  low: columns to a second plane, what the rounding of
+// dz left (0: not wanted).
 // 256 threads: 32 chunk columns x 8 rows, four rows of each thread in flight, over SLOPE_ROWS rows; workgroups: row blocks x `colblocks`.
 // dz NULL: column sums of dy alone.  FROM: what is stored is the layer's output.  WIDE: the sums are floats.  Bound by memory: dense two reads and a write, gated
 // three and two.
 #define SLOPE_ROWS 64
 template <typename T, bool GATED, bool FROM, bool WIDE> __global__ __launch_bounds__(256) void k_layer_slope(const T* dy, long long ld_dy, const void* z, const float* z_up, T* dz,
-                                                                                                   float* sums, long long rows, long long out, unsigned colblocks, int act) {
+                                                                                                   long long pitch, long long low, float* sums, long long rows, long long out, unsigned colblocks, int act) {
   static_assert(WIDE || !GATED, "a gated layer's sums are floats");
   constexpr int V = Elem<T>::VEC, NS = GATED ? 2 : 1, ROWS = GATED ? 1 : 2;
   __shared__ float part[NS][8][32 * V];
@@ -534,7 +551,7 @@ template <typename T, bool GATED, bool FROM, bool WIDE> __global__ __launch_boun
     for (int q = 0; q < ROWS; ++q) {
       const long long m = r0 + i + 8 * q;
       if (slope) {
-        Chunk<T> o;
+        Chunk<T> o, lo, lu;  // du; what the roundings left
         with_act(act, [&](auto a) {
           constexpr int ACT = decltype(a)::value;
 #pragma unroll
@@ -546,14 +563,21 @@ template <typename T, bool GATED, bool FROM, bool WIDE> __global__ __launch_boun
               const float w = t * act_value<ACT>(x);
               s[NS - 1][e] += w;
               o.e[e] = (T)w;
+              lu.e[e] = rest<T>(w, o.e[e]);
             }
             s[0][e] += v;
             d[q].e[e] = (T)v;
+            lo.e[e] = rest<T>(v, d[q].e[e]);
           }
         });
         if (m < rows && left > 0) {
-          store_part(dz + m * (NS * out) + n, d[q], left);
-          if constexpr (GATED) store_part(dz + m * (NS * out) + out + n, o, left);
+          T* at = dz + m * pitch + n;
+          store_part(at, d[q], left);
+          if constexpr (GATED) store_part(at + out, o, left);
+          if (low) {
+            store_part(at + low, lo, left);
+            if constexpr (GATED) store_part(at + low + out, lu, left);
+          }
         }
       } else {
 #pragma unroll

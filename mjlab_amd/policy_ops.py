@@ -116,10 +116,10 @@ _FROM_OUTPUT = {ACTIVATIONS[a] for a in ("relu", "elu", "tanh", "sigmoid")}
 
 
 # 16-bit dense layers whose sums are kept as floats: the slopes of these fall like exp(-2 |z|) and exp(-|z|), and a z that is rounded shows in the gradients (tanh:
-# 1.54 times the error of their own rounding, 1.41 with floats).  silu and gelu (1.46) keep floats where it costs nothing: 2^22 sums are 8 MB more each
+# 1.54 times the error of their own rounding, 1.41 with floats).  elu (1.14), silu and gelu (1.46) keep floats where it costs nothing: 2^22 sums are 8 MB more each
 # way, 3 us of a call that takes the host 70; for 24576 x 1024 it would be 20 us of 300.
 _WIDE = {ACTIVATIONS[a] for a in ("tanh", "sigmoid")}
-_WIDE_SMALL = {ACTIVATIONS[a] for a in ("silu", "gelu")}
+_WIDE_SMALL = {ACTIVATIONS[a] for a in ("elu", "silu", "gelu")}
 
 
 def _from_output(x, w_up, r, act: int) -> bool:

@@ -3,7 +3,9 @@
 The bounds are worst cases, from the sizes alone.  u = half a step of the type; sums run in 32 bits (u32 = 2^-24), in any order, so a sum of
 n products a_i b_i is off by at most (n + 2) u32 sum |a_i b_i|.  An activation is Lipschitz with constant <= 1.13 (silu, gelu) and its slope with
 constant <= 1; evaluating either in 32 bits is off by at most 16 u32 of (1 + |z|).  Forward: error of z, times 1.13, plus evaluation, plus one
-rounding.  Backward: the slope is taken at z rounded to the type (not rounded: gated layers, tanh, sigmoid, and silu and gelu up to 2^22 sums), dz is rounded to the type, then one product and one rounding more.  The
+rounding.
+Backward: the slope is taken at z rounded to the type (not rounded: gated layers, tanh, sigmoid, and elu, silu and gelu up to 2^22 sums), dz is
+rounded to the type (up to 2^28 multiplications per product: to two numbers of it, u^2 instead of u), then one product and one rounding more.  The
 slope of relu jumps at 0: where |z| is inside its error bound, the whole |dy| may be lost."""
 
 import pytest
@@ -75,7 +77,7 @@ def check_layer(m, k, n, dtype, name, gated, bias, residual, x=None, seed=0):
     z, ez = sums(w, b)
     f, df = act(z, name)
     ef = 1.13 * ez + 16 * U32 * (1 + z.abs())
-    uz, tz = (0, 0) if gated or name in ("tanh", "sigmoid") or (name in ("silu", "gelu") and m * n <= 1 << 22) else (u, tiny)  # (these sums are not rounded)
+    uz, tz = (0, 0) if gated or name in ("tanh", "sigmoid") or (name in ("elu", "silu", "gelu") and m * n <= 1 << 22) else (u, tiny)  # (these sums are not rounded)
     edf = ez + uz * z.abs() + tz + 16 * U32 * (1 + z.abs()) + ((z.abs() <= ez).double() if name == "relu" else 0)
     if name == "none" and not gated:
       edf = torch.zeros_like(z)
@@ -90,7 +92,8 @@ def check_layer(m, k, n, dtype, name, gated, bias, residual, x=None, seed=0):
     e = e + 4 * U32 * (want.abs() + (0 if r is None else r.double().abs()))
     close(y, want, e + u * (want.abs() + e) + tiny, "y")
     rounded = gated or name != "none"
-    edz = [d + (4 * U32 + (u if rounded else 0)) * (z_.abs() + d) + (tiny if rounded else 0) for z_, d in zip(dz, edz, strict=True)]
+    udz = 0 if not rounded else u if dtype == torch.float32 or (2 if gated else 1) * m * k * n > 1 << 28 else u * u
+    edz = [d + (4 * U32 + udz) * (z_.abs() + d) + (tiny if rounded else 0) for z_, d in zip(dz, edz, strict=True)]
     ws = [w, wu] if gated else [w]
     dx = sum(d @ q.double() for d, q in zip(dz, ws, strict=True))
     ex = sum(d @ q.double().abs() + (2 * n + 2) * U32 * ((z_.abs() + d) @ q.double().abs()) for z_, d, q in zip(dz, edz, ws, strict=True))
@@ -285,6 +288,29 @@ def test_refusals_on_the_device():
   for kind, call in bad:
     with pytest.raises(kind):
       call()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gated", [False, True])
+def test_sizes_whose_dz_is_one_number(dtype, gated):
+  check_layer(1203, 1001, 1003, dtype, "gelu", gated, bias=True, residual=False, seed=15)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("gated", [False, True])
+def test_an_infinite_upstream_gradient_stays_infinite(dtype, gated):
+  """... in its row of dx: its rounding leaves nothing, not a NaN."""
+  from mjlab_amd import policy_ops
+
+  x, w, wu = (torch.rand((n, 24), device="cuda").to(dtype).add_(0.5).requires_grad_(True) for n in (40, 30, 30))
+  y = policy_ops.gated(x, w, wu, activation="sigmoid") if gated else policy_ops.dense(x, w, activation="sigmoid")
+  dy = torch.ones_like(y)
+  dy[7, 3] = float("inf")
+  dx, dw = torch.autograd.grad(y, [x, w], dy)
+  bad = torch.zeros((40,), dtype=torch.bool, device="cuda")
+  bad[7] = True
+  assert (dx[7] == float("inf")).all() and dx[~bad].isfinite().all()
+  assert (dw[3] == float("inf")).all() and dw[:3].isfinite().all() and dw[4:].isfinite().all()
 
 
 def test_an_output_over_a_kept_input_is_noticed():
