@@ -29,23 +29,24 @@ struct DecayPass {
   float *seg_state, *seg_factor;  // (seg_given: seg_state is read only) (sequences * heads, segments - 1, da, dc), (sequences * heads, segments - 1)
 };
 
-// What the matrix cores read.  float as it is.  bf16 as it is; what is formed on the way (weighted rows, pairs, R) is rounded to it, like the outputs.  fp16: a b^T
+// What the matrix cores read.  float as it is.  bf16 as it is; what is formed on the way (weighted rows, pairs, R) is rounded to it, like the outputs,
+// but for the weighted rows of a pass whose R is wanted in the end (EXACT), a float output: they are three.  fp16: a b^T
 // as it is, but sums of keys and values may leave fp16's range, so all else is multiplied as sums of bf16, each the nearest to what is left: two hold
 // an fp16 number and 16 bits of R and of a pair (outputs are rounded to 11), three a weighted row (which R, a float output in the end, is made of).
-template <typename T> struct DecayCfg {
+template <typename T, bool EXACT> struct DecayCfg {
   using L = float;
   static constexpr int KS = 4, PAD = 4, A = 1, W = 1, N = 1;  // k per matrix instruction, padding of LDS rows, planes of a, of weighted b, of c, P and R
 };
-template <> struct DecayCfg<__bf16> {
+template <bool EXACT> struct DecayCfg<__bf16, EXACT> {
   using L = __bf16;
-  static constexpr int KS = 32, PAD = 8, A = 1, W = 1, N = 1;
+  static constexpr int KS = 32, PAD = 8, A = 1, W = EXACT ? 3 : 1, N = 1;
 };
-template <> struct DecayCfg<_Float16> {
+template <bool EXACT> struct DecayCfg<_Float16, EXACT> {
   using L = __bf16;
   static constexpr int KS = 32, PAD = 8, A = 2, W = 3, N = 2;
 };
 // tokens per chunk
-template <typename T> constexpr int decay_chunk(bool both_large) { return sizeof(T) == 4 || (DecayCfg<T>::N > 1 && both_large) ? 32 : 64; }
+template <typename T> constexpr int decay_chunk(bool both_large) { return sizeof(T) == 4 || (DecayCfg<T, false>::N > 1 && both_large) ? 32 : 64; }
 
 __device__ __forceinline__ f32x4 mma16(s16x8 a, s16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
@@ -75,8 +76,8 @@ __device__ __forceinline__ bool reset_at(const DecayPass& p, long long seq, long
   return p.reset_bytes == 1 ? ((const unsigned char*)p.reset)[i] != 0 : ((const int*)p.reset)[i] != 0;
 }
 
-template <typename T, int DA, int DC, bool STATE> struct DecayLds {
-  using Cfg = DecayCfg<T>;
+template <typename T, int DA, int DC, bool STATE, bool EXACT> struct DecayLds {
+  using Cfg = DecayCfg<T, EXACT>;
   using L = typename Cfg::L;
   static constexpr int C = decay_chunk<T>(DA > 64 && DC > 64), PAD = Cfg::PAD, LA = DA + PAD, LC = DC + PAD, LP = C + PAD;
   static constexpr int SW = C * LA, SC = C * LC, SP = STATE ? 8 : C * LP, SR = STATE ? 8 : DC * LA;  // a plane of each
@@ -160,10 +161,10 @@ constexpr int decay_threads(int da, int dc) { return da >= 64 && dc >= 64 ? 512 
 // 256 sequences of 1024 tokens, forward: bf16 128 x 128 75 us (3.6 TB/s), 64 x 64 47 us, 32 x 32 45 us; fp16 64 x 64 63 us, 128 x 128 235 us; float 64 x 64
 // 128 us, 128 x 128 300 us.  Large bf16 heads are near the memory's rate; the others are bound by the chain of a chunk (stage, pairs, R, with a barrier
 // and LDS reads between): 2.5 us for a chunk of 64 at 32 x 32, 2.3 with every row in L2.  More workgroups per CU, where there are more sequences, hide it.
-template <typename T, int DA, int DC, int FIT, bool STATE> __global__ __launch_bounds__(decay_threads(DA, DC), 2) void k_decay_chunks(const DecayPass p) {
-  using Cfg = DecayCfg<T>;
+template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global__ __launch_bounds__(decay_threads(DA, DC), 2) void k_decay_chunks(const DecayPass p) {
+  using Cfg = DecayCfg<T, EXACT>;
   using L = typename Cfg::L;
-  using S = DecayLds<T, DA, DC, STATE>;
+  using S = DecayLds<T, DA, DC, STATE, EXACT>;
   constexpr bool FULL = FIT == FIT_FULL;
   // The scheduler is kept from loading the fragments of every column at once: small heads have the registers for it (float 64 x 64 128 us without, 135 with)
   constexpr bool FENCE = DA * DC > 64 * 64;
@@ -328,7 +329,7 @@ template <typename T, int DA, int DC, int FIT, bool STATE> __global__ __launch_b
       const float w = row < n && !cut_out && (whole || episode(row) == e_last) ? p.us * power(n - p.e0 - row) : 0.f;
       put_weighted<PW>(s.bw + row * LA + col, S::SW, xb[i], w);
       if constexpr (!STATE) *(Chunk<T>*)(s.b + row * LA + col) = xb[i];
-      if constexpr (NN > 1) see(most, xb[i]);
+      if constexpr (PW > 1) see(most, xb[i]);
     }
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
@@ -359,7 +360,7 @@ template <typename T, int DA, int DC, int FIT, bool STATE> __global__ __launch_b
       for (int t = 0; t < TR; ++t)
 #pragma unroll
         for (int k = 0; k < KA; ++k) see(most, __builtin_bit_cast(Chunk<T>, fa[t][k]));
-    // A zero weight times infinity would be NaN: a chunk whose c holds one goes term by term.  (fp16: any operand, since a plane may be zero.)
+    // A zero weight times infinity would be NaN: a chunk whose c holds one goes term by term.  (Planes: any operand, since one may be zero.)
     const bool mine = __ballot(seen_odd<T>(most) || odd != odd) != 0;
     if (lane == 0) s.odd[wave] = mine;
     __syncthreads();

@@ -13,7 +13,7 @@ struct Split {
 Split split(const mjlab_decay_t* d) {
   const int C = decay_chunk<T>(d->dk > 64 && d->dv > 64);
   const long long chunks = (d->length + C - 1) / C, rows = d->batch * d->heads, least = d->dk < d->dv ? d->dk : d->dv, most_d = d->dk < d->dv ? d->dv : d->dk;
-  const bool alone = DecayCfg<T>::N > 1 ? least > 32 || most_d > 64 : least > 32 && most_d > 64;  // whether LDS holds one workgroup per CU, or two
+  const bool alone = DecayCfg<T, false>::N > 1 ? least > 32 || most_d > 64 : least > 32 && most_d > 64;  // whether LDS holds one workgroup per CU, or two
   const long long slots = alone ? CUS : 2 * CUS;
   if (2 * rows >= slots || chunks < 8) return {1, (int)chunks};
   const long long want = slots / rows, most = chunks / 4, s = want < most ? want : most;
@@ -24,29 +24,34 @@ Split split(const mjlab_decay_t* d) {
 long long up256(long long x) { return (x + 255) & ~255LL; }
 long long state_bytes(const mjlab_decay_t* d, const Split& s) { return up256(d->batch * d->heads * (s.segments - 1) * (long long)d->dk * d->dv * 4); }
 
-template <int DA, int DC, int FIT> hipError_t launch_sized(const DecayPass& p, long long rows, hipStream_t st) {
-  constexpr int LDS = (int)sizeof(DecayLds<T, DA, DC, false>), LDS_FIRST = (int)sizeof(DecayLds<T, DA, DC, true>);
+template <int DA, int DC, int FIT, bool EXACT> hipError_t launch_sized(const DecayPass& p, long long rows, hipStream_t st) {
+  constexpr int LDS = (int)sizeof(DecayLds<T, DA, DC, false, EXACT>), LDS_FIRST = (int)sizeof(DecayLds<T, DA, DC, true, EXACT>);
   static std::atomic<unsigned long long> asked{0}, asked_first{0};
   hipError_t e;
   if (rows * p.segments * decay_threads(DA, DC) > 0xffffffffLL) return hipErrorInvalidValue;
   if (p.segments > 1 && !p.seg_given) {
-    auto first = k_decay_chunks<T, DA, DC, FIT, true>;
+    auto first = k_decay_chunks<T, DA, DC, FIT, true, EXACT>;
     if ((e = allow_lds(first, LDS_FIRST, asked_first)) != hipSuccess) return e;
     hipLaunchKernelGGL(first, dim3((unsigned)(rows * (p.segments - 1))), dim3(decay_threads(DA, DC)), LDS_FIRST, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     hipLaunchKernelGGL(k_decay_scan<T>, dim3((unsigned)(rows * ((p.da * p.dc + 255) / 256))), dim3(256), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  auto kern = k_decay_chunks<T, DA, DC, FIT, false>;
+  auto kern = k_decay_chunks<T, DA, DC, FIT, false, EXACT>;
   if ((e = allow_lds(kern, LDS, asked)) != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3((unsigned)(rows * p.segments)), dim3(decay_threads(DA, DC)), LDS, st, p);
   return hipGetLastError();
 }
 
-template <int DA, int DC> hipError_t launch_pass(const DecayPass& p, long long rows, hipStream_t st) {
+template <int DA, int DC, bool EXACT> hipError_t launch_fit(const DecayPass& p, long long rows, hipStream_t st) {
   constexpr int V = Elem<T>::VEC;
-  if (p.da == DA && p.dc == DC) return launch_sized<DA, DC, FIT_FULL>(p, rows, st);
-  return p.da % V || p.dc % V ? launch_sized<DA, DC, FIT_ANY>(p, rows, st) : launch_sized<DA, DC, FIT_CHUNKS>(p, rows, st);
+  if (p.da == DA && p.dc == DC) return launch_sized<DA, DC, FIT_FULL, EXACT>(p, rows, st);
+  return p.da % V || p.dc % V ? launch_sized<DA, DC, FIT_ANY, EXACT>(p, rows, st) : launch_sized<DA, DC, FIT_CHUNKS, EXACT>(p, rows, st);
+}
+
+template <int DA, int DC> hipError_t launch_pass(const DecayPass& p, long long rows, hipStream_t st) {
+  if (p.state_out && DecayCfg<T, true>::W != DecayCfg<T, false>::W) return launch_fit<DA, DC, DecayCfg<T, true>::W != DecayCfg<T, false>::W>(p, rows, st);
+  return launch_fit<DA, DC, false>(p, rows, st);
 }
 
 template <int DA> hipError_t launch_dc(const DecayPass& p, long long rows, hipStream_t st) {

@@ -67,33 +67,36 @@ __device__ __forceinline__ float tanh_f(float z) {
   return q < 0.0625f ? s : d;
 }
 
-// (1 + erf(z / sqrt 2)) / 2 with e = exp(-z^2 / 2): Abramowitz and Stegun 7.1.26, off by 0.75e-7 at most
-__device__ __forceinline__ float normal_cdf(float z, float e) {
+// (1 + erf(z / sqrt 2)) / 2 with e = exp(-z^2 / 2).  Abramowitz and Stegun 7.1.26, off by 0.75e-7 at most: enough for 16 bits.  FINE: to the last bits of small
+// values too, as a float output shows them.
+template <bool FINE> __device__ __forceinline__ float normal_cdf(float z, float e) {
+  if constexpr (FINE) return 0.5f * erfcf(-0.70710678f * z);
   const float t = rcp_f(1.f + 0.3275911f * 0.70710678f * __builtin_fabsf(z));
   const float tail = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
   return z < 0.f ? tail : 1.f - tail;
 }
 
-template <int ACT> __device__ __forceinline__ float act_value(float z) {
+// FINE: for float outputs
+template <int ACT, bool FINE> __device__ __forceinline__ float act_value(float z) {
   if constexpr (ACT == MJLAB_ACT_RELU) return z < 0.f ? 0.f : z;
   if constexpr (ACT == MJLAB_ACT_ELU) return z > 0.f ? z : expm1_neg(z);
   if constexpr (ACT == MJLAB_ACT_TANH) return tanh_f(z);
   if constexpr (ACT == MJLAB_ACT_SIGMOID) return sigmoid_f(z);
   if constexpr (ACT == MJLAB_ACT_SILU) return z * sigmoid_f(z);
-  if constexpr (ACT == MJLAB_ACT_GELU) return z * normal_cdf(z, __expf(-0.5f * z * z));
+  if constexpr (ACT == MJLAB_ACT_GELU) return z * normal_cdf<FINE>(z, __expf(-0.5f * z * z));
   return z;
 }
 
 // Derivative at z.  Beyond |z| = 100 the derivative of each is its limit to all 24 bits: z is cut there, so that a z that 16 bits hold
 // as infinite gives the limit and not infinity times zero.
-template <int ACT> __device__ __forceinline__ float act_slope(float z) {
+template <int ACT, bool FINE> __device__ __forceinline__ float act_slope(float z) {
   z = z > 100.f ? 100.f : (z < -100.f ? -100.f : z);
   if constexpr (ACT == MJLAB_ACT_RELU) return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
   if constexpr (ACT == MJLAB_ACT_ELU) return z > 0.f ? 1.f : __expf(z);
   if constexpr (ACT == MJLAB_ACT_TANH) { const float e = __expf(-2.f * __builtin_fabsf(z)), r = rcp_f(1.f + e); return 4.f * e * r * r; }
   if constexpr (ACT == MJLAB_ACT_SIGMOID) { const float e = __expf(-__builtin_fabsf(z)), r = rcp_f(1.f + e); return e * r * r; }
   if constexpr (ACT == MJLAB_ACT_SILU) { const float s = sigmoid_f(z); return s * (1.f + z * (1.f - s)); }
-  if constexpr (ACT == MJLAB_ACT_GELU) { const float e = __expf(-0.5f * z * z); return normal_cdf(z, e) + z * 0.39894228f * e; }
+  if constexpr (ACT == MJLAB_ACT_GELU) { const float e = __expf(-0.5f * z * z); return normal_cdf<FINE>(z, e) + z * 0.39894228f * e; }
   return 1.f;
 }
 

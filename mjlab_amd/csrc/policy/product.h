@@ -414,8 +414,8 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
 #pragma unroll
             for (int e = 0; e < OV; ++e) {
               const float d = (float)res[q].e[e], g = v[q][e];  // (d is 0 behind the last row)
-              v[q][e] = d * act_slope<ACT>(g) * u[q][e];
-              u[q][e] = d * act_value<ACT>(g);
+              v[q][e] = d * act_slope<ACT, sizeof(T) == 4>(g) * u[q][e];
+              u[q][e] = d * act_value<ACT, sizeof(T) == 4>(g);
               const bool there = m0 + wm + i * 32 + q * RPP + lane / LPR < p.M;  // (what stands behind may be infinite)
               sum[e] += there ? v[q][e] : 0.f;
               sum_up[e] += there ? u[q][e] : 0.f;
@@ -440,7 +440,7 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
 #pragma unroll
           for (int q = 0; q < PASSES; ++q)
 #pragma unroll
-            for (int e = 0; e < OV; ++e) v[q][e] = act_value<decltype(act)::value>(v[q][e]);
+            for (int e = 0; e < OV; ++e) v[q][e] = act_value<decltype(act)::value, sizeof(T) == 4>(v[q][e]);
         });
         if constexpr (GATED) {
           if (p.z_up) rows([&](int q, long long m) { put_float(p.z_up, q, m, u[q]); });
@@ -503,7 +503,7 @@ template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_join_
     if (GATED || p.z_float) ((float*)p.z)[i] = v;
     else ((T*)p.z)[i] = (T)v;
   }
-  with_act(p.act, [&](auto act) { v = act_value<decltype(act)::value>(v); });
+  with_act(p.act, [&](auto act) { v = act_value<decltype(act)::value, sizeof(T) == 4>(v); });
   if constexpr (GATED) {
     if (p.b_up) u += (float)((const T*)p.b_up)[c];
     if (p.z_up) ((float*)p.z_up)[i] = u;
@@ -557,10 +557,10 @@ template <typename T, bool GATED, bool FROM, bool WIDE> __global__ __launch_boun
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const float x = WIDE ? z0[WIDE ? q : 0][e] : (float)g[q].e[e], t = (float)d[q].e[e];
-            float v = t * (FROM ? act_slope_out<ACT>(x) : act_slope<ACT>(x));
+            float v = t * (FROM ? act_slope_out<ACT>(x) : act_slope<ACT, sizeof(T) == 4>(x));
             if constexpr (GATED) {
               v *= z1[q][e];
-              const float w = t * act_value<ACT>(x);
+              const float w = t * act_value<ACT, sizeof(T) == 4>(x);
               s[NS - 1][e] += w;
               o.e[e] = (T)w;
               lu.e[e] = rest<T>(w, o.e[e]);
