@@ -158,7 +158,7 @@ constexpr int decay_threads(int da, int dc) { return da >= 64 && dc >= 64 ? 512 
 // 256 or 512 threads per (sequence, head, segment).  STATE: the first pass of a split sequence, the segment's contribution to R alone.
 // Products are formed such that an accumulator's four rows are neighbours in memory: P^T and out^T (columns are tokens), R (rows are da).  The rows of a go
 // from memory to the matrix cores' registers without LDS, which holds one workgroup of 128 x 128 heads per CU (bf16 96 KB).
-// 256 sequences of 1024 tokens, forward: bf16 128 x 128 75 us (3.6 TB/s), 64 x 64 47 us, 32 x 32 45 us; fp16 64 x 64 63 us, 128 x 128 235 us; float 64 x 64
+// 256 sequences of 1024 tokens, forward: bf16 128 x 128 84 us (75, 3.6 TB/s, where R is not wanted in the end), 64 x 64 57 us (47), 32 x 32 47 us (45); fp16 64 x 64 63 us, 128 x 128 235 us; float 64 x 64
 // 128 us, 128 x 128 300 us.  Large bf16 heads are near the memory's rate; the others are bound by the chain of a chunk (stage, pairs, R, with a barrier
 // and LDS reads between): 2.5 us for a chunk of 64 at 32 x 32, 2.3 with every row in L2.  More workgroups per CU, where there are more sequences, hide it.
 template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global__ __launch_bounds__(decay_threads(DA, DC), 2) void k_decay_chunks(const DecayPass p) {

@@ -67,10 +67,17 @@ __device__ __forceinline__ float tanh_f(float z) {
   return q < 0.0625f ? s : d;
 }
 
-// (1 + erf(z / sqrt 2)) / 2 with e = exp(-z^2 / 2).  Abramowitz and Stegun 7.1.26, off by 0.75e-7 at most: enough for 16 bits.  FINE: to the last bits of small
-// values too, as a float output shows them.
+// (1 + erf(z / sqrt 2)) / 2 with e = exp(-z^2 / 2).  Abramowitz and Stegun 7.1.26, off by 0.75e-7 at most: enough for 16 bits.  FINE, for float outputs: the
+// Chebyshev fit of erfc whose relative error is 1.2e-7 everywhere (Press et al., Numerical Recipes, 6.2), since small values show theirs.
+// (24576 x 512 x 512 float, us: the first form 90, the second 93, erfcf 117.)
 template <bool FINE> __device__ __forceinline__ float normal_cdf(float z, float e) {
-  if constexpr (FINE) return 0.5f * erfcf(-0.70710678f * z);
+  if constexpr (FINE) {
+    const float x = 0.70710678f * __builtin_fabsf(z), t = rcp_f(1.f + 0.5f * x);
+    const float q = 1.48851587f + t * (-0.82215223f + t * 0.17087277f);
+    const float r = 0.37409196f + t * (0.09678418f + t * (-0.18628806f + t * (0.27886807f + t * (-1.13520398f + t * q))));
+    const float tail = 0.5f * t * e * __expf(-1.26551223f + t * (1.00002368f + t * r));
+    return z < 0.f ? tail : 1.f - tail;
+  }
   const float t = rcp_f(1.f + 0.3275911f * 0.70710678f * __builtin_fabsf(z));
   const float tail = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
   return z < 0.f ? tail : 1.f - tail;

@@ -316,7 +316,8 @@ template <typename T> __device__ __forceinline__ T rest(float x, T h) {
   return (T)(__builtin_fabsf(r) < 1e38f ? r : 0.f);
 }
 
-template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __launch_bounds__(256, 2) void k_product(const Product p) {
+// (Three workgroups of 128 x 128 per CU need 168 registers: the activations' branches are held to that, or all pay, 83 -> 94 us at 24576 x 512 x 512 float.)
+template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __launch_bounds__(256, BK && BM == 128 ? 3 : 2) void k_product(const Product p) {
   using S = Shape<T, BM, BN>;
   constexpr int V = Elem<T>::VEC, WM = BM / 2, WN = BN / 2, MI = WM / 32, NI = WN / 32;
   constexpr bool SLOPE = EPI == EPI_SLOPE, GATED = EPI == EPI_GATED || SLOPE;
