@@ -283,6 +283,35 @@ def test_graph_replays_equal_eager():
       assert torch.equal(a, c)
 
 
+@pytest.mark.parametrize("t", [20, 300])
+def test_gradients_against_differences(t):
+  """The outputs are linear in each of q, k, v and the state, so (f(x + d) - f(x - d)) / 2 = grad . d but for rounding: three values, each off by as many
+  roundings as above of the same sums over magnitudes."""
+  from mjlab_amd import policy_ops
+
+  x = inputs(2, t, 3, 24, 40, torch.float32, seed=16, resets=0.02, ragged=True, carry=True)
+  names = ("q", "k", "v", "state")
+  rest = (x["reset"], x["lengths"])
+  lam = x["log_decay"].double().exp()
+
+  def f(leaves):
+    o, final = policy_ops.decay_attention(*leaves[:3], x["log_decay"], state=leaves[3], reset=rest[0], lengths=rest[1])
+    return (o.double() * x["do"].double()).sum() + (final.double() * x["dstate"].double()).sum()
+
+  leaves = [x[n].requires_grad_(True) for n in names]
+  grads = torch.autograd.grad(f(leaves), leaves)
+  gen = torch.Generator(device="cuda").manual_seed(17)
+  with torch.no_grad():
+    for i, g in enumerate(grads):
+      d = torch.randn(leaves[i].shape, generator=gen, device="cuda")
+      moved = [[a + sign * d if j == i else a for j, a in enumerate(leaves)] for sign in (1, -1)]
+      big = [(a.abs() + d.abs() if j == i else a.abs()) for j, a in enumerate(leaves)]
+      mo, ms = recurrence(*big[:3], lam, 24**-0.5, big[3], *rest)
+      mag = (mo * x["do"].double().abs()).sum() + (ms * x["dstate"].double().abs()).sum()
+      steps = 40 + t + 4 * (t // 32 + 1) + float(x["log_decay"].abs().max()) * t + 32
+      assert abs((f(moved[0]) - f(moved[1])) / 2 - (g.double() * d.double()).sum()) <= 3 * steps * U32 * mag, names[i]
+
+
 def test_only_the_wanted_gradients():
   from mjlab_amd import policy_ops
 
