@@ -53,9 +53,8 @@ int mjlab_layer_recomputes(const mjlab_layer_t* f);
  *   dense: dz = dy act'(z);                          dx = dz w;            dw = dz^T x;  db = sum over rows of dz
  *   gated: dg = dy z_up act'(z), du = dy act(z);     dx = dg w + du w_up;  dw = dg^T x, dw_up = du^T x;  db, db_up likewise
  * (the residual's gradient is dy itself).  A dense layer without activation needs no z.  Each output is dense and may be NULL (not wanted);
- * dw / dw_up and db / db_up come together.  dz is rounded to `dtype`, since the matrix cores read it, but for small layers in 16 bits: there it is two numbers
- * (the second 0 as often as not, so an infinite x or w makes NaN of the sums that it is in).  workspace: device memory of
- * mjlab_layer_backward_workspace() bytes, free again when the launches have run. */
+ * dw / dw_up and db / db_up come together.  dz, dg and du are floats, whatever `dtype` is, and multiplied to 2^-16 (float: 2^-23) of each term.
+ * workspace: device memory of mjlab_layer_backward_workspace() bytes, free again when the launches have run. */
 typedef struct mjlab_layer_grad {
   mjlab_layer_t f;
   const void* dy;

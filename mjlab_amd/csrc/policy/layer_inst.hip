@@ -4,11 +4,11 @@
 
 namespace {
 
-template <bool AK, bool BK, int BM, int BN, int EPI> hipError_t launch_tile(const Product& p, int splits, hipStream_t st) {
-  constexpr int BNO = EPI == EPI_GATED || EPI == EPI_SLOPE ? BN / 2 : BN, LDS = ProductLds<T, AK, BK, BM, BN, EPI>::BYTES;
+template <typename TA, bool AK, bool BK, int BM, int BN, int EPI> hipError_t launch_tile(const Product& p, int splits, hipStream_t st) {
+  constexpr int BNO = EPI == EPI_GATED || EPI == EPI_SLOPE ? BN / 2 : BN, LDS = ProductLds<TA, T, AK, BK, BM, BN, EPI>::BYTES;
   const long long tiles = ((p.M + BM - 1) / BM) * ((p.N + BNO - 1) / BNO);
   if (tiles > MAX_BLOCKS) return hipErrorInvalidValue;
-  auto kern = k_product<T, AK, BK, BM, BN, EPI>;
+  auto kern = k_product<TA, T, AK, BK, BM, BN, EPI>;
   static std::atomic<unsigned long long> asked{0};
   if (hipError_t e = allow_lds(kern, LDS, asked); e != hipSuccess) return e;
   hipLaunchKernelGGL(kern, dim3((unsigned)tiles, (unsigned)splits), dim3(256), LDS, st, p);
@@ -19,7 +19,7 @@ template <bool AK, bool BK, int BM, int BN, int EPI> hipError_t launch_tile(cons
 // once; a round with fewer takes up to 0.4 of a tile longer than its share, since nothing hides what it waits for.  Per element of C a smaller tile costs
 // more: 128 x 128 12 % (24 % where an operand has to be turned), 64 x 64 60 % (124 %); float, whose matrix instructions take longer, 33 % over 128 x 128.
 // Measured (us; 256 x 128 / 128 x 128 / 64 x 64): bf16 y of 16384 x 2048 x 2816 226 / 234 / 351, 24576 x 512 x 1365 71 / 63 / 83,
-// 4096 x 1024 x 1024 30 / 20 / 24; dx of 24576 x 512 x 1365 66 / 77 / 90; float y of 24576 x 1024 x 1024 - / 278 / 368, 512 x 2048 x 2048 - / 116 / 52.
+// 4096 x 1024 x 1024 30 / 20 / 24; dx of a layer without activation, 24576 x 512 x 1365, 66 / 77 / 90; float y of 24576 x 1024 x 1024 - / 278 / 368, 512 x 2048 x 2048 - / 116 / 52.
 float tile_cost(long long tiles, float cost, int at_once) {
   const long long n = (tiles + CUS - 1) / CUS, rest = n % at_once;
   return cost * (n + (rest ? 0.4f * (at_once - rest) / (at_once - 1) : 0.f));
@@ -30,33 +30,36 @@ struct Cost {
 };
 // A layer's epilogue (BK: the products that have one) is hidden behind the other workgroups of a CU, of which the large tile leaves one: counted as 0.13 of the
 // large tile's time at 1024 k (gated bf16 24576 rows, us, large / mid: 512 x 1365 122 / 110, [dg | du] 187 / 158; 1024 x 2048 264 / 264).
-template <bool BK> Cost costs(long long M, long long width, long long K, long long splits) {
+// TA: what memory holds A as: float for dz, also where T has 16 bits.  There 128 x 128 costs a quarter less than 64 x 64, and a 256 x 128 tile has no registers left.
+// (dx with its slope kernel, 128 x 128 / 64 x 64, us: bf16 24576 x 1024 x 1024 201 / 239, 4096 x 1024 x 1024 49 / 49, 1024 x 512 x 512 29 / 22;
+// fp16 237 / 292, 58 / 59, 33 / 23.)
+template <typename TA, bool BK> Cost costs(long long M, long long width, long long K, long long splits) {
   auto tiles = [&](int bm, int bn) { return (M + bm - 1) / bm * ((width + bn - 1) / bn) * splits; };
-  constexpr bool F32 = sizeof(T) == 4;
+  constexpr bool F32 = sizeof(T) == 4, MIXED = sizeof(TA) != sizeof(T);
   Cost c;
-  c.small = tile_cost(tiles(64, 64), F32 ? 0.166f : BK ? 0.2f : 0.28f, F32 ? 3 : 5);
+  c.small = tile_cost(tiles(64, 64), F32 ? 0.166f : BK || MIXED ? 0.2f : 0.28f, F32 ? 3 : 5);
   c.mid = tile_cost(tiles(128, 128), F32 ? 0.5f : BK ? 0.56f : 0.62f, BK ? 3 : 2);
-  c.large = F32 ? 1e30f : tile_cost(tiles(256, 128), BK ? 1.f + 133.f / K : 1.f, 2);
+  c.large = F32 || MIXED ? 1e30f : tile_cost(tiles(256, 128), BK ? 1.f + 133.f / K : 1.f, 2);
   c.best = c.large < c.mid && c.large < c.small ? c.large : c.mid < c.small ? c.mid : c.small;
   return c;
 }
 
-template <bool AK, bool BK, int EPI> hipError_t launch_product(const Product& p, int splits, hipStream_t st) {
-  const Cost c = costs<BK>(p.M, EPI == EPI_GATED || EPI == EPI_SLOPE ? 2 * p.N : p.N, p.K, splits);
-  if constexpr (sizeof(T) == 2)
-    if (c.best == c.large) return launch_tile<AK, BK, 256, 128, EPI>(p, splits, st);
-  return c.best == c.mid ? launch_tile<AK, BK, 128, 128, EPI>(p, splits, st) : launch_tile<AK, BK, 64, 64, EPI>(p, splits, st);
+template <typename TA, bool AK, bool BK, int EPI> hipError_t launch_product(const Product& p, int splits, hipStream_t st) {
+  const Cost c = costs<TA, BK>(p.M, EPI == EPI_GATED || EPI == EPI_SLOPE ? 2 * p.N : p.N, p.K, splits);
+  if constexpr (sizeof(TA) == 2)
+    if (c.best == c.large) return launch_tile<TA, AK, BK, 256, 128, EPI>(p, splits, st);
+  return c.best == c.mid ? launch_tile<TA, AK, BK, 128, 128, EPI>(p, splits, st) : launch_tile<TA, AK, BK, 64, 64, EPI>(p, splits, st);
 }
 
 // Few rows leave most CUs idle: the sum over k is then split, each part's sums go through memory, and a second launch joins them.  The time of an unsplit unit of
-// tile_cost() is about 21 ns per k (float 80 ns), the second launch 4 us and what it reads at 3 TB/s.
+// tile_cost() is about 21 ns per k (float 80 ns, dz in 16 bits 42 ns), the second launch 4 us and what it reads at 3 TB/s.
 // (64 rows, 2048 x 2048: float 49 us unsplit, 12 + 4 us split; bf16 17 us, 6 + 3 us.)
-template <bool BK> int sum_splits(long long M, long long width, long long K) {
-  const float per_k = sizeof(T) == 4 ? 0.08f : 0.021f;
+template <typename TA, bool BK> int sum_splits(long long M, long long width, long long K) {
+  const float per_k = sizeof(T) == 4 ? 0.08f : sizeof(TA) == 4 ? 0.042f : 0.021f;
   int best = 1;
-  float time = costs<BK>(M, width, K, 1).best * K * per_k;
+  float time = costs<TA, BK>(M, width, K, 1).best * K * per_k;
   for (int s = 2; s <= 32 && K / s >= 128; s *= 2) {
-    const float t = costs<BK>(M, width, K, s).best * K / s * per_k + 4.f + 4e-6f * M * width * s * 0.67f;
+    const float t = costs<TA, BK>(M, width, K, s).best * K / s * per_k + 4.f + 4e-6f * M * width * s * 0.67f;
     if (t < time) { time = t; best = s; }
   }
   return best;
@@ -73,14 +76,9 @@ int weight_splits(long long out, long long in, long long rows) {
 
 long long up256(long long x) { return (x + 255) & ~255LL; }
 
-// dz is rounded to the type, which small layers in 16 bits need not bear: up to 2^28 multiplications per product, dz is two numbers of the type (its rounding and
-// what that left), and the products with it are formed for both.  That takes the device 5 us more at 2^28 (a call takes the host 70), and gradients are then
-// as exact as their own rounding: off by 1.00 times it instead of 1.41, which few rows or columns make 2 now and then.
-bool two_planes(const mjlab_layer_t& f, long long ns) { return sizeof(T) == 2 && f.rows * f.in < (1LL << 28) && f.rows * f.in * ns <= (1LL << 28) / f.out; }
-
 struct Plan {
   bool gated, slope, sums, weights, again;
-  long long ns, planes, blocks, o_dz, o_sums, o_partial, bytes;
+  long long ns, blocks, o_dz, o_sums, o_partial, bytes;
   int splits, x_splits;
 };
 
@@ -90,32 +88,31 @@ Plan plan(const mjlab_layer_grad_t* g) {
   q.gated = f.w_up != nullptr;
   q.ns = q.gated ? 2 : 1;
   q.slope = q.gated || f.act != MJLAB_ACT_NONE;
-  q.planes = q.slope && two_planes(f, q.ns) ? 2 : 1;
   q.sums = g->db != nullptr;
   q.weights = g->dw != nullptr;
   q.again = q.gated && !f.z;
   q.blocks = (f.rows + SLOPE_ROWS - 1) / SLOPE_ROWS;
   if (q.again) {  // two sets of column sums per tile of rows
-    const Cost c = costs<true>(f.rows, 2 * f.out, f.in, 1);
+    const Cost c = costs<T, true>(f.rows, 2 * f.out, f.in, 1);
     const int bm = c.best == c.large ? 256 : c.best == c.mid ? 128 : 64;
     q.blocks = 2 * ((f.rows + bm - 1) / bm);
   }
-  q.splits = weight_splits(q.planes * q.ns * f.out, f.in, f.rows);
+  q.splits = weight_splits(q.ns * f.out, f.in, f.rows);
   long long at = 0;
   q.o_dz = at;
-  if (q.slope) at += up256(f.rows * q.planes * q.ns * f.out * (long long)sizeof(T));
+  if (q.slope) at += up256(f.rows * q.ns * f.out * 4);
   q.o_sums = at;
   if (q.sums) at += up256(q.blocks * q.ns * f.out * 4);
-  q.x_splits = g->dx ? sum_splits<false>(f.rows, f.in, q.gated ? 2 * f.out : q.planes * f.out) : 1;
+  const long long k = q.ns * f.out;
+  q.x_splits = !g->dx ? 1 : q.slope ? sum_splits<float, false>(f.rows, f.in, k) : sum_splits<T, false>(f.rows, f.in, k);
   q.o_partial = at;  // (dx's sums are joined before dw's are formed)
-  const long long w = q.weights && (q.splits > 1 || q.gated || q.planes > 1) ? q.splits * q.planes * q.ns * f.out * f.in : 0;
-  const long long x_parts = q.x_splits * (q.gated ? q.planes : 1), x = x_parts > 1 ? x_parts * f.rows * f.in : 0;
+  const long long w = q.weights && (q.splits > 1 || q.gated) ? q.splits * k * f.in : 0, x = q.x_splits > 1 ? q.x_splits * f.rows * f.in : 0;
   at += up256((w > x ? w : x) * 4);
   q.bytes = at;
   return q;
 }
 
-int forward_splits(const mjlab_layer_t* f) { return sum_splits<true>(f->rows, f->w_up ? 2 * f->out : f->out, f->in); }
+int forward_splits(const mjlab_layer_t* f) { return sum_splits<T, true>(f->rows, f->w_up ? 2 * f->out : f->out, f->in); }
 
 Product forward_product(const mjlab_layer_t* f) {
   Product p = {};
@@ -123,6 +120,43 @@ Product forward_product(const mjlab_layer_t* f) {
   p.M = f->rows; p.N = p.nb2 = f->out; p.K = p.kb2 = p.ksplit = f->in;
   p.act = f->act; p.z_float = f->z_bytes == 4; p.b = f->b; p.b_up = f->b_up; p.r = f->r; p.ldr = f->ldr; p.y = f->y; p.ldy = f->ldy; p.z = f->z; p.z_up = f->z_up;
   return p;
+}
+
+// dx and dw (dw_up) from d, the gradient of the sums before the activation: rows of q.ns out, `ldd` apart
+template <typename TA> hipError_t input_gradient(const mjlab_layer_grad_t* g, const Plan& q, const void* d, long long ldd, float* partial, hipStream_t st) {
+  const mjlab_layer_t& f = g->f;
+  Product p = {};
+  p.A = d; p.lda = ldd; p.B = f.w; p.ldb = f.ldw; p.B2 = f.w_up; p.ldb2 = f.ldw_up;
+  p.M = f.rows; p.N = p.nb2 = f.in; p.K = p.ksplit = q.ns * f.out; p.kb2 = f.out;
+  p.y = g->dx; p.ldy = f.in; p.partial = partial;
+  if (q.x_splits == 1) return launch_product<TA, true, false, EPI_STORE>(p, 1, st);
+  p.ksplit = per_split(p.K, q.x_splits);
+  const int splits = (int)((p.K + p.ksplit - 1) / p.ksplit);
+  const long long n = f.rows * f.in;
+  if ((n + 255) / 256 > MAX_BLOCKS) return hipErrorInvalidValue;
+  if (hipError_t e = launch_product<TA, true, false, EPI_PARTIAL>(p, splits, st); e != hipSuccess) return e;
+  hipLaunchKernelGGL(k_join_splits<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, partial, (T*)g->dx, n, n, splits);
+  return hipGetLastError();
+}
+
+template <typename TA> hipError_t weight_gradient(const mjlab_layer_grad_t* g, const Plan& q, const void* d, long long ldd, float* partial, hipStream_t st) {
+  const mjlab_layer_t& f = g->f;
+  Product p = {};
+  p.A = d; p.lda = ldd; p.B = f.x; p.ldb = f.ldx;
+  p.M = q.ns * f.out; p.N = p.nb2 = f.in; p.K = p.kb2 = f.rows;
+  p.ksplit = per_split(f.rows, q.splits);
+  const int splits = (int)((f.rows + p.ksplit - 1) / p.ksplit);
+  p.y = g->dw; p.ldy = f.in; p.partial = partial;
+  if (splits == 1 && !q.gated) return launch_product<TA, false, false, EPI_STORE>(p, 1, st);
+  if (hipError_t e = launch_product<TA, false, false, EPI_PARTIAL>(p, splits, st); e != hipSuccess) return e;
+  const long long n = f.out * f.in;
+  if ((n + 255) / 256 > MAX_BLOCKS) return hipErrorInvalidValue;
+  for (int u = 0; u < (q.gated ? 2 : 1); ++u) {
+    // (partials: splits x a gated layer's two matrices)
+    hipLaunchKernelGGL(k_join_splits<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, partial + u * n, (T*)(u ? g->dw_up : g->dw), n, q.ns * n, splits);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace
@@ -133,13 +167,13 @@ int POLICY_NAME(mjlab_layer_again)(const mjlab_layer_t* f) { return sizeof(T) ==
 hipError_t POLICY_NAME(mjlab_launch_layer_forward)(const mjlab_layer_t* f, hipStream_t st) {
   Product p = forward_product(f);
   const int s = forward_splits(f);
-  if (s == 1) return f->w_up ? launch_product<true, true, EPI_GATED>(p, 1, st) : launch_product<true, true, EPI_LAYER>(p, 1, st);
+  if (s == 1) return f->w_up ? launch_product<T, true, true, EPI_GATED>(p, 1, st) : launch_product<T, true, true, EPI_LAYER>(p, 1, st);
   Product q = p;
   q.N = f->w_up ? 2 * f->out : f->out;
   q.ksplit = per_split(f->in, s);
   q.partial = p.partial = (float*)f->workspace;
   const int splits = (int)((f->in + q.ksplit - 1) / q.ksplit);
-  if (hipError_t e = launch_product<true, true, EPI_PARTIAL>(q, splits, st); e != hipSuccess) return e;
+  if (hipError_t e = launch_product<T, true, true, EPI_PARTIAL>(q, splits, st); e != hipSuccess) return e;
   const long long blocks = (f->rows * f->out + 255) / 256;
   if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
   auto join = f->w_up ? k_join_layer<T, true> : k_join_layer<T, false>;
@@ -158,14 +192,14 @@ hipError_t POLICY_NAME(mjlab_launch_layer_backward)(const mjlab_layer_grad_t* g,
   const mjlab_layer_t& f = g->f;
   const Plan q = plan(g);
   char* ws = (char*)g->workspace;
-  T* dz = (T*)(ws + q.o_dz);
+  float* dz = (float*)(ws + q.o_dz);
   float *sums = q.sums ? (float*)(ws + q.o_sums) : nullptr, *partial = (float*)(ws + q.o_partial);
   hipError_t e = hipSuccess;
   if (q.again) {
     if constexpr (sizeof(T) == 2) {
       Product p = forward_product(&f);
-      p.r = g->dy; p.ldr = g->ld_dy; p.y = dz; p.ldy = q.planes * 2 * f.out; p.low = q.planes > 1 ? 2 * f.out : 0; p.z = p.z_up = nullptr; p.partial = sums;
-      if ((e = launch_product<true, true, EPI_SLOPE>(p, 1, st)) != hipSuccess) return e;
+      p.r = g->dy; p.ldr = g->ld_dy; p.y = dz; p.ldy = 2 * f.out; p.z = p.z_up = nullptr; p.partial = sums;
+      if ((e = launch_product<T, true, true, EPI_SLOPE>(p, 1, st)) != hipSuccess) return e;
     } else return hipErrorInvalidValue;
   } else if (q.slope || q.sums) {
     constexpr int V = Elem<T>::VEC;
@@ -175,8 +209,7 @@ hipError_t POLICY_NAME(mjlab_launch_layer_backward)(const mjlab_layer_grad_t* g,
                 : f.z_is_y ? k_layer_slope<T, false, true, false>
                 : sizeof(T) == 2 && f.z_bytes == 4 ? k_layer_slope<T, false, false, sizeof(T) == 2>
                                                    : k_layer_slope<T, false, false, false>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(colblocks * q.blocks)), dim3(256), 0, st, (const T*)g->dy, g->ld_dy, f.z, (const float*)f.z_up, q.slope ? dz : nullptr, q.planes * q.ns * f.out,
-                       q.planes > 1 ? q.ns * f.out : 0, sums, f.rows, f.out, (unsigned)colblocks, f.act);
+    hipLaunchKernelGGL(kern, dim3((unsigned)(colblocks * q.blocks)), dim3(256), 0, st, (const T*)g->dy, g->ld_dy, f.z, (const float*)f.z_up, q.slope ? dz : nullptr, q.ns * f.out, sums, f.rows, f.out, (unsigned)colblocks, f.act);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (q.sums) {
@@ -184,46 +217,10 @@ hipError_t POLICY_NAME(mjlab_launch_layer_backward)(const mjlab_layer_grad_t* g,
     hipLaunchKernelGGL(k_join_sums<T>, dim3((unsigned)((cols + 15) / 16)), dim3(256), 0, st, sums, (T*)g->db, (T*)g->db_up, f.out, cols, q.blocks);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  const void* d = q.slope ? (const void*)dz : g->dy;
-  const long long ldd = q.slope ? q.planes * q.ns * f.out : g->ld_dy;
-  if (g->dx) {
-    // a dense layer's planes are one sum over 2 out of k, with w in turn; a gated layer's two products
-    Product p = {};
-    p.A = d; p.lda = ldd; p.B = f.w; p.ldb = f.ldw; p.B2 = q.gated ? f.w_up : f.w; p.ldb2 = q.gated ? f.ldw_up : f.ldw;
-    p.M = f.rows; p.N = p.nb2 = f.in; p.K = p.ksplit = q.gated ? 2 * f.out : q.planes * f.out; p.kb2 = f.out;
-    p.y = g->dx; p.ldy = f.in; p.partial = partial;
-    const long long parts = q.gated ? q.planes : 1;
-    if (q.x_splits * parts == 1) {
-      if ((e = launch_product<true, false, EPI_STORE>(p, 1, st)) != hipSuccess) return e;
-    } else {
-      p.ksplit = per_split(p.K, q.x_splits);
-      const int splits = (int)((p.K + p.ksplit - 1) / p.ksplit);
-      const long long n = f.rows * f.in;
-      if ((n + 255) / 256 > MAX_BLOCKS) return hipErrorInvalidValue;
-      for (int part = 0; part < parts; ++part) {
-        p.A = (const T*)d + part * q.ns * f.out; p.partial = partial + part * splits * n;
-        if ((e = launch_product<true, false, EPI_PARTIAL>(p, splits, st)) != hipSuccess) return e;
-      }
-      hipLaunchKernelGGL(k_join_splits<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, partial, (T*)g->dx, n, n, splits * (int)parts);
-      if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
+  if (q.slope) {
+    if (g->dx && (e = input_gradient<float>(g, q, dz, q.ns * f.out, partial, st)) != hipSuccess) return e;
+    return g->dw ? weight_gradient<float>(g, q, dz, q.ns * f.out, partial, st) : hipSuccess;
   }
-  if (g->dw) {
-    Product p = {};
-    p.A = d; p.lda = ldd; p.B = f.x; p.ldb = f.ldx;
-    p.M = q.planes * q.ns * f.out; p.N = p.nb2 = f.in; p.K = p.kb2 = f.rows;
-    p.ksplit = per_split(f.rows, q.splits);
-    const int splits = (int)((f.rows + p.ksplit - 1) / p.ksplit);
-    p.y = g->dw; p.ldy = f.in; p.partial = partial;
-    if (splits == 1 && !q.gated && q.planes == 1) return launch_product<false, false, EPI_STORE>(p, 1, st);
-    if ((e = launch_product<false, false, EPI_PARTIAL>(p, splits, st)) != hipSuccess) return e;
-    const long long n = f.out * f.in;
-    if ((n + 255) / 256 > MAX_BLOCKS) return hipErrorInvalidValue;
-    for (int u = 0; u < (q.gated ? 2 : 1); ++u) {
-      // (partials: splits x planes x a gated layer's two matrices)
-      hipLaunchKernelGGL(k_join_splits<T>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, partial + u * n, (T*)(u ? g->dw_up : g->dw), n, q.ns * n, splits * (int)q.planes);
-      if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
-  }
-  return hipSuccess;
+  if (g->dx && (e = input_gradient<T>(g, q, g->dy, g->ld_dy, partial, st)) != hipSuccess) return e;
+  return g->dw ? weight_gradient<T>(g, q, g->dy, g->ld_dy, partial, st) : hipSuccess;
 }

@@ -15,13 +15,17 @@
 // of 16 bits, summed in 32, for one of float -- the error of a float product's own rounding, at more than the float instruction's rate (24576 x 1024 x 1024: 190 TFLOP/s; the library's float product
 // 128).  A number that has no
 // such sum (infinite, NaN, or so large that h overflows) sets a flag, and its workgroup's product is formed again with the float instruction.
+//
+// dz, 16 bits: a float in memory, since a gradient may leave fp16's range on both sides where what it is summed to does not, and since its rounding to 16 bits would
+// show in the gradients (off by 1.41 times their own rounding).  It is read as two bf16, 2^-16 of it left out, and a float16 that it meets as two, exactly:
+// hh + hm + mh, two or three products of 16 bits for one.
 #pragma once
 #include "policy_common.h"
 
 enum { EPI_LAYER = 0, EPI_GATED = 1, EPI_STORE = 2, EPI_PARTIAL = 3, EPI_SLOPE = 4 };
 
 struct Product {
-  const void *A, *B, *B2;      // B2: w_up (EPI_GATED: rows of both in turn; EPI_STORE: the rows k >= kb2 of B)
+  const void *A, *B, *B2;      // A: of the kernel's type TA, B and B2 of T.  B2: w_up (EPI_GATED: rows of both in turn; EPI_STORE: the rows k >= kb2 of B)
   long long lda, ldb, ldb2;
   long long M, N, K, kb2;      // kb2: where B's rows end and B2's begin (K where there is no B2)
   long long nb2;               // the same for a k-contiguous B outside EPI_GATED (N where there is no B2)
@@ -31,8 +35,7 @@ struct Product {
   void *y, *z, *z_up;
   long long ldr, ldy;
   float* partial;              // EPI_PARTIAL: (splits, M, N); EPI_SLOPE: column sums of y, (2 M / BM, 2 N), or NULL
-                               // EPI_SLOPE: a gated layer's sums formed again; r = dy, y = [dg | du]
-  long long low;               // EPI_SLOPE: columns from y to what its rounding left, or 0 (not wanted)
+                               // EPI_SLOPE: a gated layer's sums formed again; r = dy, y = [dg | du] as floats
 };
 
 __device__ __forceinline__ f32x16 mma(s16x8 a, s16x8 b, f32x16 c, _Float16) {
@@ -51,7 +54,7 @@ template <typename E> struct Frag { using type = s16x8; };
 template <> struct Frag<float> { using type = f32x4; };
 
 // A unit: what one thread loads, keeps and stages at a time, UE neighbouring elements of memory.
-template <typename T, int UE> struct alignas(16) Unit {
+template <typename T, int UE> struct alignas(sizeof(T) * UE < 16 ? sizeof(T) * UE : 16) Unit {
   T e[UE];
 };
 template <typename T, int UE> __device__ __forceinline__ void load_unit(Unit<T, UE>& u, const T* p) { __builtin_memcpy(&u, p, sizeof(u)); }
@@ -61,63 +64,56 @@ template <typename T, int UE> __device__ __forceinline__ void load_unit_part(Uni
   for (int i = 0; i < UE; ++i) u.e[i] = i < n ? p[i] : (T)0.f;
 }
 
-// How T is multiplied: as it is (E = T; 16 bits, or the float instruction) or as the sum of three bf16 (SPLIT).
+// How an operand is multiplied: memory holds M, the matrix cores read it as the sum of P numbers of E, each the nearest to what is left.
 // KB: bytes of k per row and plane of a tile; a k-step of the inner loop is two 16-byte chunks.
-template <typename T, bool SPLIT, int KB> struct How {
-  using E = __bf16;
-  static constexpr int PLANES = 3, UE = 8, KT = KB / 2, STEPS = KB / 32;
-};
-template <typename T, int KB> struct How<T, false, KB> {
-  using E = T;
-  static constexpr int PLANES = 1, UE = 16 / sizeof(T), KT = KB / sizeof(T), STEPS = KB / 32;
+template <typename M_, typename E_, int P_> struct Operand {
+  using M = M_;
+  using E = E_;
+  static constexpr int PLANES = P_, UE = 16 / sizeof(E);
 };
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
 
-// h, m, l of eight floats; `odd` becomes NaN if one of them has none (x - h is then infinite or NaN)
-__device__ __forceinline__ void split3(const float* x, b16x8& h, b16x8& m, b16x8& l, float& odd) {
+// The P bf16 of eight numbers, the first plane's where h points; `odd` becomes NaN if one of them has none (what is left is then infinite or NaN)
+template <int P, typename M> __device__ __forceinline__ void put_split(char* h, int plane, const M* x, float& odd) {
+  b16x8 part[P];
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
-    const f32x2 v = {x[i], x[i + 1]};
-    const b16x2 a = __builtin_convertvector(v, b16x2);
-    const unsigned ua = __builtin_bit_cast(unsigned, a);
-    const f32x2 r = {v[0] - __uint_as_float(ua << 16), v[1] - __uint_as_float(ua & 0xffff0000u)};
-    const b16x2 b = __builtin_convertvector(r, b16x2);
-    const unsigned ub = __builtin_bit_cast(unsigned, b);
-    const f32x2 q = {r[0] - __uint_as_float(ub << 16), r[1] - __uint_as_float(ub & 0xffff0000u)};
-    const b16x2 c = __builtin_convertvector(q, b16x2);
-    h[i] = a[0]; h[i + 1] = a[1]; m[i] = b[0]; m[i + 1] = b[1]; l[i] = c[0]; l[i + 1] = c[1];
-    odd = __builtin_fmaf(r[0], 0.f, odd);
-    odd = __builtin_fmaf(r[1], 0.f, odd);
+    f32x2 v = {(float)x[i], (float)x[i + 1]};
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+      const b16x2 a = __builtin_convertvector(v, b16x2);
+      part[q][i] = a[0]; part[q][i + 1] = a[1];
+      if (q + 1 == P) break;
+      const unsigned u = __builtin_bit_cast(unsigned, a);
+      v = f32x2{v[0] - __uint_as_float(u << 16), v[1] - __uint_as_float(u & 0xffff0000u)};
+      if (q == 0) odd = __builtin_fmaf(v[1], 0.f, __builtin_fmaf(v[0], 0.f, odd));
+    }
   }
+#pragma unroll
+  for (int q = 0; q < P; ++q) *(b16x8*)(h + q * plane) = part[q];
 }
 
 // LDS layout of one operand tile of R rows (m or n)
-template <typename T, bool SPLIT, int KB, bool KC, int R> struct Tile {
-  using H = How<T, SPLIT, KB>;
-  using E = typename H::E;
-  static constexpr int UE = H::UE, KT = H::KT, NU = R * KT / UE / 256;  // units per thread
+template <typename O, int KB, bool KC, int R> struct Tile {
+  using M = typename O::M;
+  using E = typename O::E;
+  static constexpr int UE = O::UE, KT = KB / (int)sizeof(E), NU = R * KT / UE / 256;  // units per thread
   static constexpr int STRIDE = KC ? KB : R * (int)sizeof(E) + 32;      // bytes; + 32: the four k rows a transposing read takes lie in other banks
-  static constexpr int PLANE = KC ? R * KB : KT * STRIDE, BYTES = H::PLANES * PLANE;
+  static constexpr int PLANE = KC ? R * KB : KT * STRIDE, BYTES = O::PLANES * PLANE;
   static constexpr int UPR = KC ? KT / UE : R / UE;                     // units per row of the tile (KC: m rows; else k rows)
 
   static __device__ __forceinline__ int swizzle(int row, int c) { return KB == 128 ? c ^ ((row >> 1) & 7) : c ^ ((row >> 2) & 3); }
   static __device__ __forceinline__ int row_of(int u) { return u / UPR; }
   static __device__ __forceinline__ int col_of(int u) { return u % UPR * UE; }
 
-  static __device__ __forceinline__ void put(char* s, int u, const Unit<T, UE>& x, float& odd) {
+  static __device__ __forceinline__ void put(char* s, int u, const Unit<M, UE>& x, float& odd) {
     const int row = u / UPR, c = u % UPR;
     char* at = s + (KC ? row * KB + (swizzle(row, c) << 4) : row * STRIDE + c * 16);
-    if constexpr (SPLIT) {
-      b16x8 h, m, l;
-      split3(x.e, h, m, l, odd);
-      *(b16x8*)at = h;
-      *(b16x8*)(at + PLANE) = m;
-      *(b16x8*)(at + 2 * PLANE) = l;
-    } else {
-      *(Unit<T, UE>*)at = x;
-    }
+    if constexpr (O::PLANES > 1) put_split<O::PLANES>(at, PLANE, x.e, odd);
+    else if constexpr (sizeof(M) == sizeof(E)) *(Unit<M, UE>*)at = x;
+    else *(f32x4*)at = f32x4{(float)x.e[0], (float)x.e[1], (float)x.e[2], (float)x.e[3]};
   }
 
   // the fragment of rows row0 .. row0 + 31 at k-step kk: lanes 0-31 hold chunk 2 kk, lanes 32-63 chunk 2 kk + 1 of k
@@ -142,16 +138,20 @@ template <typename T, bool SPLIT, int KB, bool KC, int R> struct Tile {
   }
 };
 
-// The sum over k in [kbeg, kend) for the tile at (m0, n0): 4 waves as 2 x 2, each BM / 2 x BN / 2 in 32 x 32 tiles.  -> true if (SPLIT) a number had no sum.
-template <typename T, bool SPLIT, int KB, int BUFFERS, bool AK, bool BK, int BM, int BN, bool GATED>
+// The sum over k in [kbeg, kend) for the tile at (m0, n0): 4 waves as 2 x 2, each BM / 2 x BN / 2 in 32 x 32 tiles.  -> true if a number is not the sum of its planes.
+template <typename OA, typename OB, int KB, int BUFFERS, bool AK, bool BK, int BM, int BN, bool GATED>
 __device__ __forceinline__ bool product_tile(const Product& p, long long m0, long long n0, long long kbeg, long long kend, char* lds, f32x16 (&acc)[BM / 64][BN / 64]) {
-  using H = How<T, SPLIT, KB>;
-  using TA = Tile<T, SPLIT, KB, AK, BM>;
-  using TB = Tile<T, SPLIT, KB, BK, BN>;
-  using E = typename H::E;
-  constexpr int UE = H::UE, KT = H::KT, WM = BM / 2, WN = BN / 2, MI = WM / 32, NI = WN / 32, HALF = WN / 2, BUF = TA::BYTES + TB::BYTES;
+  using TA = Tile<OA, KB, AK, BM>;
+  using TB = Tile<OB, KB, BK, BN>;
+  using E = typename OA::E;
+  using MA = typename OA::M;
+  using MB = typename OB::M;
+  constexpr int UE = OA::UE, KT = TA::KT, WM = BM / 2, WN = BN / 2, MI = WM / 32, NI = WN / 32, HALF = WN / 2, BUF = TA::BYTES + TB::BYTES;
+  constexpr int PA = OA::PLANES, PB = OB::PLANES, ORDER = PA > PB ? PA : PB, STEPS = KB / 32;
+  static_assert(sizeof(E) == sizeof(typename OB::E), "the matrix cores read both operands alike");
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wm = (wave >> 1) * WM, wn = (wave & 1) * WN;
-  const T *A = (const T*)p.A, *B = (const T*)p.B, *B2 = (const T*)p.B2;
+  const MA* A = (const MA*)p.A;
+  const MB *B = (const MB*)p.B, *B2 = (const MB*)p.B2;
   // Row-contiguous operands: no row's end cuts the tile, or rows are at least a unit apart, so that a unit read beyond a row's end stays inside the next row
   const bool in_a = AK || m0 + BM <= p.M, in_b = BK || n0 + BN <= p.N;
   const bool over_a = in_a || p.lda >= UE, over_b = in_b || (p.ldb >= UE && (p.kb2 == p.K || p.ldb2 >= UE));
@@ -160,8 +160,10 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
     return k1 <= kend && over_a && over_b && (in_a || k1 < p.K) && (in_b || (k1 < p.K && (k1 < p.kb2 || k0 >= p.kb2)));
   };
 
-  Unit<T, UE> ra[TA::NU], rb[TB::NU];
-  const T *pa[TA::NU], *pb[TB::NU];  // where this thread's units lie at the present k-tile
+  Unit<MA, UE> ra[TA::NU];
+  Unit<MB, UE> rb[TB::NU];
+  const MA* pa[TA::NU];
+  const MB* pb[TB::NU];  // where this thread's units lie at the present k-tile
   auto a_at = [&](int i, long long k0) {
     const int u = tid + i * 256, r = TA::row_of(u), c = TA::col_of(u);
     if constexpr (AK) { const long long m = m0 + r < p.M ? m0 + r : p.M - 1; return A + m * p.lda + k0 + c; }
@@ -229,22 +231,23 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
     for (int j = 0; j < NI; ++j) acc[i][j] = f32x16{};
   // Fragments of two k-steps: one is multiplied while the next comes from LDS.  (The scheduler would read into the registers of the step before and wait for
   // every read; the barriers keep it from that.)
-  constexpr int SETS = SPLIT ? 1 : 2;
-  typename Frag<E>::type fa[SETS][MI][H::PLANES], fb[SETS][NI][H::PLANES];
+  constexpr int SETS = ORDER > 1 ? 1 : 2;
+  typename Frag<E>::type fa[SETS][MI][PA], fb[SETS][NI][PB];
   auto fetch = [&](const char* sa, int kk) {
 #pragma unroll
-    for (int q = 0; q < H::PLANES; ++q) {
+    for (int q = 0; q < PA; ++q)
 #pragma unroll
       for (int i = 0; i < MI; ++i) fa[kk % SETS][i][q] = TA::frag(sa, q, wm + i * 32, kk, lane);
 #pragma unroll
+    for (int q = 0; q < PB; ++q)
+#pragma unroll
       for (int j = 0; j < NI; ++j) fb[kk % SETS][j][q] = TB::frag(sa + TA::BYTES, q, wn + j * 32, kk, lane);
-    }
   };
   auto multiply = [&](int kk) {
 #pragma unroll
-    for (int qa = 0; qa < H::PLANES; ++qa)
+    for (int qa = 0; qa < PA; ++qa)
 #pragma unroll
-      for (int qb = 0; qa + qb < H::PLANES; ++qb)
+      for (int qb = 0; qb < PB && qa + qb < ORDER; ++qb)
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
@@ -270,11 +273,11 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
       fetch(sa, 0);
     }
 #pragma unroll
-    for (int kk = 0; kk < H::STEPS; ++kk) {
+    for (int kk = 0; kk < STEPS; ++kk) {
       if constexpr (SETS == 1) {
         if (kk) fetch(sa, kk);
       } else {
-        if (kk + 1 < H::STEPS) fetch(sa, kk + 1);
+        if (kk + 1 < STEPS) fetch(sa, kk + 1);
         __builtin_amdgcn_sched_barrier(0);
       }
       multiply(kk);
@@ -293,32 +296,34 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
 // ahead 235), nor was a loop without bounds checks (220), other orders of its instructions (220 .. 224) or a wave priority (220); 256 x 256 tiles, one workgroup
 // per CU, gain where k is long (8192 x 8192 x 8192: 1040 instead of 1140) and lose where it is not, since nothing hides their ends (24576 x 1024 x 1024: 100
 // instead of 74).  The library's product takes 190 in the first and 52 in the last.
-template <typename T, int BM_, int BN_> struct Shape {
+template <typename TA, typename T, int BM_, int BN_> struct Shape {
   static constexpr int BM = BM_, BN = BN_, KB = BM_ == 256 ? 64 : 128, BUFFERS = BM_ == 128 ? 1 : 2;
-  static constexpr bool SPLIT = false;
+  using A = Operand<T, T, 1>;
+  using B = Operand<T, T, 1>;
 };
-template <int BM_, int BN_> struct Shape<float, BM_, BN_> {
+template <int BM_, int BN_> struct Shape<float, float, BM_, BN_> {
   static constexpr int BM = BM_, BN = BN_, KB = 64, BUFFERS = BM_ == 64 ? 2 : 1;
-  static constexpr bool SPLIT = true;
+  using A = Operand<float, __bf16, 3>;
+  using B = Operand<float, __bf16, 3>;
+};
+// dz: one buffer of 32 k is 4 % slower, one of 64 k 2 % (24576 x 1024 x 1024 bf16 dx with its slope kernel 207, 213, 208 us)
+template <typename T, int BM_, int BN_> struct Shape<float, T, BM_, BN_> {
+  static constexpr int BM = BM_, BN = BN_, KB = 64, BUFFERS = 2;
+  using A = Operand<float, __bf16, 2>;
+  using B = Operand<T, __bf16, Elem<T>::DTYPE == MJLAB_DTYPE_BF16 ? 1 : 2>;
 };
 
-template <typename T, bool AK, bool BK, int BM, int BN, int EPI> struct ProductLds {
-  using S = Shape<T, BM, BN>;
-  static constexpr int TILES = S::BUFFERS * (Tile<T, S::SPLIT, S::KB, AK, BM>::BYTES + Tile<T, S::SPLIT, S::KB, BK, BN>::BYTES);
-  static constexpr int AGAIN = Tile<T, false, 64, AK, BM>::BYTES + Tile<T, false, 64, BK, BN>::BYTES;  // (float's second try)
+template <typename TA, typename T, bool AK, bool BK, int BM, int BN, int EPI> struct ProductLds {
+  using S = Shape<TA, T, BM, BN>;
+  static constexpr int TILES = S::BUFFERS * (Tile<typename S::A, S::KB, AK, BM>::BYTES + Tile<typename S::B, S::KB, BK, BN>::BYTES);
+  static constexpr int AGAIN = sizeof(TA) == 4 ? Tile<Operand<TA, float, 1>, 64, AK, BM>::BYTES + Tile<Operand<T, float, 1>, 64, BK, BN>::BYTES : 0;  // (the second try)
   static constexpr int EPILOGUE = 4 * 32 * (BN / 2 + 4) * 4;
   static constexpr int BYTES = TILES > EPILOGUE ? (TILES > AGAIN ? TILES : AGAIN) : (EPILOGUE > AGAIN ? EPILOGUE : AGAIN);
 };
 
-// What rounding x to T left, as T (a second plane of dz); 0 where nothing can be left
-template <typename T> __device__ __forceinline__ T rest(float x, T h) {
-  const float r = x - (float)h;
-  return (T)(__builtin_fabsf(r) < 1e38f ? r : 0.f);
-}
-
 // (Three workgroups of 128 x 128 per CU need 168 registers: the activations' branches are held to that, or all pay, 83 -> 94 us at 24576 x 512 x 512 float.)
-template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __launch_bounds__(256, BK && BM == 128 ? 3 : 2) void k_product(const Product p) {
-  using S = Shape<T, BM, BN>;
+template <typename TA, typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __launch_bounds__(256, BK && BM == 128 ? 3 : 2) void k_product(const Product p) {
+  using S = Shape<TA, T, BM, BN>;
   constexpr int V = Elem<T>::VEC, WM = BM / 2, WN = BN / 2, MI = WM / 32, NI = WN / 32;
   constexpr bool SLOPE = EPI == EPI_SLOPE, GATED = EPI == EPI_GATED || SLOPE;
   constexpr int BNO = GATED ? BN / 2 : BN, HALF = WN / 2;  // output columns per workgroup; a gated wave owns HALF columns of both products
@@ -332,9 +337,9 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
   const long long kbeg = blockIdx.y * p.ksplit, kend = kbeg + p.ksplit < p.K ? kbeg + p.ksplit : p.K;
 
   f32x16 acc[MI][NI];
-  const bool odd = product_tile<T, S::SPLIT, S::KB, S::BUFFERS, AK, BK, BM, BN, GATED>(p, m0, n0, kbeg, kend, lds, acc);
-  if constexpr (S::SPLIT) {
-    if (__syncthreads_or(odd)) product_tile<T, false, 64, 1, AK, BK, BM, BN, GATED>(p, m0, n0, kbeg, kend, lds, acc);
+  const bool odd = product_tile<typename S::A, typename S::B, S::KB, S::BUFFERS, AK, BK, BM, BN, GATED>(p, m0, n0, kbeg, kend, lds, acc);
+  if constexpr (sizeof(TA) == 4) {
+    if (__syncthreads_or(odd)) product_tile<Operand<TA, float, 1>, Operand<T, float, 1>, 64, 1, AK, BK, BM, BN, GATED>(p, m0, n0, kbeg, kend, lds, acc);
   }
 
   // C leaves through LDS, 32 rows of the wave's own at a time: an accumulator holds one column per lane, memory wants 16 bytes of a row.
@@ -403,9 +408,9 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
         for (int e = 0; e < OV; ++e) out.e[e] = (T)x[e];
         store_part((T*)base + m * ld + n, out, left);
       };
-      auto put_float = [&](void* base, int q, long long m, const float (&x)[OV]) {
+      auto put_float = [&](void* base, long long ld, int q, long long m, const float (&x)[OV]) {
 #pragma unroll
-        for (int e = 0; e < OV; e += 4) store_part((float*)base + m * p.N + n + e, Chunk<float>{{x[e], x[e + 1], x[e + 2], x[e + 3]}}, left - e);
+        for (int e = 0; e < OV; e += 4) store_part((float*)base + m * ld + n + e, Chunk<float>{{x[e], x[e + 1], x[e + 2], x[e + 3]}}, left - e);
       };
       if constexpr (SLOPE) {
         with_act(p.act, [&](auto act) {
@@ -422,19 +427,13 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
               sum_up[e] += there ? u[q][e] : 0.f;
             }
         });
-        rows([&](int q, long long m) { put((T*)p.y + p.N, p.ldy, q, m, u[q]); });
-        if (p.low) {
-          rows([&](int q, long long m) {
-            float x[OV], y[OV];
-#pragma unroll
-            for (int e = 0; e < OV; ++e) { x[e] = (float)rest<T>(v[q][e], (T)v[q][e]); y[e] = (float)rest<T>(u[q][e], (T)u[q][e]); }
-            put((T*)p.y + p.low, p.ldy, q, m, x);
-            put((T*)p.y + p.low + p.N, p.ldy, q, m, y);
-          });
-        }
+        rows([&](int q, long long m) {
+          put_float(p.y, p.ldy, q, m, v[q]);
+          put_float((float*)p.y + p.N, p.ldy, q, m, u[q]);
+        });
       } else if constexpr (EPI != EPI_STORE) {
         if (p.z) rows([&](int q, long long m) {
-          if (GATED || p.z_float) put_float(p.z, q, m, v[q]);
+          if (GATED || p.z_float) put_float(p.z, p.N, q, m, v[q]);
           else put(p.z, p.N, q, m, v[q]);
         });
         with_act(p.act, [&](auto act) {
@@ -444,7 +443,7 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
             for (int e = 0; e < OV; ++e) v[q][e] = act_value<decltype(act)::value, sizeof(T) == 4>(v[q][e]);
         });
         if constexpr (GATED) {
-          if (p.z_up) rows([&](int q, long long m) { put_float(p.z_up, q, m, u[q]); });
+          if (p.z_up) rows([&](int q, long long m) { put_float(p.z_up, p.N, q, m, u[q]); });
 #pragma unroll
           for (int q = 0; q < PASSES; ++q)
 #pragma unroll
@@ -456,7 +455,7 @@ template <typename T, bool AK, bool BK, int BM, int BN, int EPI> __global__ __la
             for (int e = 0; e < OV; ++e) v[q][e] += (float)res[q].e[e];
         }
       }
-      rows([&](int q, long long m) { put(p.y, p.ldy, q, m, v[q]); });
+      if constexpr (!SLOPE) rows([&](int q, long long m) { put(p.y, p.ldy, q, m, v[q]); });
     }
   }
   if constexpr (SLOPE) {
@@ -513,14 +512,13 @@ template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_join_
   ((T*)p.y)[m * p.ldy + c] = (T)v;
 }
 
-// dz (rows, out | 2 out) from dy and the stored sums, and this row block's column sums for the bias gradient.  low: columns to a second plane, what the rounding of
-// dz left (0: not wanted).
+// dz (rows, out | 2 out), floats, from dy and the stored sums, and this row block's column sums for the bias gradient.
 // 256 threads: 32 chunk columns x 8 rows, four rows of each thread in flight, over SLOPE_ROWS rows; workgroups: row blocks x `colblocks`.
 // dz NULL: column sums of dy alone.  FROM: what is stored is the layer's output.  WIDE: the sums are floats.  Bound by memory: dense two reads and a write, gated
 // three and two.
 #define SLOPE_ROWS 64
-template <typename T, bool GATED, bool FROM, bool WIDE> __global__ __launch_bounds__(256) void k_layer_slope(const T* dy, long long ld_dy, const void* z, const float* z_up, T* dz,
-                                                                                                   long long pitch, long long low, float* sums, long long rows, long long out, unsigned colblocks, int act) {
+template <typename T, bool GATED, bool FROM, bool WIDE> __global__ __launch_bounds__(256) void k_layer_slope(const T* dy, long long ld_dy, const void* z, const float* z_up, float* dz,
+                                                                                                   long long pitch, float* sums, long long rows, long long out, unsigned colblocks, int act) {
   static_assert(WIDE || !GATED, "a gated layer's sums are floats");
   constexpr int V = Elem<T>::VEC, NS = GATED ? 2 : 1, ROWS = GATED ? 1 : 2;
   __shared__ float part[NS][8][32 * V];
@@ -552,32 +550,27 @@ template <typename T, bool GATED, bool FROM, bool WIDE> __global__ __launch_boun
     for (int q = 0; q < ROWS; ++q) {
       const long long m = r0 + i + 8 * q;
       if (slope) {
-        Chunk<T> o, lo, lu;  // du; what the roundings left
+        float o[V], o_up[GATED ? V : 1];
         with_act(act, [&](auto a) {
           constexpr int ACT = decltype(a)::value;
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const float x = WIDE ? z0[WIDE ? q : 0][e] : (float)g[q].e[e], t = (float)d[q].e[e];
-            float v = t * (FROM ? act_slope_out<ACT>(x) : act_slope<ACT, sizeof(T) == 4>(x));
+            o[e] = t * (FROM ? act_slope_out<ACT>(x) : act_slope<ACT, sizeof(T) == 4>(x));
             if constexpr (GATED) {
-              v *= z1[q][e];
-              const float w = t * act_value<ACT, sizeof(T) == 4>(x);
-              s[NS - 1][e] += w;
-              o.e[e] = (T)w;
-              lu.e[e] = rest<T>(w, o.e[e]);
+              o[e] *= z1[q][e];
+              o_up[e] = t * act_value<ACT, sizeof(T) == 4>(x);
+              s[NS - 1][e] += o_up[e];
             }
-            s[0][e] += v;
-            d[q].e[e] = (T)v;
-            lo.e[e] = rest<T>(v, d[q].e[e]);
+            s[0][e] += o[e];
           }
         });
         if (m < rows && left > 0) {
-          T* at = dz + m * pitch + n;
-          store_part(at, d[q], left);
-          if constexpr (GATED) store_part(at + out, o, left);
-          if (low) {
-            store_part(at + low, lo, left);
-            if constexpr (GATED) store_part(at + low + out, lu, left);
+          float* at = dz + m * pitch + n;
+#pragma unroll
+          for (int e = 0; e < V; e += 4) {
+            store_part(at + e, Chunk<float>{{o[e], o[e + 1], o[e + 2], o[e + 3]}}, left - e);
+            if constexpr (GATED) store_part(at + out + e, Chunk<float>{{o_up[e], o_up[e + 1], o_up[e + 2], o_up[e + 3]}}, left - e);
           }
         }
       } else {

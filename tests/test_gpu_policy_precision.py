@@ -1,0 +1,126 @@
+"""What the 16-bit layers keep between their forward and their gradients: nothing of it is rounded to 16 bits, and none of it leaves the range of a float.
+
+Bounds, element by element, from the sizes alone (u: half a step of the type; u32 = 2^-24).  The sums before the activation are floats: off by at most
+(k + 2) u32 sum |x w|, and the slope by that (Lipschitz with constant <= 1) and its evaluation, 16 u32 (1 + |z|).  dz is a float, formed with at most four
+roundings.  The matrix cores read it as two bfloat16, which leaves at most 2^-8 of 2^-8 of it; a float16 that it meets is two bfloat16 as well (exactly), and the
+product of the two second parts, another 2^-16, is not formed.  Three such products per term are summed in 32 bits, in any order.  Then one rounding to the type."""
+
+import pytest
+import torch
+from test_gpu_policy_layers import TINY, U, U32, act, close, rand
+
+pytestmark = pytest.mark.gpu
+
+HALVES = [torch.float16, torch.bfloat16]
+READ = {torch.float16: 2.0**-15, torch.bfloat16: 2.0**-16}
+
+
+def check_gradients(m, k, n, dtype, name, gated, seed, dy_scale=1.0, x_scale=1.0, w_scale=1.0, shift=0.0, shift_up=0.0, want_bias=True, dy=None):
+  from mjlab_amd import policy_ops
+
+  gen = torch.Generator(device="cuda").manual_seed(seed)
+  u, tiny, read = U[dtype], TINY[dtype], READ[dtype]
+  x, w = rand(gen, m, k, dtype=dtype, scale=x_scale), rand(gen, n, k, dtype=dtype, scale=w_scale * k**-0.5)
+  b = (rand(gen, n, dtype=torch.float32, scale=0.3) + shift).to(dtype)
+  wu, bu = (rand(gen, n, k, dtype=dtype, scale=w_scale * k**-0.5), (rand(gen, n, dtype=torch.float32, scale=0.3) + shift_up).to(dtype)) if gated else (None, None)
+  dy = rand(gen, m, n, dtype=torch.float32).mul(dy_scale).to(dtype) if dy is None else dy(gen)
+  leaves = [t for t in (x, w, wu, *((b, bu) if want_bias else ())) if t is not None]
+  for t in leaves:
+    t.requires_grad_(True)
+  y = policy_ops.gated(x, w, wu, b, bu, activation=name) if gated else policy_ops.dense(x, w, b, activation=name)
+  grads = dict(zip([id(t) for t in leaves], torch.autograd.grad(y, leaves, dy), strict=True))
+  with torch.no_grad():
+    X, DY = x.double(), dy.double()
+
+    def sums(wt, bt):
+      return X @ wt.double().t() + bt.double(), (k + 2) * U32 * (X.abs() @ wt.double().abs().t() + bt.double().abs())
+
+    z, ez = sums(w, b)
+    f, df = act(z, name)
+    ef, edf = 1.13 * ez + 16 * U32 * (1 + z.abs()), ez + 16 * U32 * (1 + z.abs()) + ((z.abs() <= ez).double() if name == "relu" else 0)
+    if gated:
+      up, eu = sums(wu, bu)
+      dz, edz = [DY * up * df, DY * f], [DY.abs() * (edf * (up.abs() + eu) + df.abs() * eu), DY.abs() * ef]
+    else:
+      dz, edz = [DY * df], [DY.abs() * edf]
+    edb = [d + 4 * U32 * (q.abs() + d) for q, d in zip(dz, edz, strict=True)]
+    edz = [d + read * (q.abs() + d) for q, d in zip(dz, edb, strict=True)]
+    ws = [w, wu] if gated else [w]
+    dx = sum(d @ q.double() for d, q in zip(dz, ws, strict=True))
+    ex = sum(d @ q.double().abs() + (6 * n + 2) * U32 * ((z_.abs() + d) @ q.double().abs()) for z_, d, q in zip(dz, edz, ws, strict=True))
+    close(grads[id(x)], dx, ex + u * (dx.abs() + ex) + tiny, "dx")
+    for z_, d, e, q, bias in zip(dz, edz, edb, ws, (b, bu), strict=False):
+      dw, ew = z_.t() @ X, d.t() @ X.abs() + (3 * m + 2) * U32 * ((z_.abs() + d).t() @ X.abs())
+      close(grads[id(q)], dw, ew + u * (dw.abs() + ew) + tiny, "dw")
+      if want_bias:
+        db, eb = z_.sum(0), e.sum(0) + (m + 2) * U32 * (z_.abs() + e).sum(0)
+        close(grads[id(bias)], db, eb + u * (db.abs() + eb) + tiny, "db")
+    return dz
+
+
+SIZES = [(70, 40, 83), (5, 1999, 333), (1203, 1001, 1003)]  # small, few rows (split sums), more than 2^28 multiplications
+
+
+@pytest.mark.parametrize("m,k,n", [(70, 40, 83), (6007, 70, 33), (1203, 1001, 1003)])
+@pytest.mark.parametrize("name,gated", [("tanh", False), ("silu", False), ("silu", True)])
+@pytest.mark.parametrize("scale", [2.0**-14, 2.0**-20])
+def test_small_upstream_gradients_in_fp16(m, k, n, name, gated, scale):
+  """As of a mean over many rows.  Weights of 16 keep dx inside fp16's normal numbers."""
+  check_gradients(m, k, n, torch.float16, name, gated, seed=1, dy_scale=scale, x_scale=1 / 16, w_scale=16.0)
+
+
+@pytest.mark.parametrize("m,k,n", SIZES)
+def test_dz_of_a_gated_layer_beyond_fp16(m, k, n):
+  """dg = dy * up * slope: about 1e5 and up to several 1e5, while dx and dw are finite."""
+  dz = check_gradients(m, k, n, torch.float16, "silu", True, seed=2, dy_scale=200.0, x_scale=2.0**-9, w_scale=2.0**-9 * k**0.5, shift_up=1000.0, want_bias=False)
+  assert dz[0].abs().max() > 65504
+
+
+@pytest.mark.parametrize("m,k,n", SIZES)
+def test_dz_of_a_dense_layer_beyond_fp16(m, k, n):
+  """The slope of gelu is 1.13 at 1.41: dy = +-62000 gives dz = +-70000."""
+  dz = check_gradients(m, k, n, torch.float16, "gelu", False, seed=3, x_scale=2.0**-9, w_scale=2.0**-9 * k**0.5, shift=1.41, want_bias=False,
+                       dy=lambda gen: 62000 * (rand(gen, m, n, dtype=torch.float32).sign()).half())
+  assert dz[0].abs().max() > 65504
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("name,gated", [("relu", False), ("silu", False), ("gelu", True)])
+@pytest.mark.parametrize("m,k,n", [*SIZES, (2101, 45, 2103), (64, 1031, 517), (1, 1, 1), (131, 257, 65)])
+def test_gradients(m, k, n, name, gated, dtype):
+  check_gradients(m, k, n, dtype, name, gated, seed=4)
+
+
+def only_rounded(got, want, e2, what):
+  """The 2-norm of the error is that of rounding the exact result once, and what the roundings before it leave: `e2`, the expected square of that for each output,
+  in all, with a factor of 4 for the spread."""
+  own, err = (want.to(got.dtype).double() - want).norm(), (got.double() - want).norm()
+  assert err <= own + 4 * e2.sum().sqrt(), f"{what}: off by {float(err / want.norm()):.3g} of its norm, rounding alone by {float(own / want.norm()):.3g}"
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("name,gated", [("elu", False), ("silu", False), ("gelu", False), ("tanh", False), ("silu", True)])
+@pytest.mark.parametrize("m,k,n", [(1203, 1001, 1003), (701, 333, 405)])
+def test_gradients_are_as_exact_as_their_own_rounding(m, k, n, name, gated, dtype):
+  """Roundings are independent, so a sum of terms t_i that are each off by at most r |t_i| is off by r sqrt(sum t_i^2) in the mean, and one of n additions in 32 bits
+  by sqrt(n) u32 times the same (its partial sums are no larger in the mean)."""
+  from mjlab_amd import policy_ops
+
+  gen = torch.Generator(device="cuda").manual_seed(5)
+  x, w, wu = rand(gen, m, k, dtype=dtype), *(rand(gen, n, k, dtype=dtype, scale=k**-0.5) for _ in range(2))
+  dy = rand(gen, m, n, dtype=dtype)
+  leaves = [t.requires_grad_(True) for t in ((x, w, wu) if gated else (x, w))]
+  y = policy_ops.gated(*leaves, activation=name) if gated else policy_ops.dense(*leaves, activation=name)
+  grads = torch.autograd.grad(y, leaves, dy)
+  with torch.no_grad():
+    X, DY, ws = x.double(), dy.double(), [t.double() for t in leaves[1:]]
+    z = [X @ q.t() for q in ws]
+    ez = [k**0.5 * U32 * ((X * X) @ (q * q).t()).sqrt() for q in ws]
+    f, df = act(z[0], name)
+    edf = ez[0] + 16 * U32 * (1 + z[0].abs())
+    dz = [DY * z[1] * df, DY * f] if gated else [DY * df]
+    edz = [DY.abs() * (edf * z[1].abs() + df.abs() * ez[1]), DY.abs() * edf * 1.13] if gated else [DY.abs() * edf]
+    off = [(READ[dtype] + 4 * U32) * q.abs() + d for q, d in zip(dz, edz, strict=True)]
+    only_rounded(grads[0], sum(d @ q for d, q in zip(dz, ws, strict=True)), sum((o * o + 6 * n * U32**2 * d * d) @ (q * q) for o, d, q in zip(off, dz, ws, strict=True)), "dx")
+    for g, d, o in zip(grads[1:], dz, off, strict=True):
+      only_rounded(g, d.t() @ X, (o * o + 3 * m * U32**2 * d * d).t() @ (X * X), "dw")
