@@ -29,10 +29,9 @@ const char* mjlab_policy_last_error(void);
  *   gated (w_up != NULL):  y = act(x w^T + b) * (x w_up^T + b_up)
  * x (rows, in), w and w_up (out, in), b and b_up (out) or NULL, r (rows, out) or NULL (dense only), y (rows, out); the innermost stride of
  * each is 1, ld* is the distance of rows.  All arrays hold `dtype`; sums are held in 32 bits and each output is rounded once.
- * z / z_up (rows, out), dense, or NULL: the sums before the activation, which the backward pass reads: floats for a gated layer (z and z_up
- * alike), whose gradients multiply them; of `dtype` or floats for a dense one (floats where a rounding of z would show in the slope: tanh and sigmoid,
- * whose slope falls by exp(-2 |z|) and exp(-|z|)).  z_bytes is their element size.  z_is_y (backward pass only): z points to the dense
- * output y instead, which determines the slope of relu, elu, tanh and sigmoid where no residual was added. */
+ * z / z_up (rows, out), dense, or NULL: the sums before the activation, floats whatever `dtype` is (z_bytes, their element size, is 4), which the
+ * backward pass reads.  z_is_y (backward pass of a float32 layer only): z points to the dense output y instead, which determines the slope of relu,
+ * elu, tanh and sigmoid where no residual was added. */
 typedef struct mjlab_layer {
   int dtype, act, z_is_y, z_bytes;
   long long rows, in, out;

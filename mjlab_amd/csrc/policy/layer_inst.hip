@@ -118,7 +118,7 @@ Product forward_product(const mjlab_layer_t* f) {
   Product p = {};
   p.A = f->x; p.lda = f->ldx; p.B = f->w; p.ldb = f->ldw; p.B2 = f->w_up; p.ldb2 = f->ldw_up;
   p.M = f->rows; p.N = p.nb2 = f->out; p.K = p.kb2 = p.ksplit = f->in;
-  p.act = f->act; p.z_float = f->z_bytes == 4; p.b = f->b; p.b_up = f->b_up; p.r = f->r; p.ldr = f->ldr; p.y = f->y; p.ldy = f->ldy; p.z = f->z; p.z_up = f->z_up;
+  p.act = f->act; p.b = f->b; p.b_up = f->b_up; p.r = f->r; p.ldr = f->ldr; p.y = f->y; p.ldy = f->ldy; p.z = (float*)f->z; p.z_up = (float*)f->z_up;
   return p;
 }
 
@@ -205,11 +205,8 @@ hipError_t POLICY_NAME(mjlab_launch_layer_backward)(const mjlab_layer_grad_t* g,
     constexpr int V = Elem<T>::VEC;
     const long long colblocks = (f.out + 32 * V - 1) / (32 * V);
     if (colblocks * q.blocks > MAX_BLOCKS) return hipErrorInvalidValue;
-    auto kern = q.gated ? k_layer_slope<T, true, false, true>
-                : f.z_is_y ? k_layer_slope<T, false, true, false>
-                : sizeof(T) == 2 && f.z_bytes == 4 ? k_layer_slope<T, false, false, sizeof(T) == 2>
-                                                   : k_layer_slope<T, false, false, false>;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(colblocks * q.blocks)), dim3(256), 0, st, (const T*)g->dy, g->ld_dy, f.z, (const float*)f.z_up, q.slope ? dz : nullptr, q.ns * f.out, sums, f.rows, f.out, (unsigned)colblocks, f.act);
+    auto kern = q.gated ? k_layer_slope<T, true, false> : sizeof(T) == 4 && f.z_is_y ? k_layer_slope<T, false, sizeof(T) == 4> : k_layer_slope<T, false, false>;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(colblocks * q.blocks)), dim3(256), 0, st, (const T*)g->dy, g->ld_dy, (const float*)f.z, (const float*)f.z_up, q.slope ? dz : nullptr, q.ns * f.out, sums, f.rows, f.out, (unsigned)colblocks, f.act);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   if (q.sums) {

@@ -36,9 +36,7 @@ int mjlab_sizeof_layer(void) { return (int)sizeof(mjlab_layer_t); }
 int mjlab_sizeof_layer_grad(void) { return (int)sizeof(mjlab_layer_grad_t); }
 
 static int check_z(const mjlab_layer_t& f) {
-  if ((f.z || f.z_up) && f.z_bytes != 4 && (f.w_up || f.dtype == MJLAB_DTYPE_F32 || f.z_bytes != 2)) return fail(-2, "layer: z_bytes: a gated layer's sums are floats, a dense layer's floats or of its dtype");
-  if (f.z && f.z_is_y && f.z_bytes != (f.dtype == MJLAB_DTYPE_F32 ? 4 : 2)) return fail(-2, "layer: z_bytes: y is of the layer's dtype");
-  return 0;
+  return (f.z || f.z_up) && f.z_bytes != 4 ? fail(-2, "layer: z_bytes: the sums before the activation are floats") : 0;
 }
 
 int mjlab_layer_recomputes(const mjlab_layer_t* f) {
@@ -81,7 +79,7 @@ int mjlab_layer_backward(const mjlab_layer_grad_t* g, void* stream) {
   if (!g->dy) return fail(-2, "layer_backward: null dy");
   const bool again = gated && !g->f.z && !g->f.z_up && mjlab_layer_recomputes(&g->f);
   if (!again && (gated || g->f.act != MJLAB_ACT_NONE) && !g->f.z) return fail(-2, "layer_backward: the sums before the activation (z) are missing");
-  if (g->f.z_is_y && (gated || !slope_from_output(g->f.act))) return fail(-2, "layer_backward: z_is_y: the output does not determine this layer's slope");
+  if (g->f.z_is_y && (gated || g->f.dtype != MJLAB_DTYPE_F32 || !slope_from_output(g->f.act))) return fail(-2, "layer_backward: z_is_y: the output does not determine this layer's slope");
   if (gated && !again && !g->f.z_up) return fail(-2, "layer_backward: z_up is missing");
   if ((rc = check_z(g->f))) return rc;
   if (gated && ((g->dw != nullptr) != (g->dw_up != nullptr) || (g->db != nullptr) != (g->db_up != nullptr))) return fail(-2, "layer_backward: dw / dw_up and db / db_up come together");

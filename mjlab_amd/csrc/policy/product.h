@@ -30,9 +30,10 @@ struct Product {
   long long M, N, K, kb2;      // kb2: where B's rows end and B2's begin (K where there is no B2)
   long long nb2;               // the same for a k-contiguous B outside EPI_GATED (N where there is no B2)
   long long ksplit;            // k elements per blockIdx.y
-  int act, z_float;            // z_float: z holds floats (a gated layer's always)
+  int act;
   const void *b, *b_up, *r;    // the epilogue's
-  void *y, *z, *z_up;
+  void* y;
+  float *z, *z_up;
   long long ldr, ldy;
   float* partial;              // EPI_PARTIAL: (splits, M, N); EPI_SLOPE: column sums of y, (2 M / BM, 2 N), or NULL
                                // EPI_SLOPE: a gated layer's sums formed again; r = dy, y = [dg | du] as floats
@@ -408,9 +409,9 @@ template <typename TA, typename T, bool AK, bool BK, int BM, int BN, int EPI> __
         for (int e = 0; e < OV; ++e) out.e[e] = (T)x[e];
         store_part((T*)base + m * ld + n, out, left);
       };
-      auto put_float = [&](void* base, long long ld, int q, long long m, const float (&x)[OV]) {
+      auto put_float = [&](float* base, long long ld, int q, long long m, const float (&x)[OV]) {
 #pragma unroll
-        for (int e = 0; e < OV; e += 4) store_part((float*)base + m * ld + n + e, Chunk<float>{{x[e], x[e + 1], x[e + 2], x[e + 3]}}, left - e);
+        for (int e = 0; e < OV; e += 4) store_part(base + m * ld + n + e, Chunk<float>{{x[e], x[e + 1], x[e + 2], x[e + 3]}}, left - e);
       };
       if constexpr (SLOPE) {
         with_act(p.act, [&](auto act) {
@@ -428,14 +429,11 @@ template <typename TA, typename T, bool AK, bool BK, int BM, int BN, int EPI> __
             }
         });
         rows([&](int q, long long m) {
-          put_float(p.y, p.ldy, q, m, v[q]);
+          put_float((float*)p.y, p.ldy, q, m, v[q]);
           put_float((float*)p.y + p.N, p.ldy, q, m, u[q]);
         });
       } else if constexpr (EPI != EPI_STORE) {
-        if (p.z) rows([&](int q, long long m) {
-          if (GATED || p.z_float) put_float(p.z, p.N, q, m, v[q]);
-          else put(p.z, p.N, q, m, v[q]);
-        });
+        if (p.z) rows([&](int q, long long m) { put_float(p.z, p.N, q, m, v[q]); });
         with_act(p.act, [&](auto act) {
 #pragma unroll
           for (int q = 0; q < PASSES; ++q)
@@ -499,14 +497,11 @@ template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_join_
     if constexpr (GATED) u += p.partial[(k * p.M + m) * width + p.N + c];
   }
   if (p.b) v += (float)((const T*)p.b)[c];
-  if (p.z) {
-    if (GATED || p.z_float) ((float*)p.z)[i] = v;
-    else ((T*)p.z)[i] = (T)v;
-  }
+  if (p.z) p.z[i] = v;
   with_act(p.act, [&](auto act) { v = act_value<decltype(act)::value, sizeof(T) == 4>(v); });
   if constexpr (GATED) {
     if (p.b_up) u += (float)((const T*)p.b_up)[c];
-    if (p.z_up) ((float*)p.z_up)[i] = u;
+    if (p.z_up) p.z_up[i] = u;
     v *= u;
   } else if (p.r) v += (float)((const T*)p.r)[m * p.ldr + c];
   ((T*)p.y)[m * p.ldy + c] = (T)v;
@@ -514,12 +509,10 @@ template <typename T, bool GATED> __global__ __launch_bounds__(256) void k_join_
 
 // dz (rows, out | 2 out), floats, from dy and the stored sums, and this row block's column sums for the bias gradient.
 // 256 threads: 32 chunk columns x 8 rows, four rows of each thread in flight, over SLOPE_ROWS rows; workgroups: row blocks x `colblocks`.
-// dz NULL: column sums of dy alone.  FROM: what is stored is the layer's output.  WIDE: the sums are floats.  Bound by memory: dense two reads and a write, gated
-// three and two.
+// dz NULL: column sums of dy alone.  FROM: what is stored is the output of a float layer.  Bound by memory: dense two reads and a write, gated three and two.
 #define SLOPE_ROWS 64
-template <typename T, bool GATED, bool FROM, bool WIDE> __global__ __launch_bounds__(256) void k_layer_slope(const T* dy, long long ld_dy, const void* z, const float* z_up, float* dz,
-                                                                                                   long long pitch, float* sums, long long rows, long long out, unsigned colblocks, int act) {
-  static_assert(WIDE || !GATED, "a gated layer's sums are floats");
+template <typename T, bool GATED, bool FROM> __global__ __launch_bounds__(256) void k_layer_slope(const T* dy, long long ld_dy, const float* z, const float* z_up, float* dz, long long pitch,
+                                                                                                  float* sums, long long rows, long long out, unsigned colblocks, int act) {
   constexpr int V = Elem<T>::VEC, NS = GATED ? 2 : 1, ROWS = GATED ? 1 : 2;
   __shared__ float part[NS][8][32 * V];
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -528,23 +521,21 @@ template <typename T, bool GATED, bool FROM, bool WIDE> __global__ __launch_boun
   float s[NS][V] = {};
   const bool slope = dz && (GATED || act != MJLAB_ACT_NONE);
   for (int i = ty; i < SLOPE_ROWS && r0 + i < rows; i += 8 * ROWS) {
-    Chunk<T> d[ROWS], g[ROWS];
-    float z0[WIDE ? ROWS : 1][V], z1[GATED ? ROWS : 1][V];
+    Chunk<T> d[ROWS];
+    float z0[ROWS][V], z1[GATED ? ROWS : 1][V];
 #pragma unroll
     for (int q = 0; q < ROWS; ++q) {
       const long long m = r0 + i + 8 * q, have = m < rows ? left : 0;
       d[q] = load_part(dy + m * ld_dy + n, have);
-      if constexpr (WIDE) {
 #pragma unroll
-        for (int e = 0; e < V; e += 4) {
-          const Chunk<float> x = load_part((const float*)z + m * out + n + e, slope ? have - e : 0), y = load_part(z_up + m * out + n + e, GATED ? have - e : 0);
+      for (int e = 0; e < V; e += 4) {
+        const Chunk<float> x = load_part(z + m * out + n + e, slope ? have - e : 0), y = load_part(z_up + m * out + n + e, GATED ? have - e : 0);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            z0[q][e + k] = x.e[k];
-            if constexpr (GATED) z1[q][e + k] = y.e[k];
-          }
+        for (int k = 0; k < 4; ++k) {
+          z0[q][e + k] = x.e[k];
+          if constexpr (GATED) z1[q][e + k] = y.e[k];
         }
-      } else if (slope) g[q] = load_part((const T*)z + m * out + n, have);
+      }
     }
 #pragma unroll
     for (int q = 0; q < ROWS; ++q) {
@@ -555,7 +546,7 @@ template <typename T, bool GATED, bool FROM, bool WIDE> __global__ __launch_boun
           constexpr int ACT = decltype(a)::value;
 #pragma unroll
           for (int e = 0; e < V; ++e) {
-            const float x = WIDE ? z0[WIDE ? q : 0][e] : (float)g[q].e[e], t = (float)d[q].e[e];
+            const float x = z0[q][e], t = (float)d[q].e[e];
             o[e] = t * (FROM ? act_slope_out<ACT>(x) : act_slope<ACT, sizeof(T) == 4>(x));
             if constexpr (GATED) {
               o[e] *= z1[q][e];

@@ -111,15 +111,9 @@ def _ld(t: torch.Tensor) -> int:
   return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-# float32 layers whose slope the output gives store nothing else for the backward pass (16 bits: 1 + y and 1 - y^2 would cancel)
+# float32 layers whose slope the output gives store nothing else for the backward pass.  16 bits: 1 + y and 1 - y^2 would cancel, and a rounded sum shows in the
+# gradients (tanh: 1.54 times the error of their own rounding, elu 1.14; relu: sums below half of fp16's smallest number have slope 0), so the sums are kept as floats.
 _FROM_OUTPUT = {ACTIVATIONS[a] for a in ("relu", "elu", "tanh", "sigmoid")}
-
-
-# 16-bit dense layers whose sums are kept as floats: the slopes of these fall like exp(-2 |z|) and exp(-|z|), and a z that is rounded shows in the gradients (tanh:
-# 1.54 times the error of their own rounding, 1.41 with floats).  elu (1.14), silu and gelu (1.46) keep floats where it costs nothing: 2^22 sums are 8 MB more each
-# way, 3 us of a call that takes the host 70; for 24576 x 1024 it would be 20 us of 300.
-_WIDE = {ACTIVATIONS[a] for a in ("tanh", "sigmoid")}
-_WIDE_SMALL = {ACTIVATIONS[a] for a in ("elu", "silu", "gelu")}
 
 
 def _from_output(x, w_up, r, act: int) -> bool:
@@ -139,7 +133,7 @@ def _forward(x, w, w_up, b, b_up, r, act: int, keep: bool, y=None):
       if not native.policy_lib().mjlab_layer_recomputes(_LAYER.pack(dtype, act, 0, 0, m, k, n, *inputs, *lds, 0, 0, 0, 0, 0)):
         z, z_up = (torch.empty((m, n), dtype=torch.float32, device=x.device) for _ in range(2))
     elif keep and act and not _from_output(x, w_up, r, act):
-      z = torch.empty((m, n), dtype=torch.float32 if act in _WIDE or (act in _WIDE_SMALL and m * n <= 1 << 22) else x.dtype, device=x.device)
+      z = torch.empty((m, n), dtype=torch.float32, device=x.device)
     args = (dtype, act, 0, 0 if z is None else z.element_size(), m, k, n, *inputs, *lds, y.data_ptr(), _ptr(z), _ptr(z_up))
     need = native.policy_lib().mjlab_layer_forward_workspace(_LAYER.pack(*args, 0, 0))
     if need < 0:

@@ -99,8 +99,8 @@ def only_rounded(got, want, e2, what):
 
 
 @pytest.mark.parametrize("dtype", HALVES)
-@pytest.mark.parametrize("name,gated", [("elu", False), ("silu", False), ("gelu", False), ("tanh", False), ("silu", True)])
-@pytest.mark.parametrize("m,k,n", [(1203, 1001, 1003), (701, 333, 405)])
+@pytest.mark.parametrize("name,gated", [("elu", False), ("silu", False), ("gelu", False), ("tanh", False), ("sigmoid", False), ("silu", True)])
+@pytest.mark.parametrize("m,k,n", [(1203, 1001, 1003), (2101, 45, 2103), (701, 333, 405)])
 def test_gradients_are_as_exact_as_their_own_rounding(m, k, n, name, gated, dtype):
   """Roundings are independent, so a sum of terms t_i that are each off by at most r |t_i| is off by r sqrt(sum t_i^2) in the mean, and one of n additions in 32 bits
   by sqrt(n) u32 times the same (its partial sums are no larger in the mean)."""
@@ -124,3 +124,14 @@ def test_gradients_are_as_exact_as_their_own_rounding(m, k, n, name, gated, dtyp
     only_rounded(grads[0], sum(d @ q for d, q in zip(dz, ws, strict=True)), sum((o * o + 6 * n * U32**2 * d * d) @ (q * q) for o, d, q in zip(off, dz, ws, strict=True)), "dx")
     for g, d, o in zip(grads[1:], dz, off, strict=True):
       only_rounded(g, d.t() @ X, (o * o + 3 * m * U32**2 * d * d).t() @ (X * X), "dw")
+
+
+@pytest.mark.parametrize("name,slope", [("relu", 1.0), ("silu", 0.5), ("elu", 1.0)])
+@pytest.mark.parametrize("m,n", [(3, 5), (2100, 2102)])
+def test_the_slope_at_sums_that_fp16_cannot_hold(name, slope, m, n):
+  """2^-15 * 2^-15 is 0 in fp16; its slope is that of a positive number."""
+  from mjlab_amd import policy_ops
+
+  x, w = (torch.full((s, 1), 2.0**-15, device="cuda", dtype=torch.float16, requires_grad=True) for s in (m, n))
+  dx, dw = torch.autograd.grad(policy_ops.dense(x, w, activation=name), (x, w), torch.ones((m, n), device="cuda", dtype=torch.float16))
+  assert torch.equal(dx.double(), torch.full_like(dx, slope * n * 2.0**-15).double()) and torch.equal(dw.double(), torch.full_like(dw, slope * m * 2.0**-15).double())
