@@ -14,7 +14,8 @@
 // left: 3 x 8 bits and their signs hold all 24), so a b = hh + hm + mh + mm + hl + lh and terms below 2^-23 |a b|, which are left out: six products
 // of 16 bits, summed in 32, for one of float -- the error of a float product's own rounding, at more than the float instruction's rate (24576 x 1024 x 1024: 190 TFLOP/s; the library's float product
 // 128).  A number that has no
-// such sum (infinite, NaN, or so large that h overflows) sets a flag, and its workgroup's product is formed again with the float instruction.
+// such sum (infinite, NaN, or so large that h overflows) sets a flag, and its workgroup's product is formed again with the float instruction: so do infinities of
+// whole operands, since zero times infinity is NaN.
 //
 // dz, 16 bits: a float in memory, since a gradient may leave fp16's range on both sides where what it is summed to does not, and since its rounding to 16 bits would
 // show in the gradients (off by 1.41 times their own rounding).  It is read as two bf16, 2^-16 of it left out, and a float16 that it meets as two, exactly:
@@ -109,11 +110,17 @@ template <typename O, int KB, bool KC, int R> struct Tile {
   static __device__ __forceinline__ int row_of(int u) { return u / UPR; }
   static __device__ __forceinline__ int col_of(int u) { return u % UPR * UE; }
 
-  static __device__ __forceinline__ void put(char* s, int u, const Unit<M, UE>& x, float& odd) {
+  // WATCH: the other operand has several planes, one of which may be zero where this one is infinite
+  template <bool WATCH> static __device__ __forceinline__ void put(char* s, int u, const Unit<M, UE>& x, float& odd) {
     const int row = u / UPR, c = u % UPR;
     char* at = s + (KC ? row * KB + (swizzle(row, c) << 4) : row * STRIDE + c * 16);
     if constexpr (O::PLANES > 1) put_split<O::PLANES>(at, PLANE, x.e, odd);
-    else if constexpr (sizeof(M) == sizeof(E)) *(Unit<M, UE>*)at = x;
+    else if constexpr (sizeof(M) == sizeof(E)) {
+      *(Unit<M, UE>*)at = x;
+      if constexpr (WATCH)
+#pragma unroll
+        for (int i = 0; i < UE; ++i) odd = __builtin_fmaf((float)x.e[i], 0.f, odd);
+    }
     else *(f32x4*)at = f32x4{(float)x.e[0], (float)x.e[1], (float)x.e[2], (float)x.e[3]};
   }
 
@@ -139,7 +146,7 @@ template <typename O, int KB, bool KC, int R> struct Tile {
   }
 };
 
-// The sum over k in [kbeg, kend) for the tile at (m0, n0): 4 waves as 2 x 2, each BM / 2 x BN / 2 in 32 x 32 tiles.  -> true if a number is not the sum of its planes.
+// The sum over k in [kbeg, kend) for the tile at (m0, n0): 4 waves as 2 x 2, each BM / 2 x BN / 2 in 32 x 32 tiles.  -> true if planes do not multiply as their number does.
 template <typename OA, typename OB, int KB, int BUFFERS, bool AK, bool BK, int BM, int BN, bool GATED>
 __device__ __forceinline__ bool product_tile(const Product& p, long long m0, long long n0, long long kbeg, long long kend, char* lds, f32x16 (&acc)[BM / 64][BN / 64]) {
   using TA = Tile<OA, KB, AK, BM>;
@@ -221,9 +228,9 @@ __device__ __forceinline__ bool product_tile(const Product& p, long long m0, lon
   float odd = 0.f;
   auto stage = [&](char* s) {
 #pragma unroll
-    for (int i = 0; i < TA::NU; ++i) TA::put(s, tid + i * 256, ra[i], odd);
+    for (int i = 0; i < TA::NU; ++i) TA::template put<(PB > 1)>(s, tid + i * 256, ra[i], odd);
 #pragma unroll
-    for (int i = 0; i < TB::NU; ++i) TB::put(s + TA::BYTES, tid + i * 256, rb[i], odd);
+    for (int i = 0; i < TB::NU; ++i) TB::template put<(PA > 1)>(s + TA::BYTES, tid + i * 256, rb[i], odd);
   };
 
 #pragma unroll

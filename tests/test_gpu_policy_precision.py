@@ -135,3 +135,25 @@ def test_the_slope_at_sums_that_fp16_cannot_hold(name, slope, m, n):
   x, w = (torch.full((s, 1), 2.0**-15, device="cuda", dtype=torch.float16, requires_grad=True) for s in (m, n))
   dx, dw = torch.autograd.grad(policy_ops.dense(x, w, activation=name), (x, w), torch.ones((m, n), device="cuda", dtype=torch.float16))
   assert torch.equal(dx.double(), torch.full_like(dx, slope * n * 2.0**-15).double()) and torch.equal(dw.double(), torch.full_like(dw, slope * m * 2.0**-15).double())
+
+
+@pytest.mark.parametrize("dtype", list(U))
+@pytest.mark.parametrize("name", ["silu", "none"])
+@pytest.mark.parametrize("m,k,n", [(40, 24, 30), (1203, 1001, 1003), (5, 1999, 333)])
+def test_an_infinite_input_or_weight_stays_infinite(m, k, n, name, dtype):
+  """Positive weights: the sums that the infinite number is in are infinite, so the slope there is 1 and dz = dy; dw has infinities of dy's sign in the infinite
+  input's column, dx in the infinite weight's, and numbers elsewhere."""
+  from mjlab_amd import policy_ops
+
+  gen = torch.Generator(device="cuda").manual_seed(6)
+  x, w = (torch.rand(s, generator=gen, device="cuda").add_(0.5).to(dtype) for s in ((m, k), (n, k)))
+  dy = torch.where(torch.rand((m, n), generator=gen, device="cuda") < 0.5, -1.0, 1.0).to(dtype)
+  for inputs_bad, (row, col) in ((True, (m - 2, 7)), (False, (n - 4, 11))):
+    leaves = [x.clone(), w.clone()]
+    leaves[0 if inputs_bad else 1][row, col] = float("inf")
+    for t in leaves:
+      t.requires_grad_(True)
+    g = torch.autograd.grad(policy_ops.dense(*leaves, activation=name), leaves, dy)[1 if inputs_bad else 0]
+    rest = torch.ones((k,), dtype=torch.bool, device="cuda")
+    rest[col] = False
+    assert torch.equal(g[:, col].float(), (dy[row, :] if inputs_bad else dy[:, row]).float() * float("inf")) and g[:, rest].isfinite().all()
