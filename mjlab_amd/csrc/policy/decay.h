@@ -29,21 +29,21 @@ struct DecayPass {
   float *seg_state, *seg_factor;  // (seg_given: seg_state is read only) (sequences * heads, segments - 1, da, dc), (sequences * heads, segments - 1)
 };
 
-// What the matrix cores read.  float as it is.  bf16 as it is; what is formed on the way (weighted rows, pairs, R) is rounded to it, like the outputs,
-// but for the weighted rows of a pass whose R is wanted in the end (EXACT), a float output: they are three.  fp16: a b^T
-// as it is, but sums of keys and values may leave fp16's range, so all else is multiplied as sums of bf16, each the nearest to what is left: two hold
-// an fp16 number and 16 bits of R and of a pair (outputs are rounded to 11), three a weighted row (which R, a float output in the end, is made of).
+// What the matrix cores read.  float as it is.  16 bits: a b^T as it is; what is formed on the way (weighted rows, pairs, R as the outputs read it) as sums of bf16,
+// each the nearest to what is left: two leave out 2^-16 of it, which does not show in outputs of 8 or 11 bits (one bf16: off by 1.41 times their own rounding),
+// three hold a float -- the weighted rows of a pass whose R is wanted in the end (EXACT), a float output.  fp16: two bf16 hold an fp16 number as well, exactly, and
+// sums of keys and values may leave fp16's range, so all but a b^T is multiplied as bf16.
 template <typename T, bool EXACT> struct DecayCfg {
   using L = float;
-  static constexpr int KS = 4, PAD = 4, A = 1, W = 1, N = 1;  // k per matrix instruction, padding of LDS rows, planes of a, of weighted b, of c, P and R
+  static constexpr int KS = 4, PAD = 4, A = 1, W = 1, N = 1, P = 1;  // k per matrix instruction, padding of LDS rows, planes of a, of weighted b, of c, of pairs and R
 };
 template <bool EXACT> struct DecayCfg<__bf16, EXACT> {
   using L = __bf16;
-  static constexpr int KS = 32, PAD = 8, A = 1, W = EXACT ? 3 : 1, N = 1;
+  static constexpr int KS = 32, PAD = 8, A = 1, W = EXACT ? 3 : 2, N = 1, P = 2;
 };
 template <bool EXACT> struct DecayCfg<_Float16, EXACT> {
   using L = __bf16;
-  static constexpr int KS = 32, PAD = 8, A = 2, W = 3, N = 2;
+  static constexpr int KS = 32, PAD = 8, A = 2, W = 3, N = 2, P = 2;
 };
 // tokens per chunk
 template <typename T> constexpr int decay_chunk(bool both_large) { return sizeof(T) == 4 || (DecayCfg<T, false>::N > 1 && both_large) ? 32 : 64; }
@@ -81,8 +81,11 @@ template <typename T, int DA, int DC, bool STATE, bool EXACT> struct DecayLds {
   using L = typename Cfg::L;
   static constexpr int C = decay_chunk<T>(DA > 64 && DC > 64), PAD = Cfg::PAD, LA = DA + PAD, LC = DC + PAD, LP = C + PAD;
   static constexpr int SW = C * LA, SC = C * LC, SP = STATE ? 8 : C * LP, SR = STATE ? 8 : DC * LA;  // a plane of each
+  // b times its tokens' weights into R.  bf16: the third plane takes the place of b when the pairs are formed (LDS then holds 128 x 128 heads, and two workgroups of 64 x 64)
+  static constexpr bool LATE = !STATE && Cfg::W == 3 && Cfg::N == 1;
+  L bw[(LATE ? 2 : Cfg::W) * SW];
   T b[STATE ? 8 : C * LA];
-  L bw[Cfg::W * SW], c[Cfg::N * SC], p[Cfg::N * SP], r[Cfg::N * SR];  // bw: b times its tokens' weights into R
+  L c[Cfg::N * SC], p[Cfg::P * SP], r[Cfg::P * SR];
   float enter[C];                 // of R into token i
   int episode[C], odd[8];         // the episode a token belongs to, counted in the chunk
 };
@@ -116,14 +119,26 @@ template <int NA, int NB, typename F> __device__ __forceinline__ f32x4 mma_plane
   return x;
 }
 
-// VEC elements of T times w (w 0: zeros, whatever x holds), as N planes of L
-template <int N, typename T, typename L> __device__ __forceinline__ void put_weighted(L* at, int plane, const Chunk<T>& x, float w) {
+// VEC elements of T times w (w 0: zeros, whatever x holds), as N planes of L; `last`: where the third goes instead
+template <int N, typename T, typename L> __device__ __forceinline__ void put_weighted(L* at, int plane, const Chunk<T>& x, float w, L* last = nullptr) {
 #pragma unroll
   for (int h = 0; h < Elem<T>::VEC; h += 4) {
     f32x4 y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] = w * (float)x.e[h + e];
-    put4<N>(at + h, plane, w == 0.f ? f32x4{} : y);
+    if (w == 0.f) y = f32x4{};
+    if constexpr (N == 3) {
+      if (last) {
+        put4<2>(at + h, plane, y);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] -= (float)(L)y[e];
+        put4<1>(last + h, plane, y);
+        continue;
+      }
+    }
+    put4<N>(at + h, plane, y);
   }
 }
 
@@ -153,29 +168,32 @@ template <typename T, int FIT> __device__ __forceinline__ Chunk<T> load_row(cons
   else return load_part(at, d - col);
 }
 
-constexpr int decay_threads(int da, int dc) { return da >= 64 && dc >= 64 ? 512 : 256; }
+// (bf16 128 x 32 heads, 256 sequences of 1024 tokens, forward: 256 threads 90 us, since they need all 256 registers, 512 63.  Chunks of 32 have no eight waves' rows there.)
+template <typename T> constexpr int decay_threads(int da, int dc) { return (da >= 64 && dc >= 64) || (da * dc >= 64 * 64 && decay_chunk<T>(false) == 64) ? 512 : 256; }
 
 // 256 or 512 threads per (sequence, head, segment).  STATE: the first pass of a split sequence, the segment's contribution to R alone.
 // Products are formed such that an accumulator's four rows are neighbours in memory: P^T and out^T (columns are tokens), R (rows are da).  The rows of a go
-// from memory to the matrix cores' registers without LDS, which holds one workgroup of 128 x 128 heads per CU (bf16 96 KB).
-// 256 sequences of 1024 tokens, forward: bf16 128 x 128 84 us (75, 3.6 TB/s, where R is not wanted in the end), 64 x 64 57 us (47), 32 x 32 47 us (45); fp16 64 x 64 63 us, 128 x 128 235 us; float 64 x 64
-// 128 us, 128 x 128 300 us.  Large bf16 heads are near the memory's rate; the others are bound by the chain of a chunk (stage, pairs, R, with a barrier
-// and LDS reads between): 2.5 us for a chunk of 64 at 32 x 32, 2.3 with every row in L2.  More workgroups per CU, where there are more sequences, hide it.
-template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global__ __launch_bounds__(decay_threads(DA, DC), 2) void k_decay_chunks(const DecayPass p) {
+// from memory to the matrix cores' registers without LDS, which holds one workgroup of 128 x 128 heads per CU (bf16 155 KB).
+// 256 sequences of 1024 tokens, forward with R in the end, us: bf16 128 x 128 116 (2.3 TB/s), 64 x 64 54, 32 x 32 48; fp16 128 x 128 235, 64 x 64 59; float 128 x 128
+// 295, 64 x 64 124.  All are bound by the chain of a chunk (stage, pairs, R, with a barrier and LDS reads between): 3 us for a chunk of 64 at 32 x 32, 7 at
+// 128 x 128.  More workgroups per CU, where there are more sequences, hide it.
+template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global__ __launch_bounds__(decay_threads<T>(DA, DC), 2) void k_decay_chunks(const DecayPass p) {
   using Cfg = DecayCfg<T, EXACT>;
   using L = typename Cfg::L;
   using S = DecayLds<T, DA, DC, STATE, EXACT>;
   constexpr bool FULL = FIT == FIT_FULL;
   // The scheduler is kept from loading the fragments of every column at once: small heads have the registers for it (float 64 x 64 128 us without, 135 with)
   constexpr bool FENCE = DA * DC > 64 * 64;
-  constexpr int C = S::C, KS = Cfg::KS, NA = Cfg::A, PW = Cfg::W, NN = Cfg::N, LA = S::LA, LC = S::LC, LP = S::LP, V = Elem<T>::VEC, CT = C / 16, KA = DA / KS;
-  constexpr int NT = decay_threads(DA, DC), NW = NT / 64, NB = (C * DA / V + NT - 1) / NT, NC = (C * DC / V + NT - 1) / NT;  // 16-byte chunks per thread
+  constexpr int C = S::C, KS = Cfg::KS, NA = Cfg::A, PW = Cfg::W, NN = Cfg::N, PR = Cfg::P, LA = S::LA, LC = S::LC, LP = S::LP, V = Elem<T>::VEC, CT = C / 16, KA = DA / KS;
+  constexpr int NT = decay_threads<T>(DA, DC), NW = NT / 64, NB = (C * DA / V + NT - 1) / NT, NC = (C * DC / V + NT - 1) / NT;  // 16-byte chunks per thread
   // Waves: of out, OR x OC waves of TR x TC tiles (tokens x dc); of R, RW x NW / RW waves of RR x RC tiles (da x dc)
   constexpr int OC = CT == 4 ? 2 : (DC / 16 < NW ? DC / 16 : NW);
   constexpr int OR = NW / OC, TR = CT / OR, TC = DC / 16 / OC, RW = NW == 8 && DA >= 64 ? 4 : 2, RR = DA / 16 / RW, RC = DC / 16 * RW / NW;
   static_assert(OR * OC == NW && OR * TR == CT && OC * TC == DC / 16 && RR >= 1 && RC >= 1 && RR * RW == DA / 16 && RC * (NW / RW) == DC / 16, "tiles do not cover");
   extern __shared__ __attribute__((aligned(16))) char lds[];
   S& s = *(S*)lds;
+  L* const bw = (L*)lds;  // (runs on into s.b where its third plane comes late)
+  static_assert(offsetof(S, bw) == 0 && (!S::LATE || offsetof(S, b) == 2 * S::SW * sizeof(L)), "the planes of bw are equally far apart");
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row4 = (lane >> 4) * 4, colx = lane & 15;
   const int t0 = (wave / OC) * TR, c0 = (wave % OC) * TC, r0 = wave / (NW / RW) * RR, rc0 = wave % (NW / RW) * RC;  // this wave's first tiles
@@ -251,7 +269,7 @@ template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global_
       }
     }
   };
-  // (rows row0 .. of b or R, k contiguous) (a's rows of token tile t)^T over all of da.  R, fp16: of whole numbers where something is not finite, since a plane of
+  // (rows row0 .. of b or R, k contiguous) (a's rows of token tile t)^T over all of da.  R, 16 bits: of whole numbers where something is not finite, since a plane of
   // zeros times infinity would be NaN.
   auto with_a = [&](auto of_r, const auto* rows, int row0, int t, bool whole) {
     f32x4 x = {};
@@ -262,24 +280,24 @@ template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global_
 #pragma unroll
         for (int e = 0; e < 4; ++e) x = mma16(o[e], fa[t][i][e], x);
       }
-    } else if constexpr (NN == 1) {
-#pragma unroll
-      for (int k = 0; k < KA; ++k) x = mma16(frag_kc(rows, LA, row0, k * KS, lane), fa[t][k], x);
     } else if constexpr (!decltype(of_r)::value) {
 #pragma unroll
-      for (int k = 0; k < KA; ++k) x = mma16h(frag_kc(rows, LA, row0, k * KS, lane), fa[t][k], x);
+      for (int k = 0; k < KA; ++k) {
+        const s16x8 o = frag_kc(rows, LA, row0, k * KS, lane);
+        x = NN == 1 ? mma16(o, fa[t][k], x) : mma16h(o, fa[t][k], x);
+      }
     } else if (!whole) {
 #pragma unroll
       for (int k = 0; k < KA; ++k) {
-        s16x8 o[NN];
+        s16x8 o[PR];
 #pragma unroll
-        for (int i = 0; i < NN; ++i) o[i] = frag_kc(rows + i * S::SR, LA, row0, k * KS, lane);
-        x = mma_planes<NN, NA>(o, fs[k], x);
+        for (int i = 0; i < PR; ++i) o[i] = frag_kc(rows + i * S::SR, LA, row0, k * KS, lane);
+        x = mma_planes<PR, NA>(o, NN == 1 ? &fa[t][k] : fs[k], x);
       }
     } else {
       for (int k = 0; k < KA; ++k)
         for (int e = 0; e < 8; ++e)
-          x = mma16(get<NN>(rows + (row0 + colx) * LA + k * KS + 2 * row4 + e, S::SR), (float)__builtin_bit_cast(h16x8, fa[t][k])[e], x);
+          x = mma16(get<PR>(rows + (row0 + colx) * LA + k * KS + 2 * row4 + e, S::SR), (float)__builtin_bit_cast(Chunk<T>, fa[t][k]).e[e], x);
     }
     return x;
   };
@@ -322,12 +340,13 @@ template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global_
     __syncthreads();  // the chunk before is done with LDS
     unsigned most = 0;
     float odd = 0.f;  // NaN: R is not finite
+    Chunk<L> late[S::LATE ? NB : 1];
 #pragma unroll
     for (int i = 0; i < NB; ++i) {
       const int row = (tid + i * NT) / (DA / V), col = (tid + i * NT) % (DA / V) * V;
       if (row >= C) continue;
       const float w = row < n && !cut_out && (whole || episode(row) == e_last) ? p.us * power(n - p.e0 - row) : 0.f;
-      put_weighted<PW>(s.bw + row * LA + col, S::SW, xb[i], w);
+      put_weighted<PW>(bw + row * LA + col, S::SW, xb[i], w, S::LATE ? late[S::LATE ? i : 0].e : nullptr);
       if constexpr (!STATE) *(Chunk<T>*)(s.b + row * LA + col) = xb[i];
       if constexpr (PW > 1) see(most, xb[i]);
     }
@@ -349,13 +368,13 @@ template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global_
       for (int i = 0; i < RR; ++i)
 #pragma unroll
         for (int j = 0; j < RC; ++j) {
-          put4<NN>(s.r + ((rc0 + j) * 16 + colx) * LA + (r0 + i) * 16 + row4, S::SR, acc[i][j]);
-          if constexpr (NN > 1)
+          put4<PR>(s.r + ((rc0 + j) * 16 + colx) * LA + (r0 + i) * 16 + row4, S::SR, acc[i][j]);
+          if constexpr (PR > 1)
 #pragma unroll
             for (int e = 0; e < 4; ++e) odd = __builtin_fmaf(acc[i][j][e], 0.f, odd);
         }
     }
-    if constexpr (!STATE && NN > 1)
+    if constexpr (!STATE && PR > 1)
 #pragma unroll
       for (int t = 0; t < TR; ++t)
 #pragma unroll
@@ -409,7 +428,7 @@ template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global_
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = (tj < t0 + t || j + e <= i) && i < n && (whole || s.episode[j + e] == ei) ? w[e] * y[e] : 0.f;
           }
-          put4<NN>(s.p + i * LP + tj * 16 + row4, S::SP, y);
+          put4<PR>(s.p + i * LP + tj * 16 + row4, S::SP, y);
           if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -425,18 +444,25 @@ template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global_
       }
       if (q0 + C < last) load_a(q0 + C);
       __syncthreads();
+      if constexpr (S::LATE) {  // (the pairs were the last that read b)
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const int row = (tid + i * NT) / (DA / V), col = (tid + i * NT) % (DA / V) * V;
+          if (row < C) *(Chunk<L>*)(bw + 2 * S::SW + row * LA + col) = late[i];
+        }
+      }
       if (!by_term) {
 #pragma unroll
         for (int t = 0; t < TR; ++t)
           for (int k = 0; k < (t0 + t + 1) * 16; k += KS) {
-            decltype(frag_kr(s.c, LC, 0, 0, lane)) fp[NN], fc[NN];
+            decltype(frag_kr(s.c, LC, 0, 0, lane)) fp[PR], fc[NN];
 #pragma unroll
-            for (int q = 0; q < NN; ++q) fp[q] = frag_kc(s.p + q * S::SP, LP, (t0 + t) * 16, k, lane);
+            for (int q = 0; q < PR; ++q) fp[q] = frag_kc(s.p + q * S::SP, LP, (t0 + t) * 16, k, lane);
 #pragma unroll
             for (int c = 0; c < TC; ++c) {
 #pragma unroll
               for (int q = 0; q < NN; ++q) fc[q] = frag_kr(s.c + q * S::SC, LC, (c0 + c) * 16, k, lane);
-              x[t][c] = mma_planes<NN, NN>(fc, fp, x[t][c]);
+              x[t][c] = mma_planes<NN, PR>(fc, fp, x[t][c]);
             }
             if constexpr (FENCE) __builtin_amdgcn_sched_barrier(0);
           }
@@ -446,7 +472,7 @@ template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global_
           const int i = (t0 + t) * 16 + colx, ei = s.episode[i];
           for (int j = 0; j <= i && i < n; ++j)
             if (s.episode[j] == ei) {
-              const float w = get<NN>(s.p + i * LP + j, S::SP);
+              const float w = get<PR>(s.p + i * LP + j, S::SP);
 #pragma unroll
               for (int c = 0; c < TC; ++c)
 #pragma unroll
@@ -478,6 +504,7 @@ template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global_
     }
 
     if (!STATE && !end && q0 + C >= last) break;  // nobody wants R any more
+    if constexpr (S::LATE) __syncthreads();
     const float through = carries ? power(n) : 0.f;
     factor *= through;
     if (carries) {
@@ -496,11 +523,11 @@ template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global_
     if (!by_term) {
 #pragma unroll 2
       for (int k = 0; k < C; k += KS) {
-        decltype(frag_kr(s.bw, LA, 0, 0, lane)) fb[RR][PW], fc[NN];
+        decltype(frag_kr(bw, LA, 0, 0, lane)) fb[RR][PW], fc[NN];
 #pragma unroll
         for (int i = 0; i < RR; ++i)
 #pragma unroll
-          for (int q = 0; q < PW; ++q) fb[i][q] = frag_kr(s.bw + q * S::SW, LA, (r0 + i) * 16, k, lane);
+          for (int q = 0; q < PW; ++q) fb[i][q] = frag_kr(bw + q * S::SW, LA, (r0 + i) * 16, k, lane);
 #pragma unroll
         for (int j = 0; j < RC; ++j) {
 #pragma unroll
@@ -520,7 +547,7 @@ template <typename T, int DA, int DC, int FIT, bool STATE, bool EXACT> __global_
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = (r0 + i) * 16 + row4 + e;
-              if (FULL || r < p.da) acc[i][j][e] += get<PW>(s.bw + t * LA + r, S::SW) * get<NN>(s.c + t * LC + (rc0 + j) * 16 + colx, S::SC);
+              if (FULL || r < p.da) acc[i][j][e] += get<PW>(bw + t * LA + r, S::SW) * get<NN>(s.c + t * LC + (rc0 + j) * 16 + colx, S::SC);
             }
       }
     }

@@ -13,7 +13,7 @@ struct Split {
 Split split(const mjlab_decay_t* d) {
   const int C = decay_chunk<T>(d->dk > 64 && d->dv > 64);
   const long long chunks = (d->length + C - 1) / C, rows = d->batch * d->heads, least = d->dk < d->dv ? d->dk : d->dv, most_d = d->dk < d->dv ? d->dv : d->dk;
-  const bool alone = DecayCfg<T, false>::N > 1 ? least > 32 || most_d > 64 : least > 32 && most_d > 64;  // whether LDS holds one workgroup per CU, or two
+  const bool alone = DecayCfg<T, false>::N > 1 ? least > 32 || most_d > 64 : most_d > 64 && (least > 32 || DecayCfg<T, false>::P > 1);  // whether LDS holds one workgroup per CU, or two
   const long long slots = alone ? CUS : 2 * CUS;
   if (2 * rows >= slots || chunks < 8) return {1, (int)chunks};
   const long long want = slots / rows, most = chunks / 4, s = want < most ? want : most;
@@ -28,18 +28,18 @@ template <int DA, int DC, int FIT, bool EXACT> hipError_t launch_sized(const Dec
   constexpr int LDS = (int)sizeof(DecayLds<T, DA, DC, false, EXACT>), LDS_FIRST = (int)sizeof(DecayLds<T, DA, DC, true, EXACT>);
   static std::atomic<unsigned long long> asked{0}, asked_first{0};
   hipError_t e;
-  if (rows * p.segments * decay_threads(DA, DC) > 0xffffffffLL) return hipErrorInvalidValue;
+  if (rows * p.segments * decay_threads<T>(DA, DC) > 0xffffffffLL) return hipErrorInvalidValue;
   if (p.segments > 1 && !p.seg_given) {
     auto first = k_decay_chunks<T, DA, DC, FIT, true, EXACT>;
     if ((e = allow_lds(first, LDS_FIRST, asked_first)) != hipSuccess) return e;
-    hipLaunchKernelGGL(first, dim3((unsigned)(rows * (p.segments - 1))), dim3(decay_threads(DA, DC)), LDS_FIRST, st, p);
+    hipLaunchKernelGGL(first, dim3((unsigned)(rows * (p.segments - 1))), dim3(decay_threads<T>(DA, DC)), LDS_FIRST, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
     hipLaunchKernelGGL(k_decay_scan<T>, dim3((unsigned)(rows * ((p.da * p.dc + 255) / 256))), dim3(256), 0, st, p);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   auto kern = k_decay_chunks<T, DA, DC, FIT, false, EXACT>;
   if ((e = allow_lds(kern, LDS, asked)) != hipSuccess) return e;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(rows * p.segments)), dim3(decay_threads(DA, DC)), LDS, st, p);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(rows * p.segments)), dim3(decay_threads<T>(DA, DC)), LDS, st, p);
   return hipGetLastError();
 }
 

@@ -1,6 +1,6 @@
-"""What the 16-bit layers keep between their forward and their gradients: nothing of it is rounded to 16 bits, and none of it leaves the range of a float.
+"""What 16-bit operators keep on the way to their outputs: nothing of it is rounded to 16 bits, and none of it leaves the range of a float.
 
-Bounds, element by element, from the sizes alone (u: half a step of the type; u32 = 2^-24).  The sums before the activation are floats: off by at most
+Layers: bounds, element by element, from the sizes alone (u: half a step of the type; u32 = 2^-24).  The sums before the activation are floats: off by at most
 (k + 2) u32 sum |x w|, and the slope by that (Lipschitz with constant <= 1) and its evaluation, 16 u32 (1 + |z|).  dz is a float, formed with at most four
 roundings.  The matrix cores read it as two bfloat16, which leaves at most 2^-8 of 2^-8 of it; a float16 that it meets is two bfloat16 as well (exactly), and the
 product of the two second parts, another 2^-16, is not formed.  Three such products per term are summed in 32 bits, in any order.  Then one rounding to the type."""
@@ -8,6 +8,7 @@ product of the two second parts, another 2^-16, is not formed.  Three such produ
 import pytest
 import torch
 from test_gpu_policy_layers import TINY, U, U32, act, close, rand
+from test_gpu_policy_memory import inputs, recurrence
 
 pytestmark = pytest.mark.gpu
 
@@ -157,3 +158,24 @@ def test_an_infinite_input_or_weight_stays_infinite(m, k, n, name, dtype):
     rest = torch.ones((k,), dtype=torch.bool, device="cuda")
     rest[col] = False
     assert torch.equal(g[:, col].float(), (dy[row, :] if inputs_bad else dy[:, row]).float() * float("inf")) and g[:, rest].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", HALVES)
+@pytest.mark.parametrize("b,t,h,dk,dv", [(2, 1100, 2, 128, 128), (2, 1100, 3, 64, 64), (2, 1100, 2, 127, 33), (2, 300, 2, 128, 128), (3, 150, 2, 48, 80), (2, 200, 2, 32, 128), (2, 200, 2, 128, 32)])
+def test_memory_is_as_exact_as_its_own_rounding(b, t, h, dk, dv, dtype):
+  """Linear attention: a weighted key, a pair and the state are each read as two bfloat16 at least, 2^-16 of them left out; two of them are on the way to an output, 2^-15
+  in all.  The sum of the terms' squares is the recurrence on squares.  What is wanted in the end as floats (the state, its gradient) is made of weighted keys as three bfloat16: off by roundings of
+  32 bits alone, as many as there are steps and terms of a dot product, their root in the mean."""
+  from mjlab_amd import policy_ops
+
+  x = inputs(b, t, h, dk, dv, dtype, seed=18, resets=0.005, carry=True)
+  leaves = [x[n].requires_grad_(True) for n in ("q", "k", "v", "state")]
+  o, final = policy_ops.decay_attention(*leaves[:3], x["log_decay"], state=leaves[3], reset=x["reset"])
+  got = [o, final, *torch.autograd.grad([o, final], leaves, [x["do"], x["dstate"]])]
+  with torch.no_grad():
+    lam, scale = x["log_decay"].double().exp(), dk**-0.5
+    want = recurrence(*leaves[:3], lam, scale, leaves[3], x["reset"], None, x["do"], x["dstate"])
+    squares = recurrence(*(z.double() ** 2 for z in leaves[:3]), lam**2, scale**2, leaves[3].double() ** 2, x["reset"], None, x["do"].double() ** 2, x["dstate"].double() ** 2)
+    for name, g, w, s in zip(("o", "final", "dq", "dk", "dv", "dstate"), got, want, squares, strict=True):
+      floats = name in ("final", "dstate")
+      only_rounded(g, w, s * (4 * (t + max(dk, dv)) * U32**2 if floats else 2.0**-30), name)
