@@ -421,7 +421,7 @@ class PhysicsRollout:
     return self._cut
 
   def capture_graph(self, policy=None) -> None:
-    """Capture one control step into a hipGraph (the physics kernels are launched directly
+    """Capture one control step into a hipGraph, after one control step to warm up (the physics kernels are launched directly
     inside the capture, not through the Simulation's own step/forward graphs).  With a ``policy``
     (mjlab_amd.policy.Policy) the graph begins with its action: observation rows -> network -> physics, then
     ``step()`` takes no action.  Its parameters are read at every replay, so an update in place takes effect; its
@@ -434,6 +434,8 @@ class PhysicsRollout:
     self._action_buf = torch.zeros((n, self.m.nu), device=dev)
     # with the fused reset the mask written by the library IS the result (int32, non-zero = reset): no conversion launch
     self._reset_buf = self._reset_mask if self.fused_reset else torch.zeros((n,), dtype=torch.bool, device=dev)
+    # the warm-up is a control step, too: what the step before it reset and what it resets itself are both still to be cut from a caller's memory
+    cut = None if self._cut is None else self._cut != 0
     sim_graph = self.sim.use_graph
     self.sim.use_graph = False  # nested replays cannot be captured; record the raw launches
     try:
@@ -443,6 +445,8 @@ class PhysicsRollout:
       with torch.cuda.stream(st):
         self._capture_body()
       torch.cuda.current_stream(dev).wait_stream(st)
+      if cut is not None:
+        self._cut = cut | (self._reset_buf != 0)
       g = torch.cuda.CUDAGraph()
       g.register_generator_state(self.gen)
       with torch.cuda.graph(g):
