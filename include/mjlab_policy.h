@@ -48,6 +48,11 @@ int mjlab_sizeof_layer(void);
 /* 1: the backward pass of this (gated, 16-bit) layer forms the sums again when z and z_up are NULL, which is faster than storing them; 0: it needs them. */
 int mjlab_layer_recomputes(const mjlab_layer_t* f);
 
+/* The tile that a product of this layer runs in -- its rows: 64 (x 64), 128 (x 128) or 256 (x 128) --, negative where its sums are split and joined by a second
+ * launch; 0: bad arguments.  For tests and for reading a profile: sizes choose it, callers need not know. */
+enum { MJLAB_PRODUCT_FORWARD = 0, MJLAB_PRODUCT_INPUT, MJLAB_PRODUCT_WEIGHT };
+int mjlab_layer_tile(const mjlab_layer_t* f, int product);
+
 /* The backward pass of the layer `f` (x, w, w_up, z, z_up and the sizes are read, b and b_up where the sums are formed again; r, y are not) for the upstream gradient dy:
  *   dense: dz = dy act'(z);                          dx = dz w;            dw = dz^T x;  db = sum over rows of dz
  *   gated: dg = dy z_up act'(z), du = dy act(z);     dx = dg w + du w_up;  dw = dg^T x, dw_up = du^T x;  db, db_up likewise

@@ -25,30 +25,29 @@ float tile_cost(long long tiles, float cost, int at_once) {
   return cost * (n + (rest ? 0.4f * (at_once - rest) / (at_once - 1) : 0.f));
 }
 
-struct Cost {
-  float small, mid, large, best;
-};
 // A layer's epilogue (BK: the products that have one) is hidden behind the other workgroups of a CU, of which the large tile leaves one: counted as 0.13 of the
 // large tile's time at 1024 k (gated bf16 24576 rows, us, large / mid: 512 x 1365 122 / 110, [dg | du] 187 / 158; 1024 x 2048 264 / 264).
 // TA: what memory holds A as: float for dz, also where T has 16 bits.  There 128 x 128 costs a quarter less than 64 x 64, and a 256 x 128 tile has no registers left.
 // (dx with its slope kernel, 128 x 128 / 64 x 64, us: bf16 24576 x 1024 x 1024 201 / 239, 4096 x 1024 x 1024 49 / 49, 1024 x 512 x 512 29 / 22;
 // fp16 237 / 292, 58 / 59, 33 / 23.)
-template <typename TA, bool BK> Cost costs(long long M, long long width, long long K, long long splits) {
+struct Choice {
+  int rows;  // the tile: 64 x 64, 128 x 128 or 256 x 128
+  float cost;
+};
+template <typename TA, bool BK> Choice choose(long long M, long long width, long long K, long long splits) {
   auto tiles = [&](int bm, int bn) { return (M + bm - 1) / bm * ((width + bn - 1) / bn) * splits; };
   constexpr bool F32 = sizeof(T) == 4, MIXED = sizeof(TA) != sizeof(T);
-  Cost c;
-  c.small = tile_cost(tiles(64, 64), F32 ? 0.166f : BK || MIXED ? 0.2f : 0.28f, F32 ? 3 : 5);
-  c.mid = tile_cost(tiles(128, 128), F32 ? 0.5f : BK ? 0.56f : 0.62f, BK ? 3 : 2);
-  c.large = F32 || MIXED ? 1e30f : tile_cost(tiles(256, 128), BK ? 1.f + 133.f / K : 1.f, 2);
-  c.best = c.large < c.mid && c.large < c.small ? c.large : c.mid < c.small ? c.mid : c.small;
-  return c;
+  const float small = tile_cost(tiles(64, 64), F32 ? 0.166f : BK || MIXED ? 0.2f : 0.28f, F32 ? 3 : 5);
+  const float mid = tile_cost(tiles(128, 128), F32 ? 0.5f : BK ? 0.56f : 0.62f, BK ? 3 : 2);
+  const float large = F32 || MIXED ? 1e30f : tile_cost(tiles(256, 128), BK ? 1.f + 133.f / K : 1.f, 2);
+  return large < mid && large < small ? Choice{256, large} : mid < small ? Choice{128, mid} : Choice{64, small};
 }
 
 template <typename TA, bool AK, bool BK, int EPI> hipError_t launch_product(const Product& p, int splits, hipStream_t st) {
-  const Cost c = costs<TA, BK>(p.M, EPI == EPI_GATED || EPI == EPI_SLOPE ? 2 * p.N : p.N, p.K, splits);
+  const int rows = choose<TA, BK>(p.M, EPI == EPI_GATED || EPI == EPI_SLOPE ? 2 * p.N : p.N, p.K, splits).rows;
   if constexpr (sizeof(TA) == 2)
-    if (c.best == c.large) return launch_tile<TA, AK, BK, 256, 128, EPI>(p, splits, st);
-  return c.best == c.mid ? launch_tile<TA, AK, BK, 128, 128, EPI>(p, splits, st) : launch_tile<TA, AK, BK, 64, 64, EPI>(p, splits, st);
+    if (rows == 256) return launch_tile<TA, AK, BK, 256, 128, EPI>(p, splits, st);
+  return rows == 128 ? launch_tile<TA, AK, BK, 128, 128, EPI>(p, splits, st) : launch_tile<TA, AK, BK, 64, 64, EPI>(p, splits, st);
 }
 
 // Few rows leave most CUs idle: the sum over k is then split, each part's sums go through memory, and a second launch joins them.  The time of an unsplit unit of
@@ -57,14 +56,15 @@ template <typename TA, bool AK, bool BK, int EPI> hipError_t launch_product(cons
 template <typename TA, bool BK> int sum_splits(long long M, long long width, long long K) {
   const float per_k = sizeof(T) == 4 ? 0.08f : sizeof(TA) == 4 ? 0.042f : 0.021f;
   int best = 1;
-  float time = costs<TA, BK>(M, width, K, 1).best * K * per_k;
+  float time = choose<TA, BK>(M, width, K, 1).cost * K * per_k;
   for (int s = 2; s <= 32 && K / s >= 128; s *= 2) {
-    const float t = costs<TA, BK>(M, width, K, s).best * K / s * per_k + 4.f + 4e-6f * M * width * s * 0.67f;
+    const float t = choose<TA, BK>(M, width, K, s).cost * K / s * per_k + 4.f + 4e-6f * M * width * s * 0.67f;
     if (t < time) { time = t; best = s; }
   }
   return best;
 }
 long long per_split(long long K, int splits) { return ((K + splits - 1) / splits + 63) / 64 * 64; }
+int parts(long long K, int splits) { return (int)((K + per_split(K, splits) - 1) / per_split(K, splits)); }
 
 // How many ways the sum over the rows is split in dw = dz^T x: few tiles, many rows.
 int weight_splits(long long out, long long in, long long rows) {
@@ -93,8 +93,7 @@ Plan plan(const mjlab_layer_grad_t* g) {
   q.again = q.gated && !f.z;
   q.blocks = (f.rows + SLOPE_ROWS - 1) / SLOPE_ROWS;
   if (q.again) {  // two sets of column sums per tile of rows
-    const Cost c = costs<T, true>(f.rows, 2 * f.out, f.in, 1);
-    const int bm = c.best == c.large ? 256 : c.best == c.mid ? 128 : 64;
+    const int bm = choose<T, true>(f.rows, 2 * f.out, f.in, 1).rows;
     q.blocks = 2 * ((f.rows + bm - 1) / bm);
   }
   q.splits = weight_splits(q.ns * f.out, f.in, f.rows);
@@ -131,7 +130,7 @@ template <typename TA> hipError_t input_gradient(const mjlab_layer_grad_t* g, co
   p.y = g->dx; p.ldy = f.in; p.partial = partial;
   if (q.x_splits == 1) return launch_product<TA, true, false, EPI_STORE>(p, 1, st);
   p.ksplit = per_split(p.K, q.x_splits);
-  const int splits = (int)((p.K + p.ksplit - 1) / p.ksplit);
+  const int splits = parts(p.K, q.x_splits);
   const long long n = f.rows * f.in;
   if ((n + 255) / 256 > MAX_BLOCKS) return hipErrorInvalidValue;
   if (hipError_t e = launch_product<TA, true, false, EPI_PARTIAL>(p, splits, st); e != hipSuccess) return e;
@@ -145,7 +144,7 @@ template <typename TA> hipError_t weight_gradient(const mjlab_layer_grad_t* g, c
   p.A = d; p.lda = ldd; p.B = f.x; p.ldb = f.ldx;
   p.M = q.ns * f.out; p.N = p.nb2 = f.in; p.K = p.kb2 = f.rows;
   p.ksplit = per_split(f.rows, q.splits);
-  const int splits = (int)((f.rows + p.ksplit - 1) / p.ksplit);
+  const int splits = parts(f.rows, q.splits);
   p.y = g->dw; p.ldy = f.in; p.partial = partial;
   if (splits == 1 && !q.gated) return launch_product<TA, false, false, EPI_STORE>(p, 1, st);
   if (hipError_t e = launch_product<TA, false, false, EPI_PARTIAL>(p, splits, st); e != hipSuccess) return e;
@@ -172,7 +171,7 @@ hipError_t POLICY_NAME(mjlab_launch_layer_forward)(const mjlab_layer_t* f, hipSt
   q.N = f->w_up ? 2 * f->out : f->out;
   q.ksplit = per_split(f->in, s);
   q.partial = p.partial = (float*)f->workspace;
-  const int splits = (int)((f->in + q.ksplit - 1) / q.ksplit);
+  const int splits = parts(f->in, s);
   if (hipError_t e = launch_product<T, true, true, EPI_PARTIAL>(q, splits, st); e != hipSuccess) return e;
   const long long blocks = (f->rows * f->out + 255) / 256;
   if (blocks > MAX_BLOCKS) return hipErrorInvalidValue;
@@ -184,6 +183,25 @@ hipError_t POLICY_NAME(mjlab_launch_layer_forward)(const mjlab_layer_t* f, hipSt
 long long POLICY_NAME(mjlab_layer_forward_bytes)(const mjlab_layer_t* f) {
   const int s = forward_splits(f);
   return s == 1 ? 0 : up256(s * f->rows * (f->w_up ? 2 : 1) * f->out * 4);
+}
+
+int POLICY_NAME(mjlab_layer_tile_of)(const mjlab_layer_t* f, int product) {
+  mjlab_layer_grad_t g = {};
+  g.f = *f; g.dx = g.dw = (void*)1;  // (only asked for being there)
+  const Plan q = plan(&g);
+  if (product == MJLAB_PRODUCT_FORWARD) {
+    const int s = forward_splits(f);
+    const int rows = choose<T, true>(f->rows, q.ns * f->out, f->in, s == 1 ? 1 : parts(f->in, s)).rows;
+    return s == 1 ? rows : -rows;
+  }
+  if (product == MJLAB_PRODUCT_INPUT) {
+    const long long k = q.ns * f->out, s = q.x_splits == 1 ? 1 : parts(k, q.x_splits);
+    const int rows = q.slope ? choose<float, false>(f->rows, f->in, k, s).rows : choose<T, false>(f->rows, f->in, k, s).rows;
+    return q.x_splits == 1 ? rows : -rows;
+  }
+  const int s = parts(f->rows, q.splits);
+  const int rows = q.slope ? choose<float, false>(q.ns * f->out, f->in, f->rows, s).rows : choose<T, false>(q.ns * f->out, f->in, f->rows, s).rows;
+  return s == 1 && !q.gated ? rows : -rows;
 }
 
 long long POLICY_NAME(mjlab_layer_backward_bytes)(const mjlab_layer_grad_t* g) { return plan(g).bytes; }

@@ -1,4 +1,4 @@
-// policy.hip -- C ABI of include/mjlab_policy.h: argument checks and the choice of the element type; the kernels live in layer_inst.hip.
+// policy.hip -- C ABI of include/mjlab_policy.h: argument checks and the choice of the element type; the kernels live in layer_inst.hip, decay_inst.hip and short_inst.hip.
 #include "policy_common.h"
 #include "policy_launch.h"
 
@@ -42,6 +42,11 @@ static int check_z(const mjlab_layer_t& f) {
 int mjlab_layer_recomputes(const mjlab_layer_t* f) {
   if (!f || check_layer(*f)) return 0;
   return BY_TYPE(f->dtype, mjlab_layer_again, f);
+}
+
+int mjlab_layer_tile(const mjlab_layer_t* f, int product) {
+  if (!f || product < MJLAB_PRODUCT_FORWARD || product > MJLAB_PRODUCT_WEIGHT || check_layer(*f)) return 0;
+  return BY_TYPE(f->dtype, mjlab_layer_tile_of, f, product);
 }
 
 long long mjlab_layer_forward_workspace(const mjlab_layer_t* f) {

@@ -7,6 +7,7 @@
 #define MJLAB_POLICY_DECLARE(T)                                                              \
   hipError_t mjlab_launch_layer_forward_##T(const mjlab_layer_t* f, hipStream_t st);         \
   int mjlab_layer_again_##T(const mjlab_layer_t* f);                                         \
+  int mjlab_layer_tile_of_##T(const mjlab_layer_t* f, int product);                          \
   long long mjlab_layer_forward_bytes_##T(const mjlab_layer_t* f);                           \
   long long mjlab_layer_backward_bytes_##T(const mjlab_layer_grad_t* g);                     \
   hipError_t mjlab_launch_layer_backward_##T(const mjlab_layer_grad_t* g, hipStream_t st);   \

@@ -168,7 +168,7 @@ class NativeLibraryError(RuntimeError):
 
 _POLICY_LIB: ctypes.CDLL | None = None
 
-POLICY_SYMBOLS = ("mjlab_policy_abi_version", "mjlab_policy_last_error", "mjlab_layer_recomputes", "mjlab_layer_forward_workspace", "mjlab_layer_forward", "mjlab_sizeof_layer", "mjlab_layer_backward_workspace",
+POLICY_SYMBOLS = ("mjlab_policy_abi_version", "mjlab_policy_last_error", "mjlab_layer_recomputes", "mjlab_layer_tile", "mjlab_layer_forward_workspace", "mjlab_layer_forward", "mjlab_sizeof_layer", "mjlab_layer_backward_workspace",
                   "mjlab_layer_backward", "mjlab_sizeof_layer_grad", "mjlab_decay_workspace", "mjlab_decay_forward", "mjlab_decay_backward", "mjlab_decay_step",
                   "mjlab_sizeof_decay", "mjlab_sizeof_decay_grad")  # fmt: skip
 
@@ -196,6 +196,7 @@ def policy_lib() -> ctypes.CDLL:
   L.mjlab_policy_last_error.restype = ctypes.c_char_p
   L.mjlab_layer_forward.argtypes = [vp, vp]
   L.mjlab_layer_recomputes.argtypes = [vp]
+  L.mjlab_layer_tile.argtypes = [vp, ctypes.c_int]
   for name in ("mjlab_layer_forward_workspace", "mjlab_layer_backward_workspace"):
     getattr(L, name).argtypes, getattr(L, name).restype = [vp], ctypes.c_longlong
   for name in ("mjlab_layer_backward", "mjlab_decay_forward", "mjlab_decay_backward", "mjlab_decay_step"):
