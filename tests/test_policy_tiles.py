@@ -7,6 +7,8 @@ what has 16 bits itself: not at all), and 16 u32 (1 + |z|) for an activation or 
 by itself: twelve times."""
 
 import ctypes
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -91,3 +93,16 @@ def test_every_kernel(m, k, n, name, gated, dtype):
     for i, (d, o, e) in enumerate(zip(dz, mul, off, strict=True)):
       near(rest[i], d.t() @ X, (o + 3 * m * U32**2 * d * d).t() @ (X * X), dtype, "dw")
       near(rest[len(ws) + i], d.sum(0), (e * e + m * U32**2 * d * d).sum(0), dtype, "db")
+
+
+def test_no_product_kernel_spills():
+  sys.path.insert(0, str(Path(__file__).resolve().parents[1] / "tools"))
+  import code_object
+
+  if not (code_object.LLVM / "llvm-objdump").exists():
+    pytest.skip("ROCm LLVM tools not installed")
+  native.policy_lib()
+  kernels = {n: md for n, md in code_object.kernels(native.POLICY_LIB_PATH).items() if "k_product" in n}
+  assert len(kernels) >= 78  # 16 bits: 8 products and epilogues x 3 tiles and 4 of dz x 2, of each of two types; float: 7 x 2
+  for name, md in kernels.items():
+    assert md["private_segment_fixed_size"] == 0, (name, md)
