@@ -16,7 +16,7 @@
 extern "C" {
 #endif
 
-#define MJLAB_POLICY_ABI_VERSION 1
+#define MJLAB_POLICY_ABI_VERSION 2
 
 enum { MJLAB_DTYPE_F32 = 0, MJLAB_DTYPE_F16 = 1, MJLAB_DTYPE_BF16 = 2 };
 enum { MJLAB_ACT_NONE = 0, MJLAB_ACT_RELU, MJLAB_ACT_ELU, MJLAB_ACT_TANH, MJLAB_ACT_SIGMOID, MJLAB_ACT_SILU, MJLAB_ACT_GELU, MJLAB_ACT_COUNT };
@@ -28,7 +28,7 @@ const char* mjlab_policy_last_error(void);
  *   dense (w_up == NULL):  y = act(x w^T + b) + r
  *   gated (w_up != NULL):  y = act(x w^T + b) * (x w_up^T + b_up)
  * x (rows, in), w and w_up (out, in), b and b_up (out) or NULL, r (rows, out) or NULL (dense only), y (rows, out); the innermost stride of
- * each is 1, ld* is the distance of rows.  All arrays hold `dtype`; sums are held in 32 bits and each output is rounded once.
+ * each is 1, ld* is the distance of rows.  All arrays but z hold `dtype`; sums are held in 32 bits and each output is rounded once.
  * z / z_up (rows, out), dense, or NULL: the sums before the activation, floats whatever `dtype` is (z_bytes, their element size, is 4), which the
  * backward pass reads.  z_is_y (backward pass of a float32 layer only): z points to the dense output y instead, which determines the slope of relu,
  * elu, tanh and sigmoid where no residual was added. */
@@ -57,7 +57,8 @@ int mjlab_layer_tile(const mjlab_layer_t* f, int product);
  *   dense: dz = dy act'(z);                          dx = dz w;            dw = dz^T x;  db = sum over rows of dz
  *   gated: dg = dy z_up act'(z), du = dy act(z);     dx = dg w + du w_up;  dw = dg^T x, dw_up = du^T x;  db, db_up likewise
  * (the residual's gradient is dy itself).  A dense layer without activation needs no z.  Each output is dense and may be NULL (not wanted);
- * dw / dw_up and db / db_up come together.  dz, dg and du are floats, whatever `dtype` is, and multiplied to 2^-16 (float: 2^-23) of each term.
+ * dw / dw_up and db / db_up come together.  dz, dg and du are floats, whatever `dtype` is, and the products with them hold each term to 2^-15 in 16 bits and to
+ * 2^-22 in float (terms with a factor below 2^-100 to less).
  * workspace: device memory of mjlab_layer_backward_workspace() bytes, free again when the launches have run. */
 typedef struct mjlab_layer_grad {
   mjlab_layer_t f;
@@ -77,7 +78,8 @@ int mjlab_sizeof_layer_grad(void);
  * but 1 for the innermost; dk, dv <= MJLAB_DECAY_MAX_DIM.  state (the S before token 0; NULL = 0) and state_out (S after the last token; NULL =
  * not wanted) are dense (batch, heads, dk, dv) floats and not the same memory.  reset (batch, length) of reset_bytes 1 or 4 per element, non-zero =
  * reset, or NULL.  lengths (batch) ints or NULL: sequence b ends before token lengths[b] (clamped to [0, length]); the rows of o behind it are
- * written as zeros.  A NaN or infinity reaches only the tokens that the recurrence takes it to: not earlier ones, not other episodes.
+ * written as zeros.  Weighted keys, pairs q k and the state that outputs read are held to 2^-16 in 16 bits (state_out and d_state: made of all 24).
+ * A NaN or infinity reaches only the tokens that the recurrence takes it to: not earlier ones, not other episodes.
  * workspace: mjlab_decay_workspace() bytes of device memory. */
 #define MJLAB_DECAY_MAX_DIM 128
 typedef struct mjlab_decay_rows { const void* p; long long batch, time, head; } mjlab_decay_rows_t; /* strides in elements */

@@ -26,7 +26,7 @@ float tile_cost(long long tiles, float cost, int at_once) {
 }
 
 // A layer's epilogue (BK: the products that have one) is hidden behind the other workgroups of a CU, of which the large tile leaves one: counted as 0.13 of the
-// large tile's time at 1024 k (gated bf16 24576 rows, us, large / mid: 512 x 1365 122 / 110, [dg | du] 187 / 158; 1024 x 2048 264 / 264).
+// large tile's time at 1024 k (gated bf16 24576 rows, y, us, large / mid: 512 x 1365 122 / 110; 1024 x 2048 264 / 264).
 // TA: what memory holds A as: float for dz, also where T has 16 bits.  There 128 x 128 costs a quarter less than 64 x 64, and a 256 x 128 tile has no registers left.
 // (dx with its slope kernel, 128 x 128 / 64 x 64, us: bf16 24576 x 1024 x 1024 201 / 239, 4096 x 1024 x 1024 49 / 49, 1024 x 512 x 512 29 / 22;
 // fp16 237 / 292, 58 / 59, 33 / 23.)

@@ -117,7 +117,7 @@ POLICY_LIB_PATH = Path(os.environ.get("MJLAB_POLICY_LIB", CSRC / "libmjlab_polic
 POLICY_CSRC = CSRC / "policy"
 POLICY_HEADER = Path(__file__).parents[1] / "include" / "mjlab_policy.h"
 POLICY_UNITS = ("layer_inst.hip", "decay_inst.hip", "short_inst.hip")  # compiled once per element type
-POLICY_ABI_VERSION = 1  # include/mjlab_policy.h MJLAB_POLICY_ABI_VERSION
+POLICY_ABI_VERSION = 2  # include/mjlab_policy.h MJLAB_POLICY_ABI_VERSION
 # packed fp32 instructions off: these kernels are written for plain ones
 POLICY_HIPCC_FLAGS = [*HIPCC_FLAGS, "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 

@@ -5,8 +5,9 @@
   decay_attention(q, k, v, log_decay, ...)       S_t = decay S_{t-1} + k_t v_t^T, o_t = scale q_t S_t over stored steps, S cut at resets
   decay_attention_step(q, k, v, log_decay, state, ...)  the same for one control step
 
-float32, float16 or bfloat16, the same type everywhere, sums and states in 32 bits, each output rounded once.  The first three are
-differentiable (once) in every tensor argument but log_decay.  Every call enqueues on torch's current stream of
+float32, float16 or bfloat16, the same type everywhere, sums and states in 32 bits, each output and gradient rounded once: what lies between them is held to 2^-15
+or better of each term of a sum, and has a float's range (a float16 layer's upstream gradient may be tiny, or its product with the slope beyond 65504).  The first
+three are differentiable once, in reverse mode (no vmap, no forward mode), in every tensor argument but log_decay.  Every call enqueues on torch's current stream of
 the tensors' device and may be captured into a hipGraph; nothing synchronises.  The last dimension of an argument must be contiguous, rows may
 be any distance apart.  No fallback: without the HIP library, or for a tensor that is not on the GPU, these raise.
 
